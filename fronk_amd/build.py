@@ -10,24 +10,35 @@ libfr_hip.so         the "hip" fr_backend vtable (host/hip.c, plain C11),
 """
 import os
 import subprocess
+from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
-HIP_SRC = os.path.join(HERE, "csrc", "fronk_hip.hip")
+# The expert engine, and the dense operators around it.
+HIP_SRCS = [os.path.join(HERE, "csrc", n) for n in ("fronk_hip.hip", "delta.hip", "q4.hip", "kv.hip")]
 HIP_LIB = os.path.join(HERE, "libfronk_hip.so")
 VTABLE_SRC = os.path.join(HERE, "host", "hip.c")
 VTABLE_LIB = os.path.join(HERE, "libfr_hip.so")
 REFERENCE_SRC = os.path.join(os.environ.get("FRONK_REFERENCE", "/root/reference"), "src")
 
 # Packed-FP32 instructions are disabled for every HIP translation unit.
-HIPCC_FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-shared",
+HIPCC_FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC",
                "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
                "-I" + os.path.join(ROOT, "include")]
 
 
 def build_hip(verbose=False):
-    cmd = ["hipcc", *HIPCC_FLAGS, HIP_SRC, "-o", HIP_LIB + ".tmp"]
-    subprocess.run(cmd, check=True, capture_output=not verbose)
+    """One object per source, compiled side by side, and one library of them."""
+    def compile_one(src):
+        obj = src + ".o"
+        subprocess.run(["hipcc", *HIPCC_FLAGS, "-c", src, "-o", obj], check=True, capture_output=not verbose)
+        return obj
+    with ThreadPoolExecutor(len(HIP_SRCS)) as pool:
+        objs = list(pool.map(compile_one, HIP_SRCS))
+    subprocess.run(["hipcc", "--offload-arch=gfx950", "-shared", *objs, "-o", HIP_LIB + ".tmp"], check=True,
+                   capture_output=not verbose)
+    for obj in objs:
+        os.remove(obj)
     os.replace(HIP_LIB + ".tmp", HIP_LIB)
     return HIP_LIB
 

@@ -1,0 +1,658 @@
+// kv.hip - the paged 8-bit key/value cache: written (fr_hip_kv_append), read
+// back (fr_hip_kv_read) and attended to (fr_hip_kv_attend).
+#include <limits.h>
+#include <math.h>
+
+#include "bounds.h"
+#include "dense.h"
+
+namespace {
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+struct Cache {
+  uint8_t *k_codes, *v_codes, *k_exp, *v_exp;
+  uint32_t pages, heads, page, dim;
+};
+
+__device__ __forceinline__ size_t exp_at(const Cache& C, uint32_t page, uint32_t head, uint32_t at) {
+  return fronk::exp_at(C.heads, C.page, page, head, at);
+}
+__device__ __forceinline__ size_t v_at(const Cache& C, uint32_t page, uint32_t head, uint32_t at) {
+  return fronk::v_at(C.heads, C.page, C.dim, page, head, at);
+}
+
+__device__ __forceinline__ uint32_t umax_rotate(uint32_t x) {
+  uint32_t y = max(x, __builtin_bit_cast(uint32_t, row_rotate<1>(__builtin_bit_cast(float, x))));
+  y = max(y, __builtin_bit_cast(uint32_t, row_rotate<2>(__builtin_bit_cast(float, y))));
+  y = max(y, __builtin_bit_cast(uint32_t, row_rotate<4>(__builtin_bit_cast(float, y))));
+  return max(y, __builtin_bit_cast(uint32_t, row_rotate<8>(__builtin_bit_cast(float, y))));
+}
+
+// 2^(e - 127) of an exponent byte; 255 (a vector with a non-finite value) is
+// infinity, which makes NaN of its zero codes.
+__device__ __forceinline__ float power(uint32_t e) { return __builtin_bit_cast(float, e << 23); }
+
+struct KvArgs {
+  Cache cache;
+  void *k, *v;
+  const int32_t* slot;
+  uint32_t* status;
+  int64_t k_token, k_head, v_token, v_head;
+  uint32_t tokens;
+  bool wide;
+};
+
+__device__ __forceinline__ int place(const KvArgs& A, uint32_t t, uint32_t* page, uint32_t* at) {
+  return fronk::locate(A.slot[t], A.cache.page, A.cache.pages, page, at);
+}
+
+// One vector (token, head, k or v) to D / 4 lanes, four values each.
+template <typename T, int D>
+__global__ __launch_bounds__(256) void kv_append(KvArgs A) {
+  constexpr uint32_t L = D / 4;
+  const uint64_t item = ((uint64_t)blockIdx.x * 256 + threadIdx.x) / L;
+  const uint32_t lane = threadIdx.x % L;
+  const uint32_t h = (uint32_t)(item / 2 % A.cache.heads);
+  const uint64_t t = item / 2 / A.cache.heads;
+  const bool is_v = item & 1;
+  if (t >= A.tokens) return;   // whole rows of 16 lanes: their reductions stay whole
+  uint32_t page, at;
+  const int there = place(A, (uint32_t)t, &page, &at);
+  if (there != 1) {
+    if (there == 2 && A.status && lane == 0) atomicOr(A.status, FR_HIP_BAD_SLOT);
+    return;
+  }
+  const T* src = is_v ? static_cast<const T*>(A.v) + (int64_t)t * A.v_token + h * A.v_head
+                      : static_cast<const T*>(A.k) + (int64_t)t * A.k_token + h * A.k_head;
+  float x[4];
+  load_row<4>(src + lane * 4, A.wide, x);
+  // The largest magnitude as bits, which order like it and put infinity and
+  // NaN on top.
+  uint32_t top = 0;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) top = max(top, __builtin_bit_cast(uint32_t, x[e]) & 0x7fffffffu);
+  top = umax_rotate(top);
+  if constexpr (L > 16) top = max(top, (uint32_t)__shfl_xor((int)top, 16));
+  if constexpr (L > 32) top = max(top, (uint32_t)__shfl_xor((int)top, 32));
+  const bool finite = top < 0x7f800000u;
+  const int raw = (int)(top >> 23) - 8 + ((top & 0x7fffffu) > 0x600000u);
+  const uint32_t e = finite ? (uint32_t)max(raw, 1) : 255u;
+  const float m = finite ? __builtin_bit_cast(float, (254u - e) << 23) : 0.f;
+  uint32_t codes = 0;
+  if (finite) {
+    codes = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(x[0] * m, x[1] * m, 0, false);
+    codes = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(x[2] * m, x[3] * m, (int)codes, true);
+  }
+  const Cache& C = A.cache;
+  if (is_v) {
+    uint8_t* out = C.v_codes + v_at(C, page, h, at) + lane * 64;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) out[16 * i] = (uint8_t)(codes >> (8 * i));
+  } else {
+    *reinterpret_cast<uint32_t*>(C.k_codes + exp_at(C, page, h, at) * D + lane * 4) = codes;
+  }
+  if (lane == 0) (is_v ? C.v_exp : C.k_exp)[exp_at(C, page, h, at)] = (uint8_t)e;
+}
+
+template <typename T, int D>
+__global__ __launch_bounds__(256) void kv_read(KvArgs A) {
+  constexpr uint32_t L = D / 4;
+  const uint64_t item = ((uint64_t)blockIdx.x * 256 + threadIdx.x) / L;
+  const uint32_t lane = threadIdx.x % L;
+  const uint32_t h = (uint32_t)(item / 2 % A.cache.heads);
+  const uint64_t t = item / 2 / A.cache.heads;
+  const bool is_v = item & 1;
+  if (t >= A.tokens || !(is_v ? A.v : A.k)) return;
+  uint32_t page = 0, at = 0;
+  const int there = place(A, (uint32_t)t, &page, &at);
+  if (there == 2 && A.status && lane == 0) atomicOr(A.status, FR_HIP_BAD_SLOT);
+  const Cache& C = A.cache;
+  uint32_t codes = 0;
+  float m = 0;
+  if (there == 1) {
+    if (is_v) {
+      const uint8_t* in = C.v_codes + v_at(C, page, h, at) + lane * 64;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) codes |= (uint32_t)in[16 * i] << (8 * i);
+    } else {
+      codes = *reinterpret_cast<const uint32_t*>(C.k_codes + exp_at(C, page, h, at) * D + lane * 4);
+    }
+    m = power((is_v ? C.v_exp : C.k_exp)[exp_at(C, page, h, at)]);
+  }
+  T* out = is_v ? static_cast<T*>(A.v) + (int64_t)t * A.v_token + h * A.v_head
+                : static_cast<T*>(A.k) + (int64_t)t * A.k_token + h * A.k_head;
+  const auto a = __builtin_amdgcn_cvt_pk_f32_fp8(codes, false), b = __builtin_amdgcn_cvt_pk_f32_fp8(codes, true);
+  typedef T vec __attribute__((ext_vector_type(4)));
+  const vec y = {(T)(a[0] * m), (T)(a[1] * m), (T)(b[0] * m), (T)(b[1] * m)};
+  if (A.wide) {
+    *reinterpret_cast<vec*>(out + lane * 4) = y;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) out[lane * 4 + i] = y[i];
+  }
+}
+
+// ------------------------------------------------------------------- attend
+//
+// One workgroup: one sequence, one cache head, 16 RT rows (query heads of that
+// cache head by tokens of the burst) and one stretch of the context; each of
+// its four wavefronts takes every fourth tile of 64 tokens with a running
+// maximum and sum of its own, joined through LDS at the end. Stretches are
+// joined by kv_merge.
+//
+// Both products are formed transposed, S^T = K Q^T and O^T = V^T P^T, so that a
+// lane's column is one query row throughout: the row's maximum, sum and
+// rescaling are the lane's own scalars (joined over the four lane rows), and P
+// goes from the first product's result into the second's B operand without
+// leaving the registers. That fixes which tokens a lane holds: row m of K tile
+// t is token 16 (m / 4) + 4 t + m % 4, so that lane row j ends up with tokens
+// 16 j .. 16 j + 15, the sixteen bytes that the cache's V blocks keep together.
+//
+// Codes times one are exact in bf16 and fp16. Q is an exact operand too (fp32:
+// three bf16 parts); P 2^e is fp32 in two bf16 parts (error 2^-17 of it, below
+// a 16-bit output's own rounding), three for fp32 outputs.
+struct AttendArgs {
+  Cache cache;
+  const void* q;
+  void* o;
+  float *part_o, *part_ml;       // [item][split][16 RT][D], [item][split][16 RT][2]
+  const int32_t *table, *length;
+  uint32_t* status;
+  int64_t q_token, q_head, o_token, o_head;
+  uint32_t sequences, burst, heads, per, max_context, table_stride, splits, chunk, row_blocks;
+  float scale;
+  bool wide;
+};
+
+template <typename T> struct Query {
+  typedef bf16x8 frag;
+  static constexpr int kParts = 1, kP = 2;
+};
+template <> struct Query<_Float16> {
+  typedef half8v frag;
+  static constexpr int kParts = 1, kP = 2;
+};
+template <> struct Query<float> {
+  typedef bf16x8 frag;
+  static constexpr int kParts = 3, kP = 3;
+};
+
+// Eight e4m3 codes as an operand, exactly.
+__device__ __forceinline__ bf16x8 codes8(uint32_t lo, uint32_t hi, bf16x8) {
+  const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.f, false), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.f, true);
+  const bf16x2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.f, false), d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.f, true);
+  return {a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+__device__ __forceinline__ half8v codes8(uint32_t lo, uint32_t hi, half8v) {
+  const half2v a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.f, false), b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.f, true);
+  const half2v c = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.f, false), d = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.f, true);
+  return {a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+
+// x as `N` bf16 parts whose sum it is (up to 2^-8N of it).
+template <int N> __device__ __forceinline__ void split8(const float (&x)[8], bf16x8 (&out)[N]) {
+  float rest[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) rest[e] = x[e];
+#pragma unroll
+  for (int p = 0; p < N; ++p)
+#pragma unroll
+    for (int e = 0; e < 8; e += 2) {
+      const bf16x2 h = to_bf16(rest[e], rest[e + 1]);
+      out[p][e] = h[0], out[p][e + 1] = h[1];
+      if (p + 1 < N) rest[e] -= (float)h[0], rest[e + 1] -= (float)h[1];
+    }
+}
+
+template <typename T, int D, int RT>
+__global__ __launch_bounds__(256) void kv_attend(AttendArgs A) {
+  typedef Query<T> Q;
+  typedef typename Q::frag frag;
+  constexpr int QP = Q::kParts, PP = Q::kP, KS = D / 32, SEG = D / 64, DT = D / 16, R = 16 * RT;
+  constexpr int kPad = D + 4;
+  __shared__ union {
+    uint4v q[RT][QP][KS][64];
+    float o[R][kPad];
+  } sh;
+  __shared__ float stat[4][R][2];
+  const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, j = lane >> 4;
+  const uint32_t split = blockIdx.x % A.splits, item = blockIdx.x / A.splits;
+  const uint32_t rb = item % A.row_blocks, head = item / A.row_blocks % A.cache.heads;
+  const uint32_t seq = item / A.row_blocks / A.cache.heads;
+  const uint32_t rows = A.burst * A.per, row0 = rb * R;
+
+  int32_t len = A.length[seq];
+  if (len < 0 || (uint32_t)len > A.max_context) {
+    if (A.status && threadIdx.x == 0) atomicOr(A.status, FR_HIP_BAD_LENGTH);
+    len = 0;
+  }
+  const uint32_t begin = split * A.chunk;
+  const uint32_t end = min((uint32_t)len, begin + A.chunk);   // chunk * splits < 2^31
+
+  // Q, by operand: step ks of lane (i, j) holds dims 64 (ks / 2) + 16 j + 8 (ks % 2) ..
+  if (begin < end) {
+    for (uint32_t f = wave; f < RT * KS; f += 4) {
+      const uint32_t rt = f / KS, ks = f % KS, row = row0 + rt * 16 + i;
+      const uint32_t d = ks / 2 * 64 + j * 16 + ks % 2 * 8;
+      float v[8] = {};
+      if (row < rows) {
+        const T* p = static_cast<const T*>(A.q) + (int64_t)(seq * A.burst + row / A.per) * A.q_token +
+                     (int64_t)(head * A.per + row % A.per) * A.q_head + d;
+        load_row<8>(p, A.wide, v);
+      }
+      if constexpr (QP == 3) {
+        bf16x8 parts[3];
+        split8<3>(v, parts);
+#pragma unroll
+        for (int p = 0; p < 3; ++p) sh.q[rt][p][ks][lane] = __builtin_bit_cast(uint4v, parts[p]);
+      } else {
+        frag one;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) one[e] = (decltype(one[0] + one[0]))v[e];
+        sh.q[rt][0][ks][lane] = __builtin_bit_cast(uint4v, one);
+      }
+    }
+  }
+  __syncthreads();
+
+  uint32_t limit[RT];   // the tokens that this lane's row sees
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    const uint32_t row = row0 + rt * 16 + i;
+    const int32_t n = len - (int32_t)A.burst + (int32_t)(row / A.per) + 1;
+    limit[rt] = row < rows && n > 0 ? (uint32_t)n : 0;
+  }
+  float top[RT], sum[RT];
+  float4v acc[RT][DT];
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    top[rt] = -INFINITY, sum[rt] = 0;
+#pragma unroll
+    for (int d = 0; d < DT; ++d) acc[rt][d] = float4v{0, 0, 0, 0};
+  }
+  const Cache& C = A.cache;
+  const float scale = A.scale * kLog2e;
+
+  for (uint32_t base = begin + wave * 64; base < end; base += 256) {
+    // The lane's block of 16 tokens for K (by its row) and for V (by j).
+    const uint32_t tk = base + (i >> 2) * 16, tv = base + j * 16;
+    const uint32_t pk = tk / C.page, pv = tv / C.page;
+    int32_t page_k = -1, page_v = -1;
+    if (tk < end) page_k = A.table[(size_t)seq * A.table_stride + pk];
+    if (tv < end) page_v = A.table[(size_t)seq * A.table_stride + pv];
+    const bool ok_k = fronk::page_there(page_k, C.pages), ok_v = fronk::page_there(page_v, C.pages);
+    if (tv < end && !ok_v && A.status) atomicOr(A.status, FR_HIP_BAD_PAGE);
+    uint4v kc[4][SEG], vc[DT], ke = {0, 0, 0, 0}, ve = {0, 0, 0, 0};
+    {
+      const uint8_t* p = C.k_codes + (ok_k ? exp_at(C, (uint32_t)page_k, head, tk - pk * C.page + (i & 3)) * D : 0) + j * 16;
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int s = 0; s < SEG; ++s) {
+          kc[t][s] = uint4v{0, 0, 0, 0};
+          if (ok_k) kc[t][s] = *reinterpret_cast<const uint4v*>(p + t * 4 * D + s * 64);
+        }
+    }
+    {
+      const size_t e = ok_v ? exp_at(C, (uint32_t)page_v, head, tv - pv * C.page) : 0;
+      if (ok_v) ke = *reinterpret_cast<const uint4v*>(C.k_exp + e), ve = *reinterpret_cast<const uint4v*>(C.v_exp + e);
+      const uint8_t* p = C.v_codes + e * D + i * 16;
+#pragma unroll
+      for (int d = 0; d < DT; ++d) {
+        vc[d] = uint4v{0, 0, 0, 0};
+        if (ok_v) vc[d] = *reinterpret_cast<const uint4v*>(p + d * 256);
+      }
+    }
+    // What lies past the end in a page was never written: its codes may be
+    // NaN, which no zero weight would take away.
+    if (base + 64 > end) {
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const uint32_t mask = fronk::first_bytes((int)end - (int)(tv + 4 * w));
+#pragma unroll
+        for (int d = 0; d < DT; ++d) vc[d][w] &= mask;
+      }
+    }
+
+    float4v st[RT][4] = {};
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      frag qf[RT][QP];
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+        for (int p = 0; p < QP; ++p) qf[rt][p] = __builtin_bit_cast(frag, sh.q[rt][p][ks][lane]);
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        const frag a = codes8(kc[t][ks / 2][ks % 2 * 2], kc[t][ks / 2][ks % 2 * 2 + 1], frag{});
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+          for (int p = QP - 1; p >= 0; --p) st[rt][t] = mma(a, qf[rt][p], st[rt][t]);
+      }
+    }
+
+    bf16x8 pf[RT][2][PP];
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      float now = -INFINITY;
+      bool seen[4][4];
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          seen[t][r] = ok_v && tv + 4 * t + r < limit[rt];
+          const float x = st[rt][t][r] * power(ke[t] >> (8 * r) & 255) * scale;
+          st[rt][t][r] = seen[t][r] ? x : -INFINITY;
+          now = fmaxf(now, st[rt][t][r]);
+        }
+      now = fmaxf(top[rt], max_xor32(max_xor16(now)));
+      const float base_m = now == -INFINITY ? 0.f : now;
+      const float alpha = __builtin_amdgcn_exp2f(top[rt] - base_m);
+      top[rt] = now;
+      float total = 0, w[2][8];
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float p = __builtin_amdgcn_exp2f(st[rt][t][r] - base_m);
+          total += p;
+          w[t / 2][t % 2 * 4 + r] = seen[t][r] ? p * power(ve[t] >> (8 * r) & 255) : 0.f;
+        }
+      sum[rt] = sum[rt] * alpha + total;
+      split8<PP>(w[0], pf[rt][0]);
+      split8<PP>(w[1], pf[rt][1]);
+      if (__any(alpha != 1.f)) {
+#pragma unroll
+        for (int d = 0; d < DT; ++d) acc[rt][d] *= alpha;
+      }
+    }
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        const bf16x8 a = codes8(vc[d][s * 2], vc[d][s * 2 + 1], bf16x8{});
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+          for (int p = PP - 1; p >= 0; --p) acc[rt][d] = mma(a, pf[rt][s][p], acc[rt][d]);
+      }
+  }
+
+  // Join the four wavefronts.
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    sum[rt] = add_xor32(add_xor16(sum[rt]));
+    if (j == 0) stat[wave][rt * 16 + i][0] = top[rt], stat[wave][rt * 16 + i][1] = sum[rt];
+  }
+  __syncthreads();   // also: Q is read no more
+  float all[RT], denom[RT];
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    const uint32_t row = rt * 16 + i;
+    all[rt] = fmaxf(fmaxf(stat[0][row][0], stat[1][row][0]), fmaxf(stat[2][row][0], stat[3][row][0]));
+    const float m = all[rt] == -INFINITY ? 0.f : all[rt];
+    denom[rt] = 0;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) denom[rt] += stat[w][row][1] * __builtin_amdgcn_exp2f(stat[w][row][0] - m);
+    const float f = __builtin_amdgcn_exp2f(top[rt] - m);
+#pragma unroll
+    for (int d = 0; d < DT; ++d) acc[rt][d] *= f;
+  }
+  for (uint32_t w = 0; w < 4; ++w) {
+    if (w == wave) {
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+        for (int d = 0; d < DT; ++d) {
+          float4v* p = reinterpret_cast<float4v*>(&sh.o[rt * 16 + i][d * 16 + 4 * j]);
+          *p = w ? *p + acc[rt][d] : acc[rt][d];
+        }
+    }
+    __syncthreads();
+  }
+  if (A.splits > 1) {
+    const size_t at = ((size_t)item * A.splits + split) * R;
+    if (wave == 0 && j == 0) {
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) {
+        A.part_ml[(at + rt * 16 + i) * 2] = all[rt];
+        A.part_ml[(at + rt * 16 + i) * 2 + 1] = denom[rt];
+      }
+    }
+    if (begin < end)   // kv_merge reads no sums of an empty stretch
+      for (uint32_t e = threadIdx.x; e < R * D / 4; e += 256) {
+        const uint32_t row = e / (D / 4), d = e % (D / 4) * 4;
+        *reinterpret_cast<float4v*>(A.part_o + (at + row) * D + d) = *reinterpret_cast<float4v*>(&sh.o[row][d]);
+      }
+    return;
+  }
+  if (wave == 0 && j == 0) {
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) stat[0][rt * 16 + i][0] = denom[rt];
+  }
+  __syncthreads();
+  for (uint32_t e = threadIdx.x; e < R * D; e += 256) {
+    const uint32_t r = e / D, d = e % D, row = row0 + r;
+    if (row >= rows) break;
+    const float l = stat[0][r][0];
+    T* out = static_cast<T*>(A.o) + (int64_t)(seq * A.burst + row / A.per) * A.o_token +
+             (int64_t)(head * A.per + row % A.per) * A.o_head;
+    out[d] = (T)(l == 0.f ? 0.f : sh.o[r][d] / l);
+  }
+}
+
+// The stretches of one row joined, in their order.
+template <typename T, int D>
+__global__ __launch_bounds__(256) void kv_merge(AttendArgs A, uint32_t R) {
+  constexpr uint32_t L = D / 4, G = 256 / L;
+  __shared__ float weight[256], red[4];
+  __shared__ float4v part[G][L];
+  const uint32_t rows = A.burst * A.per;
+  const uint32_t row = blockIdx.x % rows, head = blockIdx.x / rows % A.cache.heads, seq = blockIdx.x / rows / A.cache.heads;
+  const uint32_t item = (seq * A.cache.heads + head) * A.row_blocks + row / R, at = row % R;
+  const uint32_t s = threadIdx.x, wave = s >> 6;
+  float m = -INFINITY, l = 0;
+  if (s < A.splits) {
+    const float* p = A.part_ml + (((size_t)item * A.splits + s) * R + at) * 2;
+    m = p[0], l = p[1];
+  }
+  float top = m;
+  for (int o = 1; o < 64; o *= 2) top = fmaxf(top, __shfl_xor(top, o));
+  if ((s & 63) == 0) red[wave] = top;
+  __syncthreads();
+  top = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+  if (top == -INFINITY) top = 0.f;
+  const float f = __builtin_amdgcn_exp2f(m - top);   // 0 for an empty stretch
+  weight[s] = f;
+  l *= f;
+  for (int o = 1; o < 64; o *= 2) l += __shfl_xor(l, o);
+  __syncthreads();
+  if ((s & 63) == 0) red[wave] = l;
+  __syncthreads();
+  l = (red[0] + red[1]) + (red[2] + red[3]);
+  const uint32_t c = threadIdx.x % L, g = threadIdx.x / L;
+  float4v x = {0, 0, 0, 0};
+  for (uint32_t k = g; k < A.splits; k += G) {
+    const float w = weight[k];
+    if (w != 0.f) x += w * *reinterpret_cast<const float4v*>(A.part_o + (((size_t)item * A.splits + k) * R + at) * D + c * 4);
+  }
+  part[g][c] = x;
+  __syncthreads();
+  if (g) return;
+  for (uint32_t k = 1; k < G; ++k) x += part[k][c];
+  T* out = static_cast<T*>(A.o) + (int64_t)(seq * A.burst + row / A.per) * A.o_token +
+           (int64_t)(head * A.per + row % A.per) * A.o_head + c * 4;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) out[e] = (T)(l == 0.f ? 0.f : x[e] / l);
+}
+
+// ---------------------------------------------------------------------- host
+
+int check_cache(const fr_hip_kv_cache* c, unsigned type) {
+  if (type > FR_HIP_BF16 || !c->pages || !c->heads || !c->page || !c->dim) return FR_HIP_INVALID;
+  if (!c->k_codes || !c->v_codes || !c->k_exp || !c->v_exp) return FR_HIP_INVALID;
+  if (((uintptr_t)c->k_codes | (uintptr_t)c->v_codes | (uintptr_t)c->k_exp | (uintptr_t)c->v_exp) % 16) return FR_HIP_INVALID;
+  if ((c->dim != 64 && c->dim != 128 && c->dim != 256) || c->page % 16 || c->page > 4096) return FR_HIP_UNSUPPORTED;
+  if ((uint64_t)c->pages * c->page > INT_MAX || c->heads > 1024) return FR_HIP_UNSUPPORTED;
+  return FR_HIP_OK;
+}
+
+Cache cache_of(const fr_hip_kv_cache& c) {
+  return Cache{c.k_codes, c.v_codes, c.k_exp, c.v_exp, c.pages, c.heads, c.page, c.dim};
+}
+
+bool rows_wide(unsigned type, const void* k, const void* v, int64_t a, int64_t b, int64_t c, int64_t d) {
+  const int64_t n = 16 / (int64_t)elem_size(type);
+  return ((uintptr_t)k | (uintptr_t)v) % 16 == 0 && a % n == 0 && b % n == 0 && c % n == 0 && d % n == 0;
+}
+
+int check_tokens(const fr_hip_kv_cache* c, unsigned tokens, unsigned type, const void* k, const void* v, bool both,
+                 const int32_t* slot) {
+  const int rc = check_cache(c, type);
+  if (rc == FR_HIP_INVALID) return rc;
+  if (tokens > INT_MAX || (tokens && (!slot || (both ? !k || !v : !k && !v)))) return FR_HIP_INVALID;
+  if (((uintptr_t)k | (uintptr_t)v) % elem_size(type)) return FR_HIP_INVALID;
+  if (rc) return rc;
+  return (uint64_t)tokens * c->heads * 2 * (c->dim / 4) / 256 >= INT_MAX ? FR_HIP_UNSUPPORTED : FR_HIP_OK;
+}
+
+template <typename T, bool READ>
+void launch_tokens(const KvArgs& A, hipStream_t s) {
+  const uint64_t threads = (uint64_t)A.tokens * A.cache.heads * 2 * (A.cache.dim / 4);
+  const dim3 grid((uint32_t)((threads + 255) / 256)), block(256);
+  switch (A.cache.dim) {
+    case 64: hipLaunchKernelGGL((READ ? kv_read<T, 64> : kv_append<T, 64>), grid, block, 0, s, A); break;
+    case 128: hipLaunchKernelGGL((READ ? kv_read<T, 128> : kv_append<T, 128>), grid, block, 0, s, A); break;
+    default: hipLaunchKernelGGL((READ ? kv_read<T, 256> : kv_append<T, 256>), grid, block, 0, s, A); break;
+  }
+}
+
+template <bool READ>
+int tokens_call(const KvArgs& A, unsigned type, void* stream) {
+  hipStream_t s;
+  unsigned cus;
+  const int rc = fronk::enter(stream, &s, &cus);
+  if (rc || !A.tokens) return rc;
+  switch (type) {
+    case FR_HIP_F32: launch_tokens<float, READ>(A, s); break;
+    case FR_HIP_F16: launch_tokens<_Float16, READ>(A, s); break;
+    default: launch_tokens<__bf16, READ>(A, s); break;
+  }
+  FRONK_CK(hipGetLastError());
+  return FR_HIP_OK;
+}
+
+int check_query(const fr_hip_kv_query* r) {
+  if (!r) return FR_HIP_INVALID;
+  const int rc = check_cache(&r->cache, r->type);
+  if (rc == FR_HIP_INVALID) return rc;
+  if (!r->burst || !r->heads || r->heads % r->cache.heads || !isfinite(r->scale)) return FR_HIP_INVALID;
+  if (r->sequences && (!r->q || !r->o || !r->length || !r->table)) return FR_HIP_INVALID;
+  if (((uintptr_t)r->q | (uintptr_t)r->o) % elem_size(r->type)) return FR_HIP_INVALID;
+  if (r->max_context > INT_MAX - (1u << 20)) return FR_HIP_INVALID;
+  if (r->table_stride < (r->max_context + r->cache.page - 1) / r->cache.page) return FR_HIP_INVALID;
+  if (rc) return rc;
+  if (r->burst > 8 || r->heads / r->cache.heads > 64) return FR_HIP_UNSUPPORTED;
+  if ((uint64_t)r->sequences * r->burst * r->heads > INT_MAX / 256) return FR_HIP_UNSUPPORTED;
+  return FR_HIP_OK;
+}
+
+// How a call is cut: row tiles of a workgroup, blocks of rows, stretches.
+struct Cut {
+  uint32_t rt, row_blocks, splits, chunk;
+  uint64_t items;
+  size_t bytes;
+};
+Cut cut_of(const fr_hip_kv_query* r) {
+  Cut c;
+  const uint32_t rows = r->burst * (r->heads / r->cache.heads);
+  c.rt = rows > 16 ? 2 : 1;
+  c.row_blocks = (rows + 16 * c.rt - 1) / (16 * c.rt);
+  c.items = (uint64_t)r->sequences * r->cache.heads * c.row_blocks;
+  // About two workgroups for each of 256 compute units, none with less than a
+  // tile for each of its wavefronts.
+  const uint64_t want = c.items ? (512 + c.items - 1) / c.items : 1, most = (r->max_context + 255) / 256;
+  uint64_t n = want < most ? want : most;
+  n = n < 1 ? 1 : n > 256 ? 256 : n;
+  c.chunk = (uint32_t)((r->max_context + n * 256 - 1) / (n * 256)) * 256;
+  if (!c.chunk) c.chunk = 256;
+  c.splits = (r->max_context + c.chunk - 1) / c.chunk;
+  if (!c.splits) c.splits = 1;
+  c.bytes = c.splits > 1 ? (size_t)c.items * c.splits * 16 * c.rt * (r->cache.dim + 2) * sizeof(float) : 0;
+  return c;
+}
+
+template <typename T, int D>
+void launch_attend(const AttendArgs& A, const Cut& c, hipStream_t s) {
+  const dim3 grid((uint32_t)(c.items * c.splits)), block(256);
+  if (c.rt == 1) hipLaunchKernelGGL((kv_attend<T, D, 1>), grid, block, 0, s, A);
+  else hipLaunchKernelGGL((kv_attend<T, D, 2>), grid, block, 0, s, A);
+  if (c.splits > 1)
+    hipLaunchKernelGGL((kv_merge<T, D>), dim3(A.sequences * A.burst * A.heads), block, 0, s, A, 16 * c.rt);
+}
+
+template <typename T>
+void launch_dims(const AttendArgs& A, const Cut& c, hipStream_t s) {
+  switch (A.cache.dim) {
+    case 64: launch_attend<T, 64>(A, c, s); break;
+    case 128: launch_attend<T, 128>(A, c, s); break;
+    default: launch_attend<T, 256>(A, c, s); break;
+  }
+}
+
+}  // namespace
+
+extern "C" {
+
+int fr_hip_kv_append(const fr_hip_kv_write* r, void* stream) {
+  if (!r) return FR_HIP_INVALID;
+  const int rc = check_tokens(&r->cache, r->tokens, r->type, r->k, r->v, true, r->slot);
+  if (rc) return rc;
+  const KvArgs A = {cache_of(r->cache), const_cast<void*>(r->k), const_cast<void*>(r->v), r->slot, r->status,
+                    r->k_token, r->k_head, r->v_token, r->v_head, r->tokens,
+                    rows_wide(r->type, r->k, r->v, r->k_token, r->k_head, r->v_token, r->v_head)};
+  return tokens_call<false>(A, r->type, stream);
+}
+
+int fr_hip_kv_read(const fr_hip_kv_values* r, void* stream) {
+  if (!r) return FR_HIP_INVALID;
+  const int rc = check_tokens(&r->cache, r->tokens, r->type, r->k, r->v, false, r->slot);
+  if (rc) return rc;
+  const KvArgs A = {cache_of(r->cache), r->k, r->v, r->slot, r->status, r->k_token, r->k_head, r->v_token, r->v_head,
+                    r->tokens, rows_wide(r->type, r->k, r->v, r->k_token, r->k_head, r->v_token, r->v_head)};
+  return tokens_call<true>(A, r->type, stream);
+}
+
+size_t fr_hip_kv_workspace(const fr_hip_kv_query* r) { return check_query(r) ? 0 : cut_of(r).bytes; }
+
+int fr_hip_kv_attend(const fr_hip_kv_query* r, void* workspace, size_t bytes, void* stream) {
+  int rc = check_query(r);
+  if (rc) return rc;
+  const Cut c = cut_of(r);
+  if (c.bytes && (!workspace || bytes < c.bytes || (uintptr_t)workspace % 16)) return FR_HIP_INVALID;
+  hipStream_t s;
+  unsigned cus;
+  rc = fronk::enter(stream, &s, &cus);
+  if (rc || !r->sequences) return rc;
+  AttendArgs A;
+  A.cache = cache_of(r->cache);
+  A.q = r->q, A.o = r->o, A.table = r->table, A.length = r->length, A.status = r->status;
+  A.part_o = static_cast<float*>(workspace);
+  A.part_ml = A.part_o + (c.splits > 1 ? (size_t)c.items * c.splits * 16 * c.rt * r->cache.dim : 0);
+  A.q_token = r->q_token, A.q_head = r->q_head, A.o_token = r->o_token, A.o_head = r->o_head;
+  A.sequences = r->sequences, A.burst = r->burst, A.heads = r->heads, A.per = r->heads / r->cache.heads;
+  A.max_context = r->max_context, A.table_stride = r->table_stride;
+  A.splits = c.splits, A.chunk = c.chunk, A.row_blocks = c.row_blocks, A.scale = r->scale;
+  A.wide = rows_wide(r->type, r->q, r->q, r->q_token, r->q_head, 0, 0);
+  switch (r->type) {
+    case FR_HIP_F32: launch_dims<float>(A, c, s); break;
+    case FR_HIP_F16: launch_dims<_Float16>(A, c, s); break;
+    default: launch_dims<__bf16>(A, c, s); break;
+  }
+  FRONK_CK(hipGetLastError());
+  return FR_HIP_OK;
+}
+
+}  // extern "C"

@@ -234,6 +234,144 @@ int fr_hip_batch_plan(const fr_hip_batch *req, void *plan, size_t cap, size_t *u
 int fr_hip_batch_launch(const void *host_plan, const void *device_plan, void *stream);
 int fr_hip_batch_output(void *stream, float *y, size_t count, unsigned *status);
 
+/* ------------------------------------------------------------ dense operators
+ *
+ * The operators of the layers around the experts: the reference's model mixes
+ * tokens by a gated delta rule in 36 of its 48 layers and by attention in 12
+ * (src/model.h:14-15), and leaves both to an external engine. No reference
+ * counterpart. They take device memory that the caller owns, enqueue on
+ * `stream` and return without waiting; nothing is allocated, so every call can
+ * be captured in a graph. Arguments are checked before anything is enqueued
+ * (FR_HIP_INVALID; FR_HIP_UNSUPPORTED for sizes outside the ranges below;
+ * then FR_HIP_STATE without an open engine). What only the device can see
+ * (offsets, slots, pages, lengths) is bounds-checked by the kernels: a bad
+ * entry reads and writes nothing and sets its bit in *status, a device word
+ * that the caller clears (NULL: not reported).
+ *
+ * stream: a hipStream_t, NULL = the library stream (which does not wait for
+ * the default stream), FR_HIP_STREAM_DEFAULT = HIP's default stream.
+ * type: of activations in and out; sums, softmax statistics, norms and states
+ * are fp32 whatever it is. Strides are in elements and a row's last axis is
+ * contiguous; bases and strides of whole 16 bytes are read fastest, and any
+ * other element-aligned ones are taken too where not stated otherwise. */
+#define FR_HIP_STREAM_DEFAULT ((void *)1)
+enum { FR_HIP_F32 = 0, FR_HIP_F16 = 1, FR_HIP_BF16 = 2 };
+enum { FR_HIP_BAD_OFFSET = 1, FR_HIP_BAD_SLOT = 2, FR_HIP_BAD_PAGE = 4, FR_HIP_BAD_LENGTH = 8 };
+
+/* The gated delta rule. Per sequence and value head h (key head h * key_heads
+ * / heads), with the state S [key_dim][value_dim] and token t's scalars
+ * a = exp(g), b = beta:
+ *     u = b (v - a S^T k);   S <- a S + k u^T;   o = scale S^T q
+ * and with FR_HIP_DELTA_NORMALIZE k and q are first divided by
+ * sqrt(sum of squares + 1e-6). g <= 0 (a decay) keeps the state bounded; any
+ * finite g is computed.
+ * Sequence i is tokens offsets[i] .. offsets[i+1]-1, at most max_tokens of
+ * them (offsets NULL: max_tokens each), and its state is row slot[i] of the
+ * pools (slot NULL: row i); slot -1: the sequence is skipped, nothing of it is
+ * read or written. Slots are distinct. state_in NULL: states begin as zeros;
+ * state_out NULL: final states are dropped; both may be one pool. A sequence
+ * of no tokens passes its state on.
+ * key_dim 64, 128 or 256; value_dim a multiple of 16 up to 1024; key_heads
+ * divides heads. State rows are [heads][key_dim][value_dim], 16-byte aligned. */
+enum { FR_HIP_DELTA_NORMALIZE = 1 };
+typedef struct {
+    unsigned sequences, tokens, max_tokens;
+    unsigned key_heads, heads, key_dim, value_dim;
+    unsigned type, flags, slots;      /* slots: rows of the state pools */
+    float scale;
+    const void *q, *k;                /* [tokens][key_heads][key_dim] */
+    const void *v;                    /* [tokens][heads][value_dim] */
+    const float *g, *beta;            /* [tokens][heads], heads contiguous */
+    void *o;                          /* [tokens][heads][value_dim] */
+    int64_t q_token, q_head, k_token, k_head, v_token, v_head, o_token, o_head, g_token, beta_token;
+    const int32_t *offsets, *slot;    /* [sequences + 1], [sequences] */
+    const float *state_in;
+    float *state_out;
+    uint32_t *status;
+} fr_hip_delta;
+/* Bytes of device workspace (16-byte aligned) that fr_hip_delta_rule needs for
+ * these sizes; 0: none, and also for sizes that it refuses. */
+size_t fr_hip_delta_workspace(const fr_hip_delta *req);
+int fr_hip_delta_rule(const fr_hip_delta *req, void *workspace, size_t bytes, void *stream);
+
+/* y[t][n] = sum over k of x[t][k] (code[n][k] - zero[n][k / group])
+ * scale[n][k / group]: products with 4-bit weights, for 1 to 4096 tokens.
+ * codes: byte j of row n holds code 2j in its low nibble and 2j+1 in its high
+ * one; 16-byte aligned, rows cols / 2 bytes apart. scales fp16 or bf16, zeros
+ * uint8 or NULL (8), both [rows][cols / group] dense. group 32, 64 or 128;
+ * cols a multiple of group, up to 65536. A token with a non-finite x gets
+ * non-finite outputs (inf or NaN). */
+typedef struct {
+    unsigned tokens, rows, cols, group;
+    unsigned type, scale_type;        /* scale_type FR_HIP_F16 or FR_HIP_BF16 */
+    const void *x;                    /* [tokens][cols] */
+    const uint8_t *codes;
+    const void *scales;
+    const uint8_t *zeros;
+    void *y;                          /* [tokens][rows] */
+    int64_t x_token, y_token;
+} fr_hip_q4;
+size_t fr_hip_q4_workspace(const fr_hip_q4 *req);
+int fr_hip_q4_product(const fr_hip_q4 *req, void *workspace, size_t bytes, void *stream);
+
+/* A key/value cache in 8 bits, in pages of `page` tokens. A token's vector of
+ * one head is held as dim e4m3 codes (OCP: bias 7, largest 448) and one byte
+ * E, each value code * 2^(E - 127): the smallest power of two that brings the
+ * vector's largest within 448, at least 2^-126 (E = 1, also for zeros), codes
+ * rounded to nearest even. A vector with an infinity or NaN is held as E = 255
+ * and zero codes, and reads back as NaN.
+ *   k_codes [pages][heads][page][dim]
+ *   v_codes [pages][heads][page / 16][dim][16 tokens]
+ *   k_exp, v_exp [pages][heads][page]
+ * all dense, 16-byte aligned, no alignment beyond that. page a multiple of 16
+ * up to 4096; dim 64, 128 or 256. */
+typedef struct {
+    unsigned pages, heads, page, dim;
+    uint8_t *k_codes, *v_codes, *k_exp, *v_exp;
+} fr_hip_kv_cache;
+/* Token t's k and v into slot[t] = page * (tokens a page) + place; slot -1:
+ * the token is skipped. Slots are distinct. */
+typedef struct {
+    fr_hip_kv_cache cache;
+    unsigned tokens, type;
+    const void *k, *v;                /* [tokens][heads][dim] */
+    int64_t k_token, k_head, v_token, v_head;
+    const int32_t *slot;              /* [tokens] */
+    uint32_t *status;
+} fr_hip_kv_write;
+int fr_hip_kv_append(const fr_hip_kv_write *req, void *stream);
+/* The held values of slot[t] as k and v [tokens][heads][dim], rounded to
+ * `type`; slot -1 gives zeros. k or v NULL: not read. */
+typedef struct {
+    fr_hip_kv_cache cache;
+    unsigned tokens, type;
+    void *k, *v;
+    int64_t k_token, k_head, v_token, v_head;
+    const int32_t *slot;
+    uint32_t *status;
+} fr_hip_kv_values;
+int fr_hip_kv_read(const fr_hip_kv_values *req, void *stream);
+/* Attention of bursts over the cache: sequence i's `burst` tokens (1..8) are
+ * the last of its length[i] tokens, token b sees tokens 0 .. length[i] - burst
+ * + b, and per query head h (cache head h * cache.heads / heads)
+ *     o = sum_j softmax_j(scale q . k_j) v_j ;
+ * a token that sees nothing gets zeros. Token j of sequence i lies in page
+ * table[i * table_stride + j / page]. length[i] is at most max_context, which
+ * bounds the launch. cache.heads divides heads, at most 64 query heads for
+ * each cache head. A page outside the cache counts as not seen. */
+typedef struct {
+    fr_hip_kv_cache cache;
+    unsigned sequences, burst, heads, max_context, type, table_stride;
+    float scale;
+    const void *q;                    /* [sequences * burst][heads][dim] */
+    void *o;
+    int64_t q_token, q_head, o_token, o_head;
+    const int32_t *table, *length;
+    uint32_t *status;
+} fr_hip_kv_query;
+size_t fr_hip_kv_workspace(const fr_hip_kv_query *req);
+int fr_hip_kv_attend(const fr_hip_kv_query *req, void *workspace, size_t bytes, void *stream);
+
 /* Launch timing for measurement (no reference counterpart): after
  * fr_hip_timing(n), the next n launches record HIP events on their stream
  * before the main kernel, after it and after the launch's last kernel (a
