@@ -6,6 +6,8 @@
 #include <limits.h>
 #include <math.h>
 
+#include <type_traits>
+
 #include "bounds.h"
 #include "dense.h"
 
@@ -142,6 +144,439 @@ __global__ __launch_bounds__(256) void delta_step(DeltaArgs A) {
   }
 }
 
+// ------------------------------------------------------------ chunk by chunk
+//
+// Within a chunk of 64 tokens, with G the running sum of g and D_ij =
+// e^(G_i - G_j), the rule's updates u solve a lower triangular system:
+//     A_ij = beta_i (k_i . k_j) D_ij  (j < i),   T = (I + A)^-1 diag(beta)
+//     U = T (V - e^G K S)
+//     O = scale (e^G Q S + (Q K^T . D) U),   S <- e^(G_last) S + (e^(G_last - G) K)^T U
+// delta_prepare forms what does not depend on S, for all chunks at once: T, P =
+// scale Q K^T . D, and K and Q as operands. delta_scan then goes through the
+// chunks of one sequence, head and 16 columns of S.
+//
+// All products run on the bf16 matrix cores. A number that is not one bf16 is
+// the sum of parts: fp32 (T, S, U and fp32 activations) of three (8 + 8 + 8
+// bits), fp16 activations of two; products of parts down to 2^-16 of the
+// largest are taken, so that the state keeps fp32's accuracy. Outputs of 16
+// bits take two parts of S, P and U (2^-17, against their own rounding of 2^-9
+// or 2^-12). fp32 matrix instructions would do without parts at a sixteenth of
+// the rate.
+//
+// The order of the summed index in an operand is free, and taken so that a
+// result's registers are the next product's operand: a lane (i, j) of a result
+// holds rows 4j .. 4j+3 of a tile of 16, so operand element e of lane row j
+// stands for index 32 s + 16 (e / 4) + 4 j + e % 4 of step s.
+constexpr int kChunk = 64;
+
+template <typename T> struct Parts;
+template <> struct Parts<__bf16> { static constexpr int kIn = 1, kOut = 2; };
+template <> struct Parts<_Float16> { static constexpr int kIn = 2, kOut = 2; };
+template <> struct Parts<float> { static constexpr int kIn = 3, kOut = 3; };
+
+// The workspace, in operands of 64 lanes x 16 bytes, for each chunk slot.
+// A sequence's chunks begin at slot first / 64 + its index, which leaves room
+// for every sequence's last, partial chunk.
+template <typename T, int DK> struct Room {
+  static constexpr int kN = Parts<T>::kIn, kSteps = DK / 32;
+  static constexpr size_t kRows = (size_t)4 * kSteps * kN;     // K (and Q) with tokens as rows
+  static constexpr size_t kKey = 3 * kRows;                    // ... K, Q, and K with dims as rows
+  static constexpr size_t kT = 6 * 3, kP = 6 * Parts<T>::kOut; // lower triangles: 1, 1, 2, 2 steps
+  static constexpr size_t kHead = kT + kP + 1;                 // ... and 256 floats
+  static size_t bytes(const fr_hip_delta* r) {
+    const size_t slots = (size_t)r->tokens / kChunk + r->sequences;
+    return slots * (kKey * r->key_heads + kHead * r->heads) * 1024;
+  }
+};
+// Triangle operands: tile w's first.
+__device__ __forceinline__ int triangle(int w) { return w < 2 ? w : 2 * w - 2; }
+
+struct ChunkArgs {
+  DeltaArgs d;
+  uint4v *key, *head;   // [slot][key head][Room::kKey][64], [slot][head][Room::kHead][64]
+};
+// Floats of a head's last kilobyte.
+enum { kRowK = 0, kRowQ = 64, kColU = 128, kLast = 192 };
+
+template <int N> __device__ __forceinline__ void split4(float4v x, bf16x4 (&out)[N]) {
+#pragma unroll
+  for (int p = 0; p < N; ++p) {
+    const bf16x2 a = to_bf16(x[0], x[1]), b = to_bf16(x[2], x[3]);
+    out[p] = bf16x4{a[0], a[1], b[0], b[1]};
+    if (p + 1 < N) x -= float4v{(float)a[0], (float)a[1], (float)b[0], (float)b[1]};
+  }
+}
+template <int N> __device__ __forceinline__ void split8(float4v x, float4v y, bf16x8 (&out)[N]) {
+  bf16x4 a[N], b[N];
+  split4<N>(x, a);
+  split4<N>(y, b);
+#pragma unroll
+  for (int p = 0; p < N; ++p) out[p] = bf16x8{a[p][0], a[p][1], a[p][2], a[p][3], b[p][0], b[p][1], b[p][2], b[p][3]};
+}
+// What this wavefront's lanes wrote to LDS is there for all of them.
+__device__ __forceinline__ void wave_lds_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+__device__ __forceinline__ bf16x8 frag(uint4v x) { return __builtin_bit_cast(bf16x8, x); }
+
+// One workgroup: one chunk and key head, and the value heads that share it;
+// wavefront w holds tokens 16 w .. 16 w + 15 as rows.
+template <typename T, int DK>
+__global__ __launch_bounds__(256) void delta_prepare(ChunkArgs C) {
+  typedef Room<T, DK> W;
+  constexpr int N = W::kN, KS = W::kSteps, PO = Parts<T>::kOut, kPitch = kChunk + 4;
+  const DeltaArgs& A = C.d;
+  extern __shared__ uint4v lds[];
+  uint4v* kf = lds;                                            // [4][KS][N][64]
+  float(*m1)[kPitch] = reinterpret_cast<float(*)[kPitch]>(lds + W::kRows * 64);
+  float(*m2)[kPitch] = m1 + kChunk;
+  __shared__ double total[kChunk];
+  __shared__ __attribute__((aligned(16))) float kn[kChunk], qn[kChunk], bt[kChunk];
+
+  const uint32_t chunks = (A.max_tokens + kChunk - 1) / kChunk;
+  const uint32_t kh = blockIdx.x % A.key_heads, chunk = blockIdx.x / A.key_heads % chunks;
+  const uint32_t seq = blockIdx.x / A.key_heads / chunks;
+  uint32_t first, count;
+  size_t row;
+  if (!sequence(A, seq, &first, &count, &row) || chunk * kChunk >= count) return;
+  const uint32_t slot = first / kChunk + seq + chunk;
+  first += chunk * kChunk;
+  const int n = (int)min(count - chunk * kChunk, (uint32_t)kChunk);
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, i = lane & 15, j = lane >> 4;
+  uint4v* key = C.key + ((size_t)slot * A.key_heads + kh) * W::kKey * 64;
+
+  // K and Q of this wavefront's tokens as operands, and their norms.
+  bf16x8 ka[KS][N], qa[KS][N];
+  auto rows = [&](const void* base, int64_t token, int64_t head, bf16x8(&out)[KS][N], float* norm) {
+    const T* p = static_cast<const T*>(base) + (int64_t)(first + (16 * w + i < n ? 16 * w + i : 0)) * token + kh * head;
+    float sum = 0;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      float lo[4], hi[4];
+      load_row<4>(p + 32 * s + 4 * j, A.wide, lo);
+      load_row<4>(p + 32 * s + 16 + 4 * j, A.wide, hi);
+      float4v x = {lo[0], lo[1], lo[2], lo[3]}, y = {hi[0], hi[1], hi[2], hi[3]};
+      if (16 * w + i >= n) x = float4v{0, 0, 0, 0}, y = x;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sum = fmaf(x[e], x[e], fmaf(y[e], y[e], sum));
+      split8<N>(x, y, out[s]);
+    }
+    sum = add_xor32(add_xor16(sum));
+    if (j == 0) norm[16 * w + i] = A.normalize ? 1.f / sqrtf(sum + 1e-6f) : 1.f;
+  };
+  rows(A.k, A.k_token, A.k_head, ka, kn);
+  rows(A.q, A.q_token, A.q_head, qa, qn);
+#pragma unroll
+  for (int s = 0; s < KS; ++s)
+#pragma unroll
+    for (int p = 0; p < N; ++p) {
+      const int at = ((w * KS + s) * N + p) * 64 + lane;
+      kf[at] = key[at] = __builtin_bit_cast(uint4v, ka[s][p]);
+      key[W::kRows * 64 + at] = __builtin_bit_cast(uint4v, qa[s][p]);
+    }
+  __syncthreads();
+
+  // K with dims as rows: dim 16 t + i, tokens 32 s + 16 (e / 4) + 4 j + e % 4.
+  const __bf16* k16 = reinterpret_cast<const __bf16*>(kf);
+  for (int f = w; f < DK / 16 * 2 * N; f += 4) {
+    const int p = f % N, s = f / N % 2, t = f / N / 2;
+    bf16x8 x;
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      x[e] = k16[((((2 * s + e / 4) * KS + t / 2) * N + p) * 64 + 16 * (i >> 2) + 4 * j + e % 4) * 8 + 4 * (t % 2) + (i & 3)];
+    key[2 * W::kRows * 64 + f * 64 + lane] = __builtin_bit_cast(uint4v, x);
+  }
+
+  // K K^T and Q K^T, tiles at and below the diagonal.
+  float4v kk[4], qk[4];
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    kk[u] = qk[u] = float4v{0, 0, 0, 0};
+    if (u > w) continue;
+#pragma unroll
+    for (int s = 0; s < KS; ++s)
+#pragma unroll
+      for (int b = N - 1; b >= 0; --b) {
+        const bf16x8 x = frag(kf[((u * KS + s) * N + b) * 64 + lane]);
+#pragma unroll
+        for (int a = N - 1; a >= 0; --a)
+          if (a + b <= 2) {
+            kk[u] = mma(ka[s][a], x, kk[u]);
+            qk[u] = mma(qa[s][a], x, qk[u]);
+          }
+      }
+  }
+
+  const int group = (int)(A.heads / A.key_heads);
+  for (int r = 0; r < group; ++r) {
+    const uint32_t head = kh * group + r;
+    uint4v* out = C.head + ((size_t)slot * A.heads + head) * W::kHead * 64;
+    float* scalars = reinterpret_cast<float*>(out + (W::kT + W::kP) * 64);
+    if (w == 0) {
+      // In 64 bits: a sum of far decays would take the near ones' differences
+      // with it. One of -1e5 empties the state as -infinity does.
+      double x = lane < n ? (double)A.g[(int64_t)(first + lane) * A.g_token + head] : 0.0;
+      if (x < -1e5) x = -1e5;
+      for (int d = 1; d < 64; d *= 2) {
+        const double y = __shfl_up(x, d);
+        if (lane >= d) x += y;
+      }
+      total[lane] = x;
+      bt[lane] = lane < n ? A.beta[(int64_t)(first + lane) * A.beta_token + head] : 0.f;
+      const double last = __shfl(x, 63);
+      const float gamma = expf((float)x);
+      scalars[kRowK + lane] = gamma * kn[lane];
+      scalars[kRowQ + lane] = gamma * qn[lane] * A.scale;
+      scalars[kColU + lane] = expf((float)(last - x)) * kn[lane];
+      if (lane == 0) scalars[kLast] = expf((float)last);
+    }
+    __syncthreads();
+    // P row by row, then A, through m1.
+    float decay[4][4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int a = 16 * w + 4 * j + e, b = 16 * u + i;
+        decay[u][e] = a >= b ? expf((float)(total[a] - total[b])) * kn[b] : 0.f;
+        m1[a][b] = a >= b ? qk[u][e] * decay[u][e] * (qn[a] * A.scale) : 0.f;
+      }
+    __syncthreads();
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      if (s > w / 2) continue;
+      bf16x8 x[PO];
+      split8<PO>(*reinterpret_cast<const float4v*>(&m1[16 * w + i][32 * s + 4 * j]),
+                 *reinterpret_cast<const float4v*>(&m1[16 * w + i][32 * s + 16 + 4 * j]), x);
+#pragma unroll
+      for (int p = 0; p < PO; ++p)
+        out[(W::kT + (triangle(w) + s) * PO + p) * 64 + lane] = __builtin_bit_cast(uint4v, x[p]);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int a = 16 * w + 4 * j + e, b = 16 * u + i;
+        m1[a][b] = a > b ? kk[u][e] * decay[u][e] * (bt[a] * kn[a]) : 0.f;
+        m2[a][b] = 0.f;
+      }
+    __syncthreads();
+    // (I + A)^-1 in m2 by blocks of 16: the diagonal ones by substitution
+    // (lane i column i; products of powers of A would lose digits where keys
+    // are alike), then those below by the distance from it, each from blocks
+    // that are there: X_wu = -X_ww sum_{u <= v < w} A_wv X_vu.
+    {
+      float x[16];
+#pragma unroll
+      for (int a = 0; a < 16; ++a) {
+        float y = a == i ? 1.f : 0.f;
+#pragma unroll
+        for (int b = 0; b < a; ++b) y = fmaf(-m1[16 * w + a][16 * w + b], x[b], y);
+        x[a] = y;
+      }
+      if (j == 0) {
+#pragma unroll
+        for (int a = 0; a < 16; ++a) m2[16 * w + a][16 * w + i] = x[a];
+      }
+    }
+    for (int dist = 1; dist < 4; ++dist) {
+      __syncthreads();
+      if (w >= dist) {
+        const int u = w - dist;
+        float4v c = {0, 0, 0, 0};
+        for (int v = u; v < w; ++v)
+#pragma unroll
+          for (int s = 0; s < 4; ++s)
+            c = __builtin_amdgcn_mfma_f32_16x16x4f32(m1[16 * w + i][16 * v + 4 * s + j], m2[16 * v + 4 * s + j][16 * u + i], c, 0, 0, 0);
+        // The sum's place until it is an operand: the block that it becomes.
+#pragma unroll
+        for (int e = 0; e < 4; ++e) m2[16 * w + 4 * j + e][16 * u + i] = c[e];
+        wave_lds_sync();
+        float4v y = {0, 0, 0, 0};
+#pragma unroll
+        for (int s = 0; s < 4; ++s)
+          y = __builtin_amdgcn_mfma_f32_16x16x4f32(m2[16 * w + i][16 * w + 4 * s + j], m2[16 * w + 4 * s + j][16 * u + i], y, 0, 0, 0);
+        wave_lds_sync();
+#pragma unroll
+        for (int e = 0; e < 4; ++e) m2[16 * w + 4 * j + e][16 * u + i] = -y[e];
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      if (s > w / 2) continue;
+      const int c = 32 * s + 4 * j;
+      bf16x8 x[3];
+      split8<3>(*reinterpret_cast<const float4v*>(&m2[16 * w + i][c]) * *reinterpret_cast<const float4v*>(&bt[c]),
+                *reinterpret_cast<const float4v*>(&m2[16 * w + i][c + 16]) * *reinterpret_cast<const float4v*>(&bt[c + 16]), x);
+#pragma unroll
+      for (int p = 0; p < 3; ++p) out[((triangle(w) + s) * 3 + p) * 64 + lane] = __builtin_bit_cast(uint4v, x[p]);
+    }
+    __syncthreads();
+  }
+}
+
+// One workgroup: one sequence, head and 16 columns of S, chunk after chunk.
+// Wavefronts 0..3 carry the state: wavefront w has tokens 16 w .. of the chunk
+// and dims w * dk / 4 .. of S (in registers, fp32), and three times a chunk they
+// exchange operands through LDS: S, then V - e^G K S, then U. Wavefronts 4..7
+// form the outputs of the same tokens beside them.
+template <typename T, int DK>
+__global__ __launch_bounds__(512) void delta_scan(ChunkArgs C) {
+  typedef Room<T, DK> W;
+  constexpr int N = W::kN, KS = W::kSteps, PO = Parts<T>::kOut, TPW = DK / 64;
+  const DeltaArgs& A = C.d;
+  __shared__ uint4v sf[3][KS][64], rf[3][2][64], uf[PO][2][64], wf[3][2][64];
+  const int lane = threadIdx.x & 63, w = (threadIdx.x >> 6) & 3, i = lane & 15, j = lane >> 4;
+  const bool chain = threadIdx.x < 256;
+  const uint32_t tiles = A.dv / 16;
+  const uint32_t tile = blockIdx.x % tiles, head = blockIdx.x / tiles % A.heads, seq = blockIdx.x / tiles / A.heads;
+  uint32_t first, count;
+  size_t row;
+  if (!sequence(A, seq, &first, &count, &row)) return;
+  const uint32_t slot = first / kChunk + seq, chunks = (count + kChunk - 1) / kChunk, kh = head / (A.heads / A.key_heads);
+  const uint4v* key = C.key + ((size_t)slot * A.key_heads + kh) * W::kKey * 64 + lane;
+  const uint4v* per = C.head + ((size_t)slot * A.heads + head) * W::kHead * 64 + lane;
+  const size_t key_next = (size_t)A.key_heads * W::kKey * 64, per_next = (size_t)A.heads * W::kHead * 64;
+  const uint32_t col = tile * 16 + i;
+
+  // Four values of a lane into its half of an operand's parts.
+  auto put = [&](uint4v* base, int stride, int half, float4v x, auto parts) {
+    constexpr int P = decltype(parts)::value;
+    bf16x4 y[P];
+    split4<P>(x, y);
+#pragma unroll
+    for (int p = 0; p < P; ++p) reinterpret_cast<bf16x4*>(base + p * stride)[lane * 2 + half] = y[p];
+  };
+  constexpr std::integral_constant<int, 3> three{};
+  constexpr std::integral_constant<int, PO> few{};
+
+  float4v state[TPW];
+  const size_t at = ((row * A.heads + head) * DK + 16 * w * TPW + 4 * j) * A.dv + col;
+  if (chain) {
+#pragma unroll
+    for (int t = 0; t < TPW; ++t) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) state[t][e] = A.state_in ? A.state_in[at + (size_t)(16 * t + e) * A.dv] : 0.f;
+      put(&sf[0][(w * TPW + t) / 2][0], KS * 64, (w * TPW + t) % 2, state[t], three);
+    }
+  }
+
+  for (uint32_t c = 0; c < chunks; ++c, key += key_next, per += per_next) {
+    const int token = (int)(c * kChunk) + 16 * w + 4 * j;   // this lane's first of four
+    const float* scalars = reinterpret_cast<const float*>(per - lane + (W::kT + W::kP) * 64) + 16 * w + 4 * j;
+    __syncthreads();   // S is there
+    float4v acc = {0, 0, 0, 0}, low = acc;
+    if (chain) {
+      float4v v;
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        v[e] = token + e < (int)count
+                   ? (float)static_cast<const T*>(A.v)[(int64_t)(first + token + e) * A.v_token + head * A.v_head + col]
+                   : 0.f;
+#pragma unroll
+      for (int s = 0; s < KS; ++s)
+#pragma unroll
+        for (int a = 0; a < N; ++a) {
+          const bf16x8 x = frag(key[((w * KS + s) * N + a) * 64]);
+#pragma unroll
+          for (int b = 2 - a; b >= 0; --b) {
+            float4v& to = a + b ? low : acc;
+            to = mma(x, frag(sf[b][s][lane]), to);
+          }
+        }
+      acc += low;
+      const float4v rowk = *reinterpret_cast<const float4v*>(scalars + kRowK);
+      put(&rf[0][w / 2][0], 2 * 64, w % 2, v - rowk * acc, three);
+    } else {
+#pragma unroll
+      for (int s = 0; s < KS; ++s)
+#pragma unroll
+        for (int a = 0; a < N; ++a) {
+          const bf16x8 x = frag(key[W::kRows * 64 + ((w * KS + s) * N + a) * 64]);
+#pragma unroll
+          for (int b = PO - 1 - a; b >= 0; --b) {
+            float4v& to = a + b ? low : acc;
+            to = mma(x, frag(sf[b][s][lane]), to);
+          }
+        }
+      acc += low;
+      acc *= *reinterpret_cast<const float4v*>(scalars + kRowQ);
+    }
+    __syncthreads();   // V - e^G K S is there, and S is read
+    if (chain) {
+      float4v u = {0, 0, 0, 0};
+      low = u;
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        if (s > w / 2) continue;
+#pragma unroll
+        for (int a = 0; a < 3; ++a) {
+          const bf16x8 x = frag(per[((triangle(w) + s) * 3 + a) * 64]);
+#pragma unroll
+          for (int b = 2 - a; b >= 0; --b) {
+            float4v& to = a + b ? low : u;
+            to = mma(x, frag(rf[b][s][lane]), to);
+          }
+        }
+      }
+      u += low;
+      put(&uf[0][w / 2][0], 2 * 64, w % 2, u, few);
+      put(&wf[0][w / 2][0], 2 * 64, w % 2, u * *reinterpret_cast<const float4v*>(scalars + kColU), three);
+    }
+    __syncthreads();   // U is there
+    if (chain) {
+      const float last = *(scalars - 16 * w - 4 * j + kLast);
+#pragma unroll
+      for (int t = 0; t < TPW; ++t) {
+        float4v x = {0, 0, 0, 0};
+        low = x;
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+          for (int a = 0; a < N; ++a) {
+            const bf16x8 y = frag(key[2 * W::kRows * 64 + (((w * TPW + t) * 2 + s) * N + a) * 64]);
+#pragma unroll
+            for (int b = 2 - a; b >= 0; --b) {
+              float4v& to = a + b ? low : x;
+              to = mma(y, frag(wf[b][s][lane]), to);
+            }
+          }
+        state[t] = last * state[t] + (x + low);
+        put(&sf[0][(w * TPW + t) / 2][0], KS * 64, (w * TPW + t) % 2, state[t], three);
+      }
+    } else {
+      low = float4v{0, 0, 0, 0};
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        if (s > w / 2) continue;
+#pragma unroll
+        for (int a = 0; a < PO; ++a) {
+          const bf16x8 x = frag(per[(W::kT + (triangle(w) + s) * PO + a) * 64]);
+#pragma unroll
+          for (int b = PO - 1 - a; b >= 0; --b) {
+            float4v& to = a + b ? low : acc;
+            to = mma(x, frag(uf[b][s][lane]), to);
+          }
+        }
+      }
+      acc += low;
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (token + e < (int)count)
+          static_cast<T*>(A.o)[(int64_t)(first + token + e) * A.o_token + head * A.o_head + col] = (T)acc[e];
+    }
+  }
+  if (chain && A.state_out) {
+#pragma unroll
+    for (int t = 0; t < TPW; ++t)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) A.state_out[at + (size_t)(16 * t + e) * A.dv] = state[t][e];
+  }
+}
+
 // ---------------------------------------------------------------------- host
 
 int check(const fr_hip_delta* r) {
@@ -156,8 +591,9 @@ int check(const fr_hip_delta* r) {
   if (((uintptr_t)r->q | (uintptr_t)r->k | (uintptr_t)r->v | (uintptr_t)r->o) % elem_size(r->type)) return FR_HIP_INVALID;
   if (r->key_dim != 64 && r->key_dim != 128 && r->key_dim != 256) return FR_HIP_UNSUPPORTED;
   if (r->value_dim % 16 || r->value_dim > 1024 || r->heads > 65535) return FR_HIP_UNSUPPORTED;
-  // One-dimensional grids of (sequence, head, 16 columns).
+  // One-dimensional grids of (sequence, head, 16 columns) and (sequence, chunk, key head).
   if ((uint64_t)r->sequences * r->heads * (r->value_dim / 16) > INT_MAX) return FR_HIP_UNSUPPORTED;
+  if ((uint64_t)r->sequences * ((uint64_t)r->max_tokens / kChunk + 1) * r->key_heads > INT_MAX) return FR_HIP_UNSUPPORTED;
   return FR_HIP_OK;
 }
 
@@ -176,7 +612,7 @@ DeltaArgs arguments(const fr_hip_delta* r) {
   A.q_token = r->q_token, A.q_head = r->q_head, A.k_token = r->k_token, A.k_head = r->k_head;
   A.v_token = r->v_token, A.v_head = r->v_head, A.o_token = r->o_token, A.o_head = r->o_head;
   A.g_token = r->g_token, A.beta_token = r->beta_token;
-  A.sequences = r->sequences, A.tokens = r->tokens, A.max_tokens = r->max_tokens;
+  A.sequences = r->sequences, A.tokens = r->tokens, A.max_tokens = r->max_tokens < r->tokens ? r->max_tokens : r->tokens;
   A.key_heads = r->key_heads, A.heads = r->heads, A.dv = r->value_dim;
   // Without state pools a slot only says whether the sequence is skipped.
   A.slots = r->state_in || r->state_out || r->slot ? r->slots : (uint32_t)INT_MAX;
@@ -202,29 +638,69 @@ void launch_step(const fr_hip_delta* r, const DeltaArgs& A, hipStream_t s) {
   }
 }
 
+// Bursts go token by token; from this many tokens on, chunks.
+constexpr unsigned kChunkFrom = 33;
+bool in_chunks(const fr_hip_delta* r) { return r->max_tokens >= kChunkFrom; }
+
+template <typename T, int DK>
+int launch_chunks(const fr_hip_delta* r, const DeltaArgs& A, void* workspace, hipStream_t s) {
+  typedef Room<T, DK> W;
+  constexpr size_t kLds = W::kRows * 1024 + 2 * kChunk * (kChunk + 4) * sizeof(float);
+  const size_t slots = (size_t)r->tokens / kChunk + r->sequences;
+  const ChunkArgs C = {A, static_cast<uint4v*>(workspace), static_cast<uint4v*>(workspace) + slots * W::kKey * r->key_heads * 64};
+  static const hipError_t wide = hipFuncSetAttribute(reinterpret_cast<const void*>(&delta_prepare<T, DK>),
+                                                     hipFuncAttributeMaxDynamicSharedMemorySize, (int)kLds);
+  FRONK_CK(wide);
+  const uint32_t chunks = (A.max_tokens + kChunk - 1) / kChunk;
+  hipLaunchKernelGGL((delta_prepare<T, DK>), dim3(r->sequences * chunks * r->key_heads), dim3(256), kLds, s, C);
+  hipLaunchKernelGGL((delta_scan<T, DK>), dim3(r->sequences * r->heads * (r->value_dim / 16)), dim3(512), 0, s, C);
+  return FR_HIP_OK;
+}
+
+template <typename T>
+size_t room(const fr_hip_delta* r) {
+  return r->key_dim == 64 ? Room<T, 64>::bytes(r) : r->key_dim == 128 ? Room<T, 128>::bytes(r) : Room<T, 256>::bytes(r);
+}
+size_t workspace_bytes(const fr_hip_delta* r) {
+  if (!in_chunks(r) || !r->tokens) return 0;
+  return r->type == FR_HIP_F32 ? room<float>(r) : r->type == FR_HIP_F16 ? room<_Float16>(r) : room<__bf16>(r);
+}
+
+template <typename T>
+int launch(const fr_hip_delta* r, const DeltaArgs& A, void* workspace, hipStream_t s) {
+  if (!workspace_bytes(r)) {
+    launch_step<T>(r, A, s);
+    return FR_HIP_OK;
+  }
+  switch (r->key_dim) {
+    case 64: return launch_chunks<T, 64>(r, A, workspace, s);
+    case 128: return launch_chunks<T, 128>(r, A, workspace, s);
+    default: return launch_chunks<T, 256>(r, A, workspace, s);
+  }
+}
+
 }  // namespace
 
 extern "C" {
 
-size_t fr_hip_delta_workspace(const fr_hip_delta* req) {
-  (void)req;
-  return 0;
-}
+size_t fr_hip_delta_workspace(const fr_hip_delta* req) { return check(req) ? 0 : workspace_bytes(req); }
 
 int fr_hip_delta_rule(const fr_hip_delta* req, void* workspace, size_t bytes, void* stream) {
-  (void)workspace, (void)bytes;
   int rc = check(req);
   if (rc) return rc;
+  const size_t need = workspace_bytes(req);
+  if (need && (!workspace || bytes < need || (uintptr_t)workspace % 16)) return FR_HIP_INVALID;
   hipStream_t s;
   unsigned cus;
   rc = fronk::enter(stream, &s, &cus);
   if (rc || !req->sequences) return rc;
   const DeltaArgs A = arguments(req);
   switch (req->type) {
-    case FR_HIP_F32: launch_step<float>(req, A, s); break;
-    case FR_HIP_F16: launch_step<_Float16>(req, A, s); break;
-    default: launch_step<__bf16>(req, A, s); break;
+    case FR_HIP_F32: rc = launch<float>(req, A, workspace, s); break;
+    case FR_HIP_F16: rc = launch<_Float16>(req, A, workspace, s); break;
+    default: rc = launch<__bf16>(req, A, workspace, s); break;
   }
+  if (rc) return rc;
   FRONK_CK(hipGetLastError());
   return FR_HIP_OK;
 }
