@@ -163,10 +163,11 @@ __global__ __launch_bounds__(256) void delta_step(DeltaArgs A) {
 // or 2^-12). fp32 matrix instructions would do without parts at a sixteenth of
 // the rate.
 //
-// The order of the summed index in an operand is free, and taken so that a
-// result's registers are the next product's operand: a lane (i, j) of a result
+// The order of the summed index in an operand is free. Over dims it is theirs,
+// so that rows of K and Q are read as they lie; over tokens it is taken so that
+// a result's registers are the next product's operand: a lane (i, j) of a result
 // holds rows 4j .. 4j+3 of a tile of 16, so operand element e of lane row j
-// stands for index 32 s + 16 (e / 4) + 4 j + e % 4 of step s.
+// stands for token 32 s + 16 (e / 4) + 4 j + e % 4 of step s.
 constexpr int kChunk = 64;
 
 template <typename T> struct Parts;
@@ -218,6 +219,13 @@ __device__ __forceinline__ void wave_lds_sync() {
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   __builtin_amdgcn_wave_barrier();
 }
+// All of the workgroup's LDS writes are there for all of it; loads and stores of
+// memory go on.
+__device__ __forceinline__ void lds_barrier() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
 __device__ __forceinline__ bf16x8 frag(uint4v x) { return __builtin_bit_cast(bf16x8, x); }
 
 // One workgroup: one chunk and key head, and the value heads that share it;
@@ -253,10 +261,9 @@ __global__ __launch_bounds__(256) void delta_prepare(ChunkArgs C) {
     float sum = 0;
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
-      float lo[4], hi[4];
-      load_row<4>(p + 32 * s + 4 * j, A.wide, lo);
-      load_row<4>(p + 32 * s + 16 + 4 * j, A.wide, hi);
-      float4v x = {lo[0], lo[1], lo[2], lo[3]}, y = {hi[0], hi[1], hi[2], hi[3]};
+      float f[8];
+      load_row<8>(p + 32 * s + 8 * j, A.wide, f);
+      float4v x = {f[0], f[1], f[2], f[3]}, y = {f[4], f[5], f[6], f[7]};
       if (16 * w + i >= n) x = float4v{0, 0, 0, 0}, y = x;
 #pragma unroll
       for (int e = 0; e < 4; ++e) sum = fmaf(x[e], x[e], fmaf(y[e], y[e], sum));
@@ -284,7 +291,7 @@ __global__ __launch_bounds__(256) void delta_prepare(ChunkArgs C) {
     bf16x8 x;
 #pragma unroll
     for (int e = 0; e < 8; ++e)
-      x[e] = k16[((((2 * s + e / 4) * KS + t / 2) * N + p) * 64 + 16 * (i >> 2) + 4 * j + e % 4) * 8 + 4 * (t % 2) + (i & 3)];
+      x[e] = k16[((((2 * s + e / 4) * KS + t / 2) * N + p) * 64 + 16 * (2 * (t % 2) + (i >> 3)) + 4 * j + e % 4) * 8 + (i & 7)];
     key[2 * W::kRows * 64 + f * 64 + lane] = __builtin_bit_cast(uint4v, x);
   }
 
@@ -423,157 +430,218 @@ __global__ __launch_bounds__(256) void delta_prepare(ChunkArgs C) {
 // and dims w * dk / 4 .. of S (in registers, fp32), and three times a chunk they
 // exchange operands through LDS: S, then V - e^G K S, then U. Wavefronts 4..7
 // form the outputs of the same tokens beside them.
+//
+// A chunk costs three barriers and the products between them, so nothing may
+// wait for memory there: each operand's registers are filled for the next chunk
+// as soon as this one's product has read them (kAhead; with fp32's 54 operands
+// at dk 256, which do not fit, K's rows and dims take turns). The two kinds of
+// wavefronts have loops of their own, so that neither's loads are waited for on
+// account of the other's.
 template <typename T, int DK>
 __global__ __launch_bounds__(512) void delta_scan(ChunkArgs C) {
   typedef Room<T, DK> W;
   constexpr int N = W::kN, KS = W::kSteps, PO = Parts<T>::kOut, TPW = DK / 64;
+  constexpr bool kAhead = KS * N + TPW * 2 * N <= 32;
   const DeltaArgs& A = C.d;
   __shared__ uint4v sf[3][KS][64], rf[3][2][64], uf[PO][2][64], wf[3][2][64];
-  const int lane = threadIdx.x & 63, w = (threadIdx.x >> 6) & 3, i = lane & 15, j = lane >> 4;
-  const bool chain = threadIdx.x < 256;
-  const uint32_t tiles = A.dv / 16;
-  const uint32_t tile = blockIdx.x % tiles, head = blockIdx.x / tiles % A.heads, seq = blockIdx.x / tiles / A.heads;
+  const int lane = threadIdx.x & 63, i = lane & 15, j = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), w = wave & 3;
+  const bool chain = wave < 4;
+  // The heads of a key head and their tiles follow each other at a distance of
+  // key_heads, which for a multiple of 8 puts them on one die and its L2.
+  const uint32_t group = A.heads / A.key_heads, tiles = A.dv / 16;
+  const uint32_t kh = blockIdx.x % A.key_heads, head = kh * group + blockIdx.x / A.key_heads % group;
+  const uint32_t tile = blockIdx.x / A.heads % tiles, seq = blockIdx.x / A.heads / tiles;
   uint32_t first, count;
   size_t row;
   if (!sequence(A, seq, &first, &count, &row)) return;
-  const uint32_t slot = first / kChunk + seq, chunks = (count + kChunk - 1) / kChunk, kh = head / (A.heads / A.key_heads);
-  const uint4v* key = C.key + ((size_t)slot * A.key_heads + kh) * W::kKey * 64 + lane;
-  const uint4v* per = C.head + ((size_t)slot * A.heads + head) * W::kHead * 64 + lane;
-  const size_t key_next = (size_t)A.key_heads * W::kKey * 64, per_next = (size_t)A.heads * W::kHead * 64;
+  const uint32_t slot = first / kChunk + seq, chunks = (count + kChunk - 1) / kChunk;
   const uint32_t col = tile * 16 + i;
+  const int steps = w < 2 ? 1 : 2;   // of T's and P's row tile w
 
-  // Four values of a lane into its half of an operand's parts.
-  auto put = [&](uint4v* base, int stride, int half, float4v x, auto parts) {
+  // Four values of lane row r into half h of an operand's parts.
+  auto put = [&](uint4v* base, int stride, int r, int half, float4v x, auto parts) {
     constexpr int P = decltype(parts)::value;
     bf16x4 y[P];
     split4<P>(x, y);
 #pragma unroll
-    for (int p = 0; p < P; ++p) reinterpret_cast<bf16x4*>(base + p * stride)[lane * 2 + half] = y[p];
+    for (int p = 0; p < P; ++p) reinterpret_cast<bf16x4*>(base + p * stride)[(i + 16 * r) * 2 + half] = y[p];
   };
   constexpr std::integral_constant<int, 3> three{};
   constexpr std::integral_constant<int, PO> few{};
 
-  float4v state[TPW];
-  const size_t at = ((row * A.heads + head) * DK + 16 * w * TPW + 4 * j) * A.dv + col;
+  const uint4v* key = C.key + ((size_t)slot * A.key_heads + kh) * W::kKey * 64 + (chain ? 0 : W::kRows * 64) + lane;
+  const uint4v* per = C.head + ((size_t)slot * A.heads + head) * W::kHead * 64 + lane;
+  const size_t key_next = (size_t)A.key_heads * W::kKey * 64, per_next = (size_t)A.heads * W::kHead * 64;
+  // Chunk c's rows of K (or Q), rows of T (or P), and scalars from `at` on.
+  uint4v a1[KS][N], a2[2][3];
+  auto load1 = [&](uint32_t c) {
+    const uint4v* p = key + c * key_next + w * KS * N * 64;
+#pragma unroll
+    for (int s = 0; s < KS; ++s)
+#pragma unroll
+      for (int a = 0; a < N; ++a) a1[s][a] = p[(s * N + a) * 64];
+  };
+  auto load2 = [&](uint32_t c, auto parts) {
+    constexpr int P = decltype(parts)::value;
+    const uint4v* p = per + c * per_next + triangle(w) * P * 64;
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+      for (int a = 0; a < P; ++a)
+        if (s < steps) a2[s][a] = p[(s * P + a) * 64];
+  };
+  auto scalars = [&](uint32_t c, int at) {
+    return *reinterpret_cast<const float4v*>(reinterpret_cast<const float*>(per - lane + c * per_next + (W::kT + W::kP) * 64) +
+                                             at + 16 * w + 4 * j);
+  };
+
   if (chain) {
+    uint4v a3[TPW][2][N];
+    float4v row_scale, col_scale;
+    float last;
+    T v[4];
+    auto load3 = [&](uint32_t c) {
+      const uint4v* p = key + c * key_next + (2 * W::kRows + w * TPW * 2 * N) * 64;
+#pragma unroll
+      for (int t = 0; t < TPW; ++t)
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+          for (int a = 0; a < N; ++a) a3[t][s][a] = p[((t * 2 + s) * N + a) * 64];
+      last = reinterpret_cast<const float*>(per - lane + c * per_next + (W::kT + W::kP) * 64)[kLast];
+    };
+    auto load_v = [&](uint32_t c) {
+      const T* x = static_cast<const T*>(A.v) + (int64_t)first * A.v_token + head * A.v_head + col;
+      const uint32_t token = c * kChunk + 16 * w + 4 * j;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = x[(int64_t)min(token + e, count - 1) * A.v_token];
+      row_scale = scalars(c, kRowK);
+    };
+    // S's operands go by dims in their order, as rows of K and Q lie in memory.
+    auto put_state = [&](int t, float4v x) {
+      const int at = w * TPW + t;
+      put(&sf[0][at / 2][0], KS * 64, 2 * (at % 2) + j / 2, j % 2, x, three);
+    };
+    if (chunks) {
+      load1(0), load_v(0), load2(0, three);
+      col_scale = scalars(0, kColU);
+      if constexpr (kAhead) load3(0);
+    }
+    float4v state[TPW];
+    const size_t at = ((row * A.heads + head) * DK + 16 * w * TPW + 4 * j) * A.dv + col;
 #pragma unroll
     for (int t = 0; t < TPW; ++t) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) state[t][e] = A.state_in ? A.state_in[at + (size_t)(16 * t + e) * A.dv] : 0.f;
-      put(&sf[0][(w * TPW + t) / 2][0], KS * 64, (w * TPW + t) % 2, state[t], three);
+      put_state(t, state[t]);
     }
-  }
-
-  for (uint32_t c = 0; c < chunks; ++c, key += key_next, per += per_next) {
-    const int token = (int)(c * kChunk) + 16 * w + 4 * j;   // this lane's first of four
-    const float* scalars = reinterpret_cast<const float*>(per - lane + (W::kT + W::kP) * 64) + 16 * w + 4 * j;
-    __syncthreads();   // S is there
-    float4v acc = {0, 0, 0, 0}, low = acc;
-    if (chain) {
-      float4v v;
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        v[e] = token + e < (int)count
-                   ? (float)static_cast<const T*>(A.v)[(int64_t)(first + token + e) * A.v_token + head * A.v_head + col]
-                   : 0.f;
+    for (uint32_t c = 0; c < chunks; ++c) {
+      const uint32_t next = c + 1 < chunks ? c + 1 : c;
+      lds_barrier();   // S is there
+      float4v x[3] = {};
 #pragma unroll
       for (int s = 0; s < KS; ++s)
 #pragma unroll
-        for (int a = 0; a < N; ++a) {
-          const bf16x8 x = frag(key[((w * KS + s) * N + a) * 64]);
+        for (int b = 2; b >= 0; --b) {
+          const bf16x8 y = frag(sf[b][s][lane]);
 #pragma unroll
-          for (int b = 2 - a; b >= 0; --b) {
-            float4v& to = a + b ? low : acc;
-            to = mma(x, frag(sf[b][s][lane]), to);
-          }
+          for (int a = 0; a < N && a + b <= 2; ++a) x[a + b] = mma(frag(a1[s][a]), y, x[a + b]);
         }
-      acc += low;
-      const float4v rowk = *reinterpret_cast<const float4v*>(scalars + kRowK);
-      put(&rf[0][w / 2][0], 2 * 64, w % 2, v - rowk * acc, three);
-    } else {
+      const uint32_t token = c * kChunk + 16 * w + 4 * j;
+      float4v r;
 #pragma unroll
-      for (int s = 0; s < KS; ++s)
-#pragma unroll
-        for (int a = 0; a < N; ++a) {
-          const bf16x8 x = frag(key[W::kRows * 64 + ((w * KS + s) * N + a) * 64]);
-#pragma unroll
-          for (int b = PO - 1 - a; b >= 0; --b) {
-            float4v& to = a + b ? low : acc;
-            to = mma(x, frag(sf[b][s][lane]), to);
-          }
-        }
-      acc += low;
-      acc *= *reinterpret_cast<const float4v*>(scalars + kRowQ);
-    }
-    __syncthreads();   // V - e^G K S is there, and S is read
-    if (chain) {
-      float4v u = {0, 0, 0, 0};
-      low = u;
+      for (int e = 0; e < 4; ++e) r[e] = token + e < count ? (float)v[e] : 0.f;
+      r -= row_scale * (x[0] + (x[1] + x[2]));
+      if constexpr (kAhead) load1(next);
+      else load3(c);
+      load_v(next);
+      put(&rf[0][w / 2][0], 2 * 64, j, w % 2, r, three);
+      lds_barrier();   // V - e^G K S is there, and S is read
+      float4v u[3] = {};
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
-        if (s > w / 2) continue;
+        if (s >= steps) continue;
 #pragma unroll
-        for (int a = 0; a < 3; ++a) {
-          const bf16x8 x = frag(per[((triangle(w) + s) * 3 + a) * 64]);
+        for (int b = 2; b >= 0; --b) {
+          const bf16x8 y = frag(rf[b][s][lane]);
 #pragma unroll
-          for (int b = 2 - a; b >= 0; --b) {
-            float4v& to = a + b ? low : u;
-            to = mma(x, frag(rf[b][s][lane]), to);
-          }
+          for (int a = 0; a + b <= 2; ++a) u[a + b] = mma(frag(a2[s][a]), y, u[a + b]);
         }
       }
-      u += low;
-      put(&uf[0][w / 2][0], 2 * 64, w % 2, u, few);
-      put(&wf[0][w / 2][0], 2 * 64, w % 2, u * *reinterpret_cast<const float4v*>(scalars + kColU), three);
-    }
-    __syncthreads();   // U is there
-    if (chain) {
-      const float last = *(scalars - 16 * w - 4 * j + kLast);
+      u[0] += u[1] + u[2];
+      put(&uf[0][w / 2][0], 2 * 64, j, w % 2, u[0], few);
+      put(&wf[0][w / 2][0], 2 * 64, j, w % 2, u[0] * col_scale, three);
+      load2(next, three);
+      col_scale = scalars(next, kColU);
+      lds_barrier();   // U is there
 #pragma unroll
       for (int t = 0; t < TPW; ++t) {
-        float4v x = {0, 0, 0, 0};
-        low = x;
+        float4v z[3] = {};
 #pragma unroll
         for (int s = 0; s < 2; ++s)
 #pragma unroll
-          for (int a = 0; a < N; ++a) {
-            const bf16x8 y = frag(key[2 * W::kRows * 64 + (((w * TPW + t) * 2 + s) * N + a) * 64]);
+          for (int b = 2; b >= 0; --b) {
+            const bf16x8 y = frag(wf[b][s][lane]);
 #pragma unroll
-            for (int b = 2 - a; b >= 0; --b) {
-              float4v& to = a + b ? low : x;
-              to = mma(y, frag(wf[b][s][lane]), to);
-            }
+            for (int a = 0; a < N && a + b <= 2; ++a) z[a + b] = mma(frag(a3[t][s][a]), y, z[a + b]);
           }
-        state[t] = last * state[t] + (x + low);
-        put(&sf[0][(w * TPW + t) / 2][0], KS * 64, (w * TPW + t) % 2, state[t], three);
+        state[t] = last * state[t] + (z[0] + (z[1] + z[2]));
+        put_state(t, state[t]);
       }
-    } else {
-      low = float4v{0, 0, 0, 0};
+      if constexpr (kAhead) load3(next);
+      else load1(next);
+    }
+    if (A.state_out) {
+#pragma unroll
+      for (int t = 0; t < TPW; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) A.state_out[at + (size_t)(16 * t + e) * A.dv] = state[t][e];
+    }
+  } else {
+    per += W::kT * 64;   // P
+    float4v row_scale;
+    auto rows_of = [&](uint32_t c) {
+      load1(c);
+      row_scale = *reinterpret_cast<const float4v*>(
+          reinterpret_cast<const float*>(per - lane + c * per_next + W::kP * 64) + kRowQ + 16 * w + 4 * j);
+    };
+    if (chunks) rows_of(0), load2(0, few);
+    for (uint32_t c = 0; c < chunks; ++c) {
+      const uint32_t next = c + 1 < chunks ? c + 1 : c;
+      lds_barrier();   // S is there
+      float4v acc[3] = {};
+#pragma unroll
+      for (int s = 0; s < KS; ++s)
+#pragma unroll
+        for (int b = PO - 1; b >= 0; --b) {
+          const bf16x8 y = frag(sf[b][s][lane]);
+#pragma unroll
+          for (int a = 0; a < N && a + b < PO; ++a) acc[a + b] = mma(frag(a1[s][a]), y, acc[a + b]);
+        }
+      acc[0] = row_scale * (acc[0] + (acc[1] + acc[2]));
+      acc[1] = acc[2] = float4v{0, 0, 0, 0};
+      rows_of(next);
+      lds_barrier();   // S is read
+      lds_barrier();   // U is there
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
-        if (s > w / 2) continue;
+        if (s >= steps) continue;
 #pragma unroll
-        for (int a = 0; a < PO; ++a) {
-          const bf16x8 x = frag(per[(W::kT + (triangle(w) + s) * PO + a) * 64]);
+        for (int b = PO - 1; b >= 0; --b) {
+          const bf16x8 y = frag(uf[b][s][lane]);
 #pragma unroll
-          for (int b = PO - 1 - a; b >= 0; --b) {
-            float4v& to = a + b ? low : acc;
-            to = mma(x, frag(uf[b][s][lane]), to);
-          }
+          for (int a = 0; a + b < PO; ++a) acc[a + b] = mma(frag(a2[s][a]), y, acc[a + b]);
         }
       }
-      acc += low;
+      load2(next, few);
+      acc[0] += acc[1] + acc[2];
+      const uint32_t token = c * kChunk + 16 * w + 4 * j;
+      T* out = static_cast<T*>(A.o) + (int64_t)first * A.o_token + head * A.o_head + col;
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        if (token + e < (int)count)
-          static_cast<T*>(A.o)[(int64_t)(first + token + e) * A.o_token + head * A.o_head + col] = (T)acc[e];
+        if (token + e < count) out[(int64_t)(token + e) * A.o_token] = (T)acc[0][e];
     }
-  }
-  if (chain && A.state_out) {
-#pragma unroll
-    for (int t = 0; t < TPW; ++t)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) A.state_out[at + (size_t)(16 * t + e) * A.dv] = state[t][e];
   }
 }
 
