@@ -433,10 +433,10 @@ __global__ __launch_bounds__(256) void delta_prepare(ChunkArgs C) {
 //
 // A chunk costs three barriers and the products between them, so nothing may
 // wait for memory there: each operand's registers are filled for the next chunk
-// as soon as this one's product has read them (kAhead; with fp32's 54 operands
-// at dk 256, which do not fit, K's rows and dims take turns). The two kinds of
-// wavefronts have loops of their own, so that neither's loads are waited for on
-// account of the other's.
+// in the phase after the product that read them, behind that phase's LDS reads
+// (kAhead; with fp32's 54 operands at dk 256, which do not fit, K's rows and
+// dims take turns). The two kinds of wavefronts have loops of their own, so that
+// neither's loads are waited for on account of the other's.
 template <typename T, int DK>
 __global__ __launch_bounds__(512) void delta_scan(ChunkArgs C) {
   typedef Room<T, DK> W;
@@ -511,11 +511,19 @@ __global__ __launch_bounds__(512) void delta_scan(ChunkArgs C) {
           for (int a = 0; a < N; ++a) a3[t][s][a] = p[((t * 2 + s) * N + a) * 64];
       last = reinterpret_cast<const float*>(per - lane + c * per_next + (W::kT + W::kP) * 64)[kLast];
     };
-    auto load_v = [&](uint32_t c) {
-      const T* x = static_cast<const T*>(A.v) + (int64_t)first * A.v_token + head * A.v_head + col;
-      const uint32_t token = c * kChunk + 16 * w + 4 * j;
+    const T* values = static_cast<const T*>(A.v) + (int64_t)first * A.v_token + head * A.v_head + col;
+    const T* mine[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = x[(int64_t)min(token + e, count - 1) * A.v_token];
+    for (int e = 0; e < 4; ++e) mine[e] = values + (int64_t)(16 * w + 4 * j + e) * A.v_token;
+    auto load_v = [&](uint32_t c) {
+      if ((c + 1) * kChunk <= count) {
+        const int64_t on = (int64_t)(c * kChunk) * A.v_token;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = mine[e][on];
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = values[(int64_t)min(c * kChunk + 16 * w + 4 * j + e, count - 1) * A.v_token];
+      }
       row_scale = scalars(c, kRowK);
     };
     // S's operands go by dims in their order, as rows of K and Q lie in memory.
@@ -536,62 +544,76 @@ __global__ __launch_bounds__(512) void delta_scan(ChunkArgs C) {
       for (int e = 0; e < 4; ++e) state[t][e] = A.state_in ? A.state_in[at + (size_t)(16 * t + e) * A.dv] : 0.f;
       put_state(t, state[t]);
     }
+    // The chain is what the chunk's time is: its instructions go first.
+    __builtin_amdgcn_s_setprio(3);
     for (uint32_t c = 0; c < chunks; ++c) {
       const uint32_t next = c + 1 < chunks ? c + 1 : c;
       lds_barrier();   // S is there
       float4v x[3] = {};
+      bf16x8 y[3][2];
+      if constexpr (kAhead) {
+        if (c) load3(c);
+      }
 #pragma unroll
       for (int s = 0; s < KS; ++s)
 #pragma unroll
         for (int b = 2; b >= 0; --b) {
-          const bf16x8 y = frag(sf[b][s][lane]);
+          const bf16x8 z = frag(sf[b][s][lane]);
 #pragma unroll
-          for (int a = 0; a < N && a + b <= 2; ++a) x[a + b] = mma(frag(a1[s][a]), y, x[a + b]);
+          for (int a = 0; a < N && a + b <= 2; ++a) x[a + b] = mma(frag(a1[s][a]), z, x[a + b]);
         }
       const uint32_t token = c * kChunk + 16 * w + 4 * j;
       float4v r;
 #pragma unroll
       for (int e = 0; e < 4; ++e) r[e] = token + e < count ? (float)v[e] : 0.f;
       r -= row_scale * (x[0] + (x[1] + x[2]));
+      put(&rf[0][w / 2][0], 2 * 64, j, w % 2, r, three);
+      lds_barrier();   // V - e^G K S is there, and S is read
+#pragma unroll
+      for (int b = 2; b >= 0; --b)
+#pragma unroll
+        for (int s = 0; s < 2; ++s) y[b][s] = frag(rf[b][s][lane]);
+      __builtin_amdgcn_sched_barrier(0);
       if constexpr (kAhead) load1(next);
       else load3(c);
       load_v(next);
-      put(&rf[0][w / 2][0], 2 * 64, j, w % 2, r, three);
-      lds_barrier();   // V - e^G K S is there, and S is read
+      __builtin_amdgcn_sched_barrier(0);
       float4v u[3] = {};
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
         if (s >= steps) continue;
 #pragma unroll
-        for (int b = 2; b >= 0; --b) {
-          const bf16x8 y = frag(rf[b][s][lane]);
+        for (int b = 2; b >= 0; --b)
 #pragma unroll
-          for (int a = 0; a + b <= 2; ++a) u[a + b] = mma(frag(a2[s][a]), y, u[a + b]);
-        }
+          for (int a = 0; a + b <= 2; ++a) u[a + b] = mma(frag(a2[s][a]), y[b][s], u[a + b]);
       }
       u[0] += u[1] + u[2];
-      put(&uf[0][w / 2][0], 2 * 64, j, w % 2, u[0], few);
       put(&wf[0][w / 2][0], 2 * 64, j, w % 2, u[0] * col_scale, three);
+      put(&uf[0][w / 2][0], 2 * 64, j, w % 2, u[0], few);
+      lds_barrier();   // U is there
+#pragma unroll
+      for (int b = 2; b >= 0; --b)
+#pragma unroll
+        for (int s = 0; s < 2; ++s) y[b][s] = frag(wf[b][s][lane]);
+      __builtin_amdgcn_sched_barrier(0);
       load2(next, three);
       col_scale = scalars(next, kColU);
-      lds_barrier();   // U is there
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int t = 0; t < TPW; ++t) {
         float4v z[3] = {};
 #pragma unroll
         for (int s = 0; s < 2; ++s)
 #pragma unroll
-          for (int b = 2; b >= 0; --b) {
-            const bf16x8 y = frag(wf[b][s][lane]);
+          for (int b = 2; b >= 0; --b)
 #pragma unroll
-            for (int a = 0; a < N && a + b <= 2; ++a) z[a + b] = mma(frag(a3[t][s][a]), y, z[a + b]);
-          }
+            for (int a = 0; a < N && a + b <= 2; ++a) z[a + b] = mma(frag(a3[t][s][a]), y[b][s], z[a + b]);
         state[t] = last * state[t] + (z[0] + (z[1] + z[2]));
         put_state(t, state[t]);
       }
-      if constexpr (kAhead) load3(next);
-      else load1(next);
+      if constexpr (!kAhead) load1(next);
     }
+    __builtin_amdgcn_s_setprio(0);
     if (A.state_out) {
 #pragma unroll
       for (int t = 0; t < TPW; ++t)
