@@ -1,6 +1,7 @@
 // q4.hip - products with 4-bit weights and group scales (fr_hip_q4_product):
 //     y[t][n] = sum_g scale[n][g] sum_{k in g} x[t][k] (code[n][k] - zero[n][g]) .
 #include <limits.h>
+#include <math.h>
 
 #include <type_traits>
 
@@ -16,7 +17,7 @@ struct Q4Args {
   void* y;
   int64_t x_token, y_token;
   uint32_t tokens, rows, cols, groups;
-  bool bf16_scales, wide;   // wide: x rows are of whole 16 bytes
+  bool bf16_scales, wide, wide_y;   // wide: rows of x (of y) are of whole 16 bytes
 };
 
 // The matrix cores' operand type: fp16 activations meet fp16 codes, all others
@@ -226,6 +227,267 @@ __global__ __launch_bounds__(512) void q4_rows(Q4Args A) {
   }
 }
 
+// ------------------------------------------------------------ many tokens
+//
+// From a block of tokens on, W is decoded for 64 tokens at a time straight into
+// the wavefronts that multiply it, and x is laid out beforehand (q4_pack) as the
+// operands that all of them share through LDS.
+//
+// Both operands are fp16 here, where two codes are numbers after two packed
+// instructions: 0x6400 | c is 1024 + c, and with c four bits higher 1024 + 16 c,
+// so that one packed add or fma gives c - zero exactly. fp16 activations go as
+// they are; a bf16 token is scaled by the power of two that brings its largest
+// to 2^14 .. 2^15, which keeps every value down to 2^-32 of the largest exact
+// and the others to 2^-40 of it, below fp32's rounding of their sum; an fp32
+// token takes two such parts (2^-23 of each value).
+constexpr int kTokens = 64;
+
+template <typename T> struct Packed { static constexpr int kParts = std::is_same<T, float>::value ? 2 : 1; };
+
+struct TileArgs {
+  Q4Args a;
+  uint4v* packed;      // [block of 128 columns][tile of 16 tokens][part][step][lane]
+  int32_t* exponent;   // of each token
+  uint32_t tiles;      // of tokens, a multiple of 4
+  bool whole;          // scales (and zeros) of a block of columns are aligned words
+};
+
+// One workgroup: 16 tokens, and every gridDim.y-th sixteenth of their operands.
+template <typename T, int G>
+__global__ __launch_bounds__(1024) void q4_pack(TileArgs C) {
+  const Q4Args& A = C.a;
+  constexpr int P = Packed<T>::kParts;
+  constexpr bool kScaled = !std::is_same<T, _Float16>::value;
+  __shared__ uint32_t largest[16];
+  const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, j = lane >> 4, tile = blockIdx.x;
+  if constexpr (kScaled) {
+    uint32_t top = 0;
+    if (tile * 16 + wave < A.tokens) {
+      const T* x = static_cast<const T*>(A.x) + (int64_t)(tile * 16 + wave) * A.x_token;
+      for (uint32_t c = lane * 8; c < A.cols; c += 512) {
+        float v[8];
+        load_row<8>(x + c, A.wide, v);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) top = max(top, __builtin_bit_cast(uint32_t, v[e]) & 0x7fffffffu);
+      }
+    }
+    for (int d = 1; d < 64; d *= 2) top = max(top, (uint32_t)__shfl_xor((int)top, d));
+    if (lane == 0) largest[wave] = top;
+    __syncthreads();
+  }
+  const uint32_t top = kScaled ? largest[i] : 0;
+  const bool finite = top < 0x7f800000u;
+  const int shift = kScaled ? 141 - (int)max(top >> 23, 1u) : 0;
+  if (blockIdx.y == 0 && wave == 0 && j == 0) C.exponent[tile * 16 + i] = finite ? -shift : 0;
+  const uint32_t pieces = (A.cols + 127) / 128 * 4;
+  const T* x = static_cast<const T*>(A.x) + (int64_t)(tile * 16 + i) * A.x_token;
+  for (uint32_t f = blockIdx.y * 16 + wave; f < pieces; f += gridDim.y * 16) {
+    const uint32_t kb = f / 4, s = f % 4, c = kb * 128 + (G == 128 ? 32 * j + 8 * s : 32 * s + 8 * j);
+    float v[8] = {};
+    if (tile * 16 + i < A.tokens && c < A.cols) load_row<8>(x + c, A.wide, v);
+    half8v out[P];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      // The order in which a word of codes is decoded: 0 4 1 5 2 6 3 7.
+      const float y = v[e / 2 + e % 2 * 4];
+      const float z = kScaled ? (finite ? ldexpf(y, shift) : NAN) : y;
+      out[0][e] = (_Float16)z;
+      if constexpr (P == 2) out[1][e] = (_Float16)(z - (float)out[0][e]);
+    }
+#pragma unroll
+    for (int p = 0; p < P; ++p)
+      C.packed[(((size_t)kb * C.tiles + tile) * P + p) * 256 + s * 64 + lane] = __builtin_bit_cast(uint4v, out[p]);
+  }
+}
+
+__device__ __forceinline__ half8v minus_zero(uint32_t w, half2v z1024, half2v z64) {
+  const half2v sixteenth = {(_Float16)0.0625f, (_Float16)0.0625f};
+  const half2v a = __builtin_bit_cast(half2v, (w & 0x000f000fu) | 0x64006400u) + z1024;
+  const half2v b = __builtin_bit_cast(half2v, (w & 0x00f000f0u) | 0x64006400u) * sixteenth + z64;
+  w >>= 8;
+  const half2v c = __builtin_bit_cast(half2v, (w & 0x000f000fu) | 0x64006400u) + z1024;
+  const half2v d = __builtin_bit_cast(half2v, (w & 0x00f000f0u) | 0x64006400u) * sixteenth + z64;
+  return {a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+
+// One workgroup: 64 tokens by 64 NT rows of W. Its two halves of four wavefronts
+// take every other block of 128 columns and join through LDS; a wavefront has
+// 16 NT rows of its own, which nothing else decodes, and all of the tokens.
+// A block's x and codes are asked for while the one before is multiplied. One
+// group's sums are formed from zero and enter the result times their scale, a
+// fused multiply-add for every 2 G operations of a lane's result.
+template <typename T, int G, int NT>
+__global__ __launch_bounds__(512) void q4_tiles(TileArgs C, uint32_t token_blocks) {
+  const Q4Args& A = C.a;
+  constexpr int P = Packed<T>::kParts, GPB = 128 / G, SB = G == 128 ? 4 : 2, SPG = G / 32 < SB ? G / 32 : SB;
+  constexpr int kPitch = 64 * NT + 4;
+  extern __shared__ uint4v lds[];   // [half][2][P * 1024], then the sums [64][kPitch]
+  const int lane = threadIdx.x & 63, i = lane & 15, j = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = wave >> 2, w = wave & 3;
+  // Workgroups go to the dies in turn: all blocks of tokens of the same rows to one.
+  const uint32_t tn = blockIdx.x % 8 + blockIdx.x / (8 * token_blocks) * 8, tm = blockIdx.x / 8 % token_blocks;
+  const uint32_t n0 = (tn * 4 + w) * 16 * NT;
+  if (tn * 64 * NT >= A.rows) return;
+
+  const uint32_t blocks = (A.cols + 127) / 128;
+  const uint8_t* code[NT];
+  size_t group0[NT];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    const uint32_t row = n0 + n * 16 + i < A.rows ? n0 + n * 16 + i : A.rows - 1;
+    code[n] = A.codes + (size_t)row * (A.cols / 2) + j * 16;
+    group0[n] = (size_t)row * A.groups;
+  }
+  struct Weights {
+    uint4v w[NT];
+    uint16_t scale[NT][GPB];
+    uint8_t zero[NT][GPB];
+  };
+  auto load_w = [&](uint32_t kb, Weights& b) {
+    const bool in = kb * 128 + j * 32 < A.cols;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      b.w[n] = uint4v{0, 0, 0, 0};
+      if (in) b.w[n] = *reinterpret_cast<const uint4v*>(code[n] + kb * 64);
+    }
+    if (GPB > 1 && C.whole) {
+      typedef uint16_t words __attribute__((ext_vector_type(GPB)));
+      typedef uint8_t bytes __attribute__((ext_vector_type(GPB)));
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        const size_t at = group0[n] + kb * GPB;
+        const words s = *reinterpret_cast<const words*>(A.scales + at);
+        bytes z = 8;
+        if (A.zeros) z = *reinterpret_cast<const bytes*>(A.zeros + at);
+#pragma unroll
+        for (int g = 0; g < GPB; ++g) b.scale[n][g] = s[g], b.zero[n][g] = z[g];
+      }
+    } else {
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int g = 0; g < GPB; ++g) {
+          const size_t at = group0[n] + (kb * GPB + g < A.groups ? kb * GPB + g : A.groups - 1);
+          b.scale[n][g] = A.scales[at];
+          b.zero[n][g] = A.zeros ? A.zeros[at] : 8;
+        }
+    }
+  };
+  uint4v stage[4 * P];
+  const int thread = threadIdx.x & 255;
+  auto load_x = [&](uint32_t kb) {
+    const uint4v* p = C.packed + ((size_t)kb * C.tiles + tm * 4) * P * 256 + thread;
+#pragma unroll
+    for (int n = 0; n < 4 * P; ++n) stage[n] = p[n * 256];
+  };
+  auto store_x = [&](int buffer) {
+#pragma unroll
+    for (int n = 0; n < 4 * P; ++n) lds[(half * 2 + buffer) * P * 1024 + n * 256 + thread] = stage[n];
+  };
+
+  float4v acc[4][NT] = {};
+  Weights cur, next;
+  if ((uint32_t)half < blocks) {
+    load_x(half);
+    load_w(half, cur);
+    store_x(0);
+  }
+  for (uint32_t it = 0; it * 2 < blocks; ++it) {
+    const uint32_t kb = it * 2 + half;
+    __syncthreads();   // this block's x is there, and the last one's is read
+    if (kb + 2 < blocks) {
+      load_x(kb + 2);
+      load_w(kb + 2, next);
+    }
+    if (kb < blocks) {
+      const uint4v* x = lds + (half * 2 + it % 2) * P * 1024 + lane;
+      uint32_t d[NT][4];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+#pragma unroll
+        for (int s = 0; s < 4; ++s) d[n][s] = cur.w[n][s];
+        if constexpr (G < 128) transpose4(d[n]);
+      }
+#pragma unroll
+      for (int sub = 0; sub < 4 / SB; ++sub) {
+        half8v b[NT][SB];
+        float scale[NT][SB / SPG];
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int g = 0; g < SB / SPG; ++g) {
+            const int at = (sub * SB + g * SPG) * 32 / G;
+            const float zero = (float)cur.zero[n][at];
+            const _Float16 z1 = (_Float16)(-1024.f - zero), z2 = (_Float16)(-64.f - zero);
+            scale[n][g] = scale_of(cur.scale[n][at], A.bf16_scales);
+#pragma unroll
+            for (int s = 0; s < SPG; ++s)
+              b[n][g * SPG + s] = minus_zero(d[n][sub * SB + g * SPG + s], half2v{z1, z1}, half2v{z2, z2});
+          }
+#pragma unroll
+        for (int m = 0; m < 4; ++m) {
+          half8v a[P][SB];
+#pragma unroll
+          for (int p = 0; p < P; ++p)
+#pragma unroll
+            for (int s = 0; s < SB; ++s) a[p][s] = __builtin_bit_cast(half8v, x[((m * P + p) * 4 + sub * SB + s) * 64]);
+#pragma unroll
+          for (int g = 0; g < SB / SPG; ++g) {
+            float4v c[NT] = {};
+#pragma unroll
+            for (int s = g * SPG; s < (g + 1) * SPG; ++s)
+#pragma unroll
+              for (int p = P - 1; p >= 0; --p)
+#pragma unroll
+                for (int n = 0; n < NT; ++n) c[n] = mma(a[p][s], b[n][s], c[n]);
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+              for (int r = 0; r < 4; ++r) acc[m][n][r] = fmaf(scale[n][g], c[n][r], acc[m][n][r]);
+          }
+        }
+      }
+    }
+    if (kb + 2 < blocks) {
+      store_x((it + 1) % 2);
+      cur = next;
+    }
+  }
+
+  __syncthreads();
+  float* sums = reinterpret_cast<float*>(lds);
+  auto each = [&](auto f) {
+#pragma unroll
+    for (int m = 0; m < 4; ++m)
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) f(sums[(m * 16 + 4 * j + r) * kPitch + (w * NT + n) * 16 + i], acc[m][n][r]);
+  };
+  if (half) each([](float& at, float x) { at = x; });
+  __syncthreads();
+  if (!half) each([](float& at, float x) { at += x; });
+  __syncthreads();
+  const uint32_t t0 = tm * kTokens, left = A.rows - tn * 64 * NT;
+  for (uint32_t e = threadIdx.x; e < kTokens * 8 * NT; e += 512) {
+    const uint32_t t = e / (8 * NT), n = e % (8 * NT) * 8;
+    if (t0 + t >= A.tokens) break;
+    const int ex = C.exponent[t0 + t];
+    T* y = static_cast<T*>(A.y) + (int64_t)(t0 + t) * A.y_token + tn * 64 * NT + n;
+    typedef T vec __attribute__((ext_vector_type(8)));
+    vec out;
+#pragma unroll
+    for (int r = 0; r < 8; ++r) out[r] = (T)ldexpf(sums[t * kPitch + n + r], ex);
+    if (A.wide_y && n + 8 <= left) {
+      *reinterpret_cast<vec*>(y) = out;
+    } else {
+#pragma unroll
+      for (int r = 0; r < 8; ++r)
+        if (n + r < left) y[r] = out[r];
+    }
+  }
+}
+
 // ---------------------------------------------------------------------- host
 
 int check(const fr_hip_q4* r) {
@@ -251,6 +513,51 @@ void launch_rows(const Q4Args& A, hipStream_t s) {
   hipLaunchKernelGGL((q4_rows<T, MT, 1, G>), grid, dim3(64 * waves), waves * MT * 16 * 16 * sizeof(float), s, A);
 }
 
+// From this many tokens on W is decoded for 64 of them at a time.
+constexpr unsigned kTilesFrom = 33;
+bool in_tiles(const fr_hip_q4* r) { return r->tokens >= kTilesFrom; }
+uint32_t token_blocks(const fr_hip_q4* r) { return (r->tokens + kTokens - 1) / kTokens; }
+size_t packed_units(const fr_hip_q4* r) {   // of 16 bytes
+  return (size_t)((r->cols + 127) / 128) * token_blocks(r) * 4 * 256 * (r->type == FR_HIP_F32 ? 2 : 1);
+}
+size_t workspace_bytes(const fr_hip_q4* r) {
+  if (!in_tiles(r) || !r->rows) return 0;
+  return packed_units(r) * 16 + (size_t)token_blocks(r) * kTokens * sizeof(int32_t);
+}
+
+template <typename T, int G, int NT>
+int launch_tiles(const TileArgs& C, uint32_t blocks, hipStream_t s) {
+  constexpr size_t x = (size_t)4 * Packed<T>::kParts * 1024 * 16, sums = (size_t)kTokens * (64 * NT + 4) * sizeof(float);
+  constexpr size_t lds = x > sums ? x : sums;
+  static const hipError_t wide = hipFuncSetAttribute(reinterpret_cast<const void*>(&q4_tiles<T, G, NT>),
+                                                     hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+  FRONK_CK(wide);
+  const uint32_t tiles = (C.a.rows + 64 * NT - 1) / (64 * NT);
+  hipLaunchKernelGGL((q4_tiles<T, G, NT>), dim3((tiles + 7) / 8 * 8 * blocks), dim3(512), lds, s, C, blocks);
+  return FR_HIP_OK;
+}
+
+template <typename T, int G>
+int launch_blocks(const fr_hip_q4* r, const Q4Args& A, void* workspace, hipStream_t s) {
+  constexpr unsigned GPB = 128 / G;
+  const uint32_t blocks = token_blocks(r);
+  TileArgs C;
+  C.a = A;
+  C.packed = static_cast<uint4v*>(workspace);
+  C.exponent = reinterpret_cast<int32_t*>(C.packed + packed_units(r));
+  C.tiles = blocks * 4;
+  C.whole = A.groups % GPB == 0 && (uintptr_t)A.scales % (2 * GPB) == 0 && (uintptr_t)A.zeros % GPB == 0;
+  const uint32_t pieces = (A.cols + 127) / 128 * 4;
+  hipLaunchKernelGGL((q4_pack<T, G>), dim3(C.tiles, pieces >= 64 ? 4 : 1), dim3(1024), 0, s, C);
+  // The widest tiles that still give every compute unit one. Those of 256 rows
+  // have no registers for a second part of x or for four groups a block.
+  const uint64_t columns = (A.rows + 63) / 64;
+  if constexpr (Packed<T>::kParts == 1 && G > 32)
+    if (columns * blocks >= 4 * 256) return launch_tiles<T, G, 4>(C, blocks, s);
+  if (columns * blocks >= 2 * 256) return launch_tiles<T, G, 2>(C, blocks, s);
+  return launch_tiles<T, G, 1>(C, blocks, s);
+}
+
 template <typename T, int MT>
 void launch_group(const Q4Args& A, unsigned group, hipStream_t s) {
   switch (group) {
@@ -261,26 +568,33 @@ void launch_group(const Q4Args& A, unsigned group, hipStream_t s) {
 }
 
 template <typename T>
-void launch_tokens(const Q4Args& A, unsigned group, hipStream_t s) {
+int launch(const fr_hip_q4* r, const Q4Args& A, void* workspace, hipStream_t s) {
+  const unsigned group = r->group;
+  if (in_tiles(r)) {
+    switch (group) {
+      case 32: return launch_blocks<T, 32>(r, A, workspace, s);
+      case 64: return launch_blocks<T, 64>(r, A, workspace, s);
+      default: return launch_blocks<T, 128>(r, A, workspace, s);
+    }
+  }
   const uint32_t rows = A.tokens * Operand<T>::kParts;
   if (rows <= 16) launch_group<T, 1>(A, group, s);
   else if (rows <= 32) launch_group<T, 2>(A, group, s);
   else launch_group<T, 4>(A, group, s);
+  return FR_HIP_OK;
 }
 
 }  // namespace
 
 extern "C" {
 
-size_t fr_hip_q4_workspace(const fr_hip_q4* req) {
-  (void)req;
-  return 0;
-}
+size_t fr_hip_q4_workspace(const fr_hip_q4* req) { return check(req) ? 0 : workspace_bytes(req); }
 
 int fr_hip_q4_product(const fr_hip_q4* req, void* workspace, size_t bytes, void* stream) {
-  (void)workspace, (void)bytes;
   int rc = check(req);
   if (rc) return rc;
+  const size_t need = workspace_bytes(req);
+  if (need && (!workspace || bytes < need || (uintptr_t)workspace % 16)) return FR_HIP_INVALID;
   hipStream_t s;
   unsigned cus;
   rc = fronk::enter(stream, &s, &cus);
@@ -292,11 +606,13 @@ int fr_hip_q4_product(const fr_hip_q4* req, void* workspace, size_t bytes, void*
   A.tokens = req->tokens, A.rows = req->rows, A.cols = req->cols, A.groups = req->cols / req->group;
   A.bf16_scales = req->scale_type == FR_HIP_BF16;
   A.wide = (uintptr_t)req->x % 16 == 0 && req->x_token % n == 0;
+  A.wide_y = (uintptr_t)req->y % 16 == 0 && req->y_token % n == 0;
   switch (req->type) {
-    case FR_HIP_F32: launch_tokens<float>(A, req->group, s); break;
-    case FR_HIP_F16: launch_tokens<_Float16>(A, req->group, s); break;
-    default: launch_tokens<__bf16>(A, req->group, s); break;
+    case FR_HIP_F32: rc = launch<float>(req, A, workspace, s); break;
+    case FR_HIP_F16: rc = launch<_Float16>(req, A, workspace, s); break;
+    default: rc = launch<__bf16>(req, A, workspace, s); break;
   }
+  if (rc) return rc;
   FRONK_CK(hipGetLastError());
   return FR_HIP_OK;
 }
