@@ -551,9 +551,6 @@ __global__ __launch_bounds__(512) void delta_scan(ChunkArgs C) {
       lds_barrier();   // S is there
       float4v x[3] = {};
       bf16x8 y[3][2];
-      if constexpr (kAhead) {
-        if (c) load3(c);
-      }
 #pragma unroll
       for (int s = 0; s < KS; ++s)
 #pragma unroll
@@ -611,7 +608,8 @@ __global__ __launch_bounds__(512) void delta_scan(ChunkArgs C) {
         state[t] = last * state[t] + (z[0] + (z[1] + z[2]));
         put_state(t, state[t]);
       }
-      if constexpr (!kAhead) load1(next);
+      if constexpr (kAhead) load3(next);
+      else load1(next);
     }
     __builtin_amdgcn_s_setprio(0);
     if (A.state_out) {

@@ -300,26 +300,37 @@ __global__ __launch_bounds__(1024) void q4_pack(TileArgs C) {
   }
 }
 
-__device__ __forceinline__ half8v minus_zero(uint32_t w, half2v z1024, half2v z64) {
+// What decoding needs in registers, where the compiler would otherwise put it
+// into each instruction and split the bit select into an and and an or.
+struct Magic {
+  uint32_t low = 0x000f000fu, high = 0x00f000f0u, base = 0x64006400u;
+  __device__ __forceinline__ Magic() { asm("" : "+s"(low), "+s"(high), "+v"(base)); }
+};
+__device__ __forceinline__ half8v minus_zero(uint32_t w, half2v z1024, half2v z64, const Magic& c) {
   const half2v sixteenth = {(_Float16)0.0625f, (_Float16)0.0625f};
-  const half2v a = __builtin_bit_cast(half2v, (w & 0x000f000fu) | 0x64006400u) + z1024;
-  const half2v b = __builtin_bit_cast(half2v, (w & 0x00f000f0u) | 0x64006400u) * sixteenth + z64;
-  w >>= 8;
-  const half2v c = __builtin_bit_cast(half2v, (w & 0x000f000fu) | 0x64006400u) + z1024;
-  const half2v d = __builtin_bit_cast(half2v, (w & 0x00f000f0u) | 0x64006400u) * sixteenth + z64;
-  return {a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+  auto pick = [&](uint32_t x, uint32_t mask) { return __builtin_bit_cast(half2v, (x & mask) | c.base); };
+  const uint32_t v = w >> 8;
+  const half2v a = pick(w, c.low) + z1024, b = pick(w, c.high) * sixteenth + z64;
+  const half2v d = pick(v, c.low) + z1024, e = pick(v, c.high) * sixteenth + z64;
+  return {a[0], a[1], b[0], b[1], d[0], d[1], e[0], e[1]};
 }
 
 // One workgroup: 64 tokens by 64 NT rows of W. Its two halves of four wavefronts
-// take every other block of 128 columns and join through LDS; a wavefront has
-// 16 NT rows of its own, which nothing else decodes, and all of the tokens.
-// A block's x and codes are asked for while the one before is multiplied. One
-// group's sums are formed from zero and enter the result times their scale, a
-// fused multiply-add for every 2 G operations of a lane's result.
-template <typename T, int G, int NT>
+// take half of the blocks of 128 columns each and join through LDS; a wavefront
+// has 16 NT rows of its own, which nothing else decodes, and all of the tokens.
+// Rows of W lie apart by powers of two more often than not, and then one block
+// of all rows lies in few channels of the L2: the halves and the tiles of one
+// die begin at different blocks.
+// A block's x and codes are asked for while the one before is multiplied, and 16
+// rows are decoded while the 16 before them are. One group's sums are formed
+// from zero and enter the result times their scale, a fused multiply-add for
+// every 2 G operations of a lane's result. Loads are never left out, not even
+// behind the last block: only then are those that a wait is for told from those
+// behind them.
+template <typename T, int G, int NT, bool ZEROS, bool WHOLE>
 __global__ __launch_bounds__(512) void q4_tiles(TileArgs C, uint32_t token_blocks) {
   const Q4Args& A = C.a;
-  constexpr int P = Packed<T>::kParts, GPB = 128 / G, SB = G == 128 ? 4 : 2, SPG = G / 32 < SB ? G / 32 : SB;
+  constexpr int P = Packed<T>::kParts, GPB = 128 / G, SPG = G / 32;
   constexpr int kPitch = 64 * NT + 4;
   extern __shared__ uint4v lds[];   // [half][2][P * 1024], then the sums [64][kPitch]
   const int lane = threadIdx.x & 63, i = lane & 15, j = lane >> 4;
@@ -330,13 +341,17 @@ __global__ __launch_bounds__(512) void q4_tiles(TileArgs C, uint32_t token_block
   if (tn * 64 * NT >= A.rows) return;
 
   const uint32_t blocks = (A.cols + 127) / 128;
-  const uint8_t* code[NT];
-  size_t group0[NT];
+  // The wavefront's first row, and the lane's from there (below 2^21 bytes).
+  const uint32_t row0 = n0 < A.rows ? n0 : A.rows - 1;
+  const uint8_t* codes = A.codes + (size_t)row0 * (A.cols / 2);
+  const uint16_t* scales = A.scales + (size_t)row0 * A.groups;
+  const uint8_t* zeros = ZEROS ? A.zeros + (size_t)row0 * A.groups : nullptr;
+  uint32_t code[NT], group0[NT];
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
-    const uint32_t row = n0 + n * 16 + i < A.rows ? n0 + n * 16 + i : A.rows - 1;
-    code[n] = A.codes + (size_t)row * (A.cols / 2) + j * 16;
-    group0[n] = (size_t)row * A.groups;
+    const uint32_t row = (n0 + n * 16 + i < A.rows ? n0 + n * 16 + i : A.rows - 1) - row0;
+    code[n] = row * (A.cols / 2) + j * 16;
+    group0[n] = row * A.groups;
   }
   struct Weights {
     uint4v w[NT];
@@ -344,33 +359,34 @@ __global__ __launch_bounds__(512) void q4_tiles(TileArgs C, uint32_t token_block
     uint8_t zero[NT][GPB];
   };
   auto load_w = [&](uint32_t kb, Weights& b) {
-    const bool in = kb * 128 + j * 32 < A.cols;
+    // Past the last column any codes do: x is zero there.
+    const uint32_t back = kb * 128 + j * 32 < A.cols ? 0 : j * 16;
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      b.w[n] = uint4v{0, 0, 0, 0};
-      if (in) b.w[n] = *reinterpret_cast<const uint4v*>(code[n] + kb * 64);
-    }
-    if (GPB > 1 && C.whole) {
+    for (int n = 0; n < NT; ++n) b.w[n] = *reinterpret_cast<const uint4v*>(codes + (size_t)kb * 64 + (code[n] - back));
+    if constexpr (GPB > 1 && WHOLE) {
       typedef uint16_t words __attribute__((ext_vector_type(GPB)));
       typedef uint8_t bytes __attribute__((ext_vector_type(GPB)));
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
-        const size_t at = group0[n] + kb * GPB;
-        const words s = *reinterpret_cast<const words*>(A.scales + at);
-        bytes z = 8;
-        if (A.zeros) z = *reinterpret_cast<const bytes*>(A.zeros + at);
+        const words s = *reinterpret_cast<const words*>(scales + kb * GPB + group0[n]);
+        bytes z;
+        if constexpr (ZEROS) z = *reinterpret_cast<const bytes*>(zeros + kb * GPB + group0[n]);
 #pragma unroll
-        for (int g = 0; g < GPB; ++g) b.scale[n][g] = s[g], b.zero[n][g] = z[g];
+        for (int g = 0; g < GPB; ++g) {
+          b.scale[n][g] = s[g];
+          if constexpr (ZEROS) b.zero[n][g] = z[g];
+        }
       }
     } else {
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
+      for (int g = 0; g < GPB; ++g) {
+        const uint32_t at = kb * GPB + g < A.groups ? kb * GPB + g : A.groups - 1;
 #pragma unroll
-        for (int g = 0; g < GPB; ++g) {
-          const size_t at = group0[n] + (kb * GPB + g < A.groups ? kb * GPB + g : A.groups - 1);
-          b.scale[n][g] = A.scales[at];
-          b.zero[n][g] = A.zeros ? A.zeros[at] : 8;
+        for (int n = 0; n < NT; ++n) {
+          b.scale[n][g] = scales[at + group0[n]];
+          if constexpr (ZEROS) b.zero[n][g] = zeros[at + group0[n]];
         }
+      }
     }
   };
   uint4v stage[4 * P];
@@ -386,72 +402,76 @@ __global__ __launch_bounds__(512) void q4_tiles(TileArgs C, uint32_t token_block
   };
 
   float4v acc[4][NT] = {};
-  Weights cur, next;
-  if ((uint32_t)half < blocks) {
-    load_x(half);
-    load_w(half, cur);
-    store_x(0);
-  }
-  for (uint32_t it = 0; it * 2 < blocks; ++it) {
-    const uint32_t kb = it * 2 + half;
+  const Magic magic;
+  auto compute = [&](const uint4v* x, const Weights& b) {
+    half8v a[4][P][4];
+#pragma unroll
+    for (int m = 0; m < 4; ++m)
+#pragma unroll
+      for (int p = 0; p < P; ++p)
+#pragma unroll
+        for (int s = 0; s < 4; ++s) a[m][p][s] = __builtin_bit_cast(half8v, x[((m * P + p) * 4 + s) * 64]);
+    half8v w[2][4];
+    auto decode = [&](int n) {
+      uint32_t d[4] = {b.w[n][0], b.w[n][1], b.w[n][2], b.w[n][3]};
+      if constexpr (G < 128) transpose4(d);
+#pragma unroll
+      for (int g = 0; g < GPB; ++g) {
+        // -(1024 + zero) by its bits, and 960 more than it.
+        const uint32_t z = ZEROS ? b.zero[n][g] : 8u;
+        const half2v z1 = __builtin_bit_cast(half2v, (z | z << 16) | 0xe400e400u);
+        const half2v z2 = z1 + half2v{(_Float16)960.f, (_Float16)960.f};
+#pragma unroll
+        for (int s = g * SPG; s < (g + 1) * SPG; ++s) w[n % 2][s] = minus_zero(d[s], z1, z2, magic);
+      }
+    };
+    decode(0);
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      if (n + 1 < NT) decode(n + 1);
+#pragma unroll
+      for (int g = 0; g < GPB; ++g) {
+        float4v c[4] = {};
+#pragma unroll
+        for (int s = g * SPG; s < (g + 1) * SPG; ++s)
+#pragma unroll
+          for (int p = P - 1; p >= 0; --p)
+#pragma unroll
+            for (int m = 0; m < 4; ++m) c[m] = mma(a[m][p][s], w[n % 2][s], c[m]);
+        const float scale = scale_of(b.scale[n][g], A.bf16_scales);
+#pragma unroll
+        for (int m = 0; m < 4; ++m)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) acc[m][n][r] = fmaf(scale, c[m][r], acc[m][n][r]);
+      }
+#pragma unroll
+      for (int k = 0; k < 16 * P; ++k) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);          // a matrix instruction,
+        __builtin_amdgcn_sched_group_barrier(0x002, P == 1 ? 4 : 2, 0);   // and what fits beside it
+      }
+    }
+  };
+
+  Weights b[2];
+  const uint32_t count = half ? blocks / 2 : (blocks + 1) / 2, from = half && count ? blocks - count : 0;
+  uint32_t at = count ? tn / 8 * 4 % count : 0;   // the block that is loaded next
+  auto load = [&](Weights& to) {
+    load_x(from + at);
+    load_w(from + at, to);
+    at = at + 1 < count ? at + 1 : 0;
+  };
+  load(b[0]);
+  store_x(0);
+  __builtin_amdgcn_s_waitcnt(0x0f70);   // all loads: the loop's own waits are then for its own
+  auto step = [&](uint32_t k, int buffer, const Weights& now, Weights& then) {
     __syncthreads();   // this block's x is there, and the last one's is read
-    if (kb + 2 < blocks) {
-      load_x(kb + 2);
-      load_w(kb + 2, next);
-    }
-    if (kb < blocks) {
-      const uint4v* x = lds + (half * 2 + it % 2) * P * 1024 + lane;
-      uint32_t d[NT][4];
-#pragma unroll
-      for (int n = 0; n < NT; ++n) {
-#pragma unroll
-        for (int s = 0; s < 4; ++s) d[n][s] = cur.w[n][s];
-        if constexpr (G < 128) transpose4(d[n]);
-      }
-#pragma unroll
-      for (int sub = 0; sub < 4 / SB; ++sub) {
-        half8v b[NT][SB];
-        float scale[NT][SB / SPG];
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-          for (int g = 0; g < SB / SPG; ++g) {
-            const int at = (sub * SB + g * SPG) * 32 / G;
-            const float zero = (float)cur.zero[n][at];
-            const _Float16 z1 = (_Float16)(-1024.f - zero), z2 = (_Float16)(-64.f - zero);
-            scale[n][g] = scale_of(cur.scale[n][at], A.bf16_scales);
-#pragma unroll
-            for (int s = 0; s < SPG; ++s)
-              b[n][g * SPG + s] = minus_zero(d[n][sub * SB + g * SPG + s], half2v{z1, z1}, half2v{z2, z2});
-          }
-#pragma unroll
-        for (int m = 0; m < 4; ++m) {
-          half8v a[P][SB];
-#pragma unroll
-          for (int p = 0; p < P; ++p)
-#pragma unroll
-            for (int s = 0; s < SB; ++s) a[p][s] = __builtin_bit_cast(half8v, x[((m * P + p) * 4 + sub * SB + s) * 64]);
-#pragma unroll
-          for (int g = 0; g < SB / SPG; ++g) {
-            float4v c[NT] = {};
-#pragma unroll
-            for (int s = g * SPG; s < (g + 1) * SPG; ++s)
-#pragma unroll
-              for (int p = P - 1; p >= 0; --p)
-#pragma unroll
-                for (int n = 0; n < NT; ++n) c[n] = mma(a[p][s], b[n][s], c[n]);
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-              for (int r = 0; r < 4; ++r) acc[m][n][r] = fmaf(scale[n][g], c[n][r], acc[m][n][r]);
-          }
-        }
-      }
-    }
-    if (kb + 2 < blocks) {
-      store_x((it + 1) % 2);
-      cur = next;
-    }
+    load(then);
+    if (k < count) compute(lds + (half * 2 + buffer) * P * 1024 + lane, now);
+    store_x(1 - buffer);
+  };
+  for (uint32_t k = 0; 2 * k < blocks; k += 2) {   // as often for both halves
+    step(k, 0, b[0], b[1]);
+    if (2 * k + 2 < blocks) step(k + 1, 1, b[1], b[0]);
   }
 
   __syncthreads();
@@ -525,16 +545,35 @@ size_t workspace_bytes(const fr_hip_q4* r) {
   return packed_units(r) * 16 + (size_t)token_blocks(r) * kTokens * sizeof(int32_t);
 }
 
-template <typename T, int G, int NT>
+template <typename T, int G, int NT, bool ZEROS, bool WHOLE>
 int launch_tiles(const TileArgs& C, uint32_t blocks, hipStream_t s) {
   constexpr size_t x = (size_t)4 * Packed<T>::kParts * 1024 * 16, sums = (size_t)kTokens * (64 * NT + 4) * sizeof(float);
   constexpr size_t lds = x > sums ? x : sums;
-  static const hipError_t wide = hipFuncSetAttribute(reinterpret_cast<const void*>(&q4_tiles<T, G, NT>),
+  static const hipError_t wide = hipFuncSetAttribute(reinterpret_cast<const void*>(&q4_tiles<T, G, NT, ZEROS, WHOLE>),
                                                      hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
   FRONK_CK(wide);
   const uint32_t tiles = (C.a.rows + 64 * NT - 1) / (64 * NT);
-  hipLaunchKernelGGL((q4_tiles<T, G, NT>), dim3((tiles + 7) / 8 * 8 * blocks), dim3(512), lds, s, C, blocks);
+  hipLaunchKernelGGL((q4_tiles<T, G, NT, ZEROS, WHOLE>), dim3((tiles + 7) / 8 * 8 * blocks), dim3(512), lds, s, C, blocks);
   return FR_HIP_OK;
+}
+template <typename T, int G, int NT, bool ZEROS>
+int launch_tiles(const TileArgs& C, uint32_t blocks, hipStream_t s) {
+  if constexpr (G < 128)
+    if (!C.whole) return launch_tiles<T, G, NT, ZEROS, false>(C, blocks, s);
+  return launch_tiles<T, G, NT, ZEROS, true>(C, blocks, s);
+}
+// The widest tiles that still give every compute unit one, as far as their
+// registers go: 256 rows leave none for a second part of x, zero points or
+// several groups a block, 128 rows none for both of the first and the last.
+template <typename T, int G, bool ZEROS>
+int launch_widest(const TileArgs& C, uint32_t blocks, hipStream_t s) {
+  constexpr int P = Packed<T>::kParts, kMost = P == 1 ? (G == 128 && !ZEROS ? 4 : 2) : G == 128 ? 2 : 1;
+  const uint64_t tiles = (uint64_t)((C.a.rows + 63) / 64) * blocks;
+  if constexpr (kMost >= 4)
+    if (tiles >= 4 * 256) return launch_tiles<T, G, 4, ZEROS>(C, blocks, s);
+  if constexpr (kMost >= 2)
+    if (tiles >= 2 * 256) return launch_tiles<T, G, 2, ZEROS>(C, blocks, s);
+  return launch_tiles<T, G, 1, ZEROS>(C, blocks, s);
 }
 
 template <typename T, int G>
@@ -549,13 +588,7 @@ int launch_blocks(const fr_hip_q4* r, const Q4Args& A, void* workspace, hipStrea
   C.whole = A.groups % GPB == 0 && (uintptr_t)A.scales % (2 * GPB) == 0 && (uintptr_t)A.zeros % GPB == 0;
   const uint32_t pieces = (A.cols + 127) / 128 * 4;
   hipLaunchKernelGGL((q4_pack<T, G>), dim3(C.tiles, pieces >= 64 ? 4 : 1), dim3(1024), 0, s, C);
-  // The widest tiles that still give every compute unit one. Those of 256 rows
-  // have no registers for a second part of x or for four groups a block.
-  const uint64_t columns = (A.rows + 63) / 64;
-  if constexpr (Packed<T>::kParts == 1 && G > 32)
-    if (columns * blocks >= 4 * 256) return launch_tiles<T, G, 4>(C, blocks, s);
-  if (columns * blocks >= 2 * 256) return launch_tiles<T, G, 2>(C, blocks, s);
-  return launch_tiles<T, G, 1>(C, blocks, s);
+  return A.zeros ? launch_widest<T, G, true>(C, blocks, s) : launch_widest<T, G, false>(C, blocks, s);
 }
 
 template <typename T, int MT>
