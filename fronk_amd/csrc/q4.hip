@@ -290,6 +290,7 @@ __global__ __launch_bounds__(1024) void q4_pack(TileArgs C) {
     uint32_t top = 0;
     if (tile * 16 + wave < A.tokens) {
       const T* x = static_cast<const T*>(A.x) + (int64_t)(tile * 16 + wave) * A.x_token;
+#pragma unroll 4
       for (uint32_t c = lane * 8; c < A.cols; c += 512) {
         float v[8];
         load_row<8>(x + c, A.wide, v);
@@ -600,8 +601,17 @@ int launch_rows(const Q4Args& A, bool whole, hipStream_t s) {
   return A.zeros ? launch_rows<T, MT, G, true, true>(C, grid, waves, s) : launch_rows<T, MT, G, false, true>(C, grid, waves, s);
 }
 
-// From this many tokens on W is decoded for 64 of them at a time.
-bool in_tiles(const fr_hip_q4* r) { return r->tokens > (r->type == FR_HIP_F32 ? 16 : 32); }
+// Tiles of 64 tokens, or rows for 32 (fp32: 16) at a time? Tiles cost 6 to 10 us
+// more to begin with (q4_pack, and x through one more launch), rows decode W once
+// for each of their blocks of tokens. Measured, rows against tiles in us, bf16 64
+// tokens: 15.0, 17.7 (2560 x 2560, 6400 cells), 18.1, 22.3 (4096 x 4096, 16384),
+// 26.4, 23.8 (4096 x 8192, 32768); 256 tokens of 2560 x 2560 (25600) 23.6, 19.5;
+// fp32 32 tokens of 4096 x 8192 (32768) 27.4, 37.6.
+bool in_tiles(const fr_hip_q4* r) {
+  const uint32_t tokens = r->type == FR_HIP_F32 ? 16 : 32;
+  const uint64_t cells = (uint64_t)((r->rows + 15) / 16) * ((r->cols + 127) / 128) * ((r->tokens + tokens - 1) / tokens);
+  return r->tokens > tokens && cells > (r->type == FR_HIP_F32 ? 48 << 10 : 24 << 10);
+}
 uint32_t token_blocks(const fr_hip_q4* r) { return (r->tokens + kTokens - 1) / kTokens; }
 size_t packed_units(const fr_hip_q4* r) {   // of 16 bytes
   return (size_t)padded_blocks(r->cols) * token_blocks(r) * 4 * 256 * (r->type == FR_HIP_F32 ? 2 : 1);

@@ -60,6 +60,60 @@ def test_chunks(tokens, rows, group, dtype):
     compare(5, tokens, 384, rows, group, dtype, group == 64)
 
 
+# Products large enough for tiles of 64 tokens: 64, 128 and 256 rows wide.
+TILED = [(200, 1856, 4096), (70, 1184, 16400), (260, 640, 16500)]
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("tokens,cols,rows,group,zeros", [(*TILED[0], 64, True), (*TILED[0], 32, False),
+                                                          (*TILED[1], 32, True), (*TILED[1], 32, False),
+                                                          (*TILED[2], 128, False), (*TILED[2], 128, True),
+                                                          (*TILED[2], 64, False)])
+def test_tiles(tokens, cols, rows, group, zeros, dtype):
+    compare(15, tokens, cols, rows, group, dtype, zeros, BF16 if group == 64 else F16)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+def test_tiles_views_and_bad_tokens(dtype):
+    """x and y at odd elements of wider rows; a token with an infinity or NaN
+    has no finite output and the others keep their bits; zeros and magnitudes
+    far from one in rows of their own."""
+    codes, scales, z = q4_weights(16, 8200, 1536, 128, True)
+    x = torch.randn(130, 1536, generator=gen(17))
+    x[5], x[6], x[7] = 0.0, x[6] * (2e3 if dtype == F16 else 1e30), x[7] * (2e-3 if dtype == F16 else 1e-30)
+    x[8] *= torch.logspace(-4, 3, 1536)
+    x = x.to(dtype)
+    want, size = q4(x, codes, scales, z)
+    wide = torch.full((130, 1541), float("nan"), dtype=dtype).cuda()
+    wide[:, 3:1539] = x.cuda()
+    out = torch.full((130, 8207), 4.0, dtype=dtype).cuda()
+    dev = [t.cuda() for t in (codes, scales, z)]
+    y = dense.q4_product(wide[:, 3:1539], *dev, out=out[:, 5:8205])
+    near(y, want, tolerance(want, size, dtype, 1536, 128) + (1e-36 if dtype != F16 else 2.0 ** -25), "y")
+    assert (out[:, :5] == 4.0).all() and (out[:, 8205:] == 4.0).all()
+    clean = y.clone()
+    wide[0, 80], wide[129, 700] = float("inf"), float("nan")
+    dense.q4_product(wide[:, 3:1539], *dev, out=out[:, 5:8205])
+    assert torch.equal(y[1:129], clean[1:129]) and not torch.isfinite(y[::129]).any()
+
+
+def test_tiles_in_a_graph():
+    codes, scales, _ = (t.cuda() if t is not None else None for t in q4_weights(18, 8200, 1536, 128, False))
+    x = torch.randn(130, 1536, generator=gen(19)).to(BF16).cuda()
+    keep = x.clone()
+    dense.q4_product(x, codes, scales)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = dense.q4_product(x, codes, scales)
+    for k in (1.0, -2.0, 0.5):
+        x.copy_(keep * k)
+        y.fill_(1.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, dense.q4_product(x, codes, scales))
+        torch.cuda.synchronize()
+
+
 @pytest.mark.parametrize("dtype", [BF16, F16, F32])
 @pytest.mark.parametrize("tokens", [2, 150])
 def test_bf16_scales(dtype, tokens):
