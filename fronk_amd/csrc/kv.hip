@@ -3,6 +3,8 @@
 #include <limits.h>
 #include <math.h>
 
+#include <type_traits>
+
 #include "bounds.h"
 #include "dense.h"
 
@@ -161,6 +163,7 @@ struct AttendArgs {
   uint32_t* status;
   int64_t q_token, q_head, o_token, o_head;
   uint32_t sequences, burst, heads, per, max_context, table_stride, splits, chunk, row_blocks;
+  uint32_t page16, reciprocal;   // blocks of 16 tokens a page, and 2^32 by it, rounded down
   float scale;
   bool wide;
 };
@@ -206,7 +209,7 @@ template <int N> __device__ __forceinline__ void split8(const float (&x)[8], bf1
 }
 
 template <typename T, int D, int RT>
-__global__ __launch_bounds__(256) void kv_attend(AttendArgs A) {
+__global__ __launch_bounds__(256, D * RT * (sizeof(T) == 4 ? 2 : 1) <= 256 ? 2 : 1) void kv_attend(AttendArgs A) {
   typedef Query<T> Q;
   typedef typename Q::frag frag;
   constexpr int QP = Q::kParts, PP = Q::kP, KS = D / 32, SEG = D / 64, DT = D / 16, R = 16 * RT;
@@ -216,8 +219,13 @@ __global__ __launch_bounds__(256) void kv_attend(AttendArgs A) {
     float o[R][kPad];
   } sh;
   __shared__ float stat[4][R][2];
-  const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, j = lane >> 4;
-  const uint32_t split = blockIdx.x % A.splits, item = blockIdx.x / A.splits;
+  const uint32_t lane = threadIdx.x & 63, i = lane & 15, j = lane >> 4;
+  const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  // Stretches vary slowest: neighbouring workgroups, which go to different dies,
+  // are the same stretch of different items, and contexts that end early leave
+  // work for all dies.
+  const uint32_t items = A.sequences * A.cache.heads * A.row_blocks;
+  const uint32_t split = blockIdx.x / items, item = blockIdx.x % items;
   const uint32_t rb = item % A.row_blocks, head = item / A.row_blocks % A.cache.heads;
   const uint32_t seq = item / A.row_blocks / A.cache.heads;
   const uint32_t rows = A.burst * A.per, row0 = rb * R;
@@ -229,6 +237,73 @@ __global__ __launch_bounds__(256) void kv_attend(AttendArgs A) {
   }
   const uint32_t begin = split * A.chunk;
   const uint32_t end = min((uint32_t)len, begin + A.chunk);   // chunk * splits < 2^31
+  const Cache& C = A.cache;
+  const int32_t* table = A.table + (size_t)seq * A.table_stride;
+
+  // The lane's blocks of 16 tokens of a tile, for K by its row, for V by j: what
+  // the table says, and where they begin (as exponents are counted). Blocks past
+  // the end are taken to be the last one.
+  struct Pages {
+    int32_t k, v;
+  };
+  struct Tile {
+    size_t k, v;
+    bool there;   // v's page
+  };
+  auto block_of = [&](uint32_t token, uint32_t* page, uint32_t* in) {
+    const uint32_t n = (token < end ? token : end - 1) >> 4;
+    uint32_t q = __umulhi(n, A.reciprocal), r = n - q * A.page16;   // q or one below
+    if (r >= A.page16) ++q, r -= A.page16;
+    *page = q, *in = r * 16;
+  };
+  auto look_up = [&](uint32_t base) {
+    uint32_t page, in;
+    Pages p;
+    block_of(base + (i >> 2) * 16, &page, &in);
+    p.k = table[page];
+    block_of(base + j * 16, &page, &in);
+    p.v = table[page];
+    return p;
+  };
+  bool bad = false;
+  auto locate = [&](uint32_t base, Pages p) {
+    uint32_t page, in;
+    Tile t;
+    const bool k = fronk::page_there(p.k, C.pages), v = fronk::page_there(p.v, C.pages);
+    block_of(base + (i >> 2) * 16, &page, &in);
+    t.k = exp_at(C, k ? (uint32_t)p.k : 0, head, in);
+    block_of(base + j * 16, &page, &in);
+    t.v = exp_at(C, v ? (uint32_t)p.v : 0, head, in);
+    t.there = v;
+    bad |= !v;   // (past the end it is the last block's page)
+    return t;
+  };
+  uint4v kc[4][SEG], vc[DT], ke, ve;
+  // What is not there is read from somewhere that is, and counts for nothing.
+  auto load_k = [&](const Tile& t) {
+    const uint8_t* p = C.k_codes + (t.k + (i & 3)) * D + j * 16;
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+      for (int s = 0; s < SEG; ++s) kc[r][s] = *reinterpret_cast<const uint4v*>(p + r * 4 * D + s * 64);
+    ke = *reinterpret_cast<const uint4v*>(C.k_exp + t.v);
+  };
+  auto load_v = [&](const Tile& t) {
+    ve = *reinterpret_cast<const uint4v*>(C.v_exp + t.v);
+    const uint8_t* p = C.v_codes + t.v * D + i * 16;
+#pragma unroll
+    for (int d = 0; d < DT; ++d) vc[d] = *reinterpret_cast<const uint4v*>(p + d * 256);
+  };
+  uint32_t base = begin + wave * 64;
+  Tile now;
+  Pages pages;   // of the tile after this one
+  if (base < end) {
+    const Pages first = look_up(base);
+    pages = look_up(base + 256);
+    now = locate(base, first);
+    load_k(now);
+    load_v(now);
+  }
 
   // Q, by operand: step ks of lane (i, j) holds dims 64 (ks / 2) + 16 j + 8 (ks % 2) ..
   if (begin < end) {
@@ -261,8 +336,10 @@ __global__ __launch_bounds__(256) void kv_attend(AttendArgs A) {
   for (int rt = 0; rt < RT; ++rt) {
     const uint32_t row = row0 + rt * 16 + i;
     const int32_t n = len - (int32_t)A.burst + (int32_t)(row / A.per) + 1;
-    limit[rt] = row < rows && n > 0 ? (uint32_t)n : 0;
+    // (what rows beyond the last would see is not of account)
+    limit[rt] = n <= 0 ? 0 : n < len ? (uint32_t)n : (uint32_t)len;
   }
+  const uint32_t all_see = (uint32_t)max(len - (int32_t)A.burst + 1, 0);
   float top[RT], sum[RT];
   float4v acc[RT][DT];
 #pragma unroll
@@ -271,50 +348,18 @@ __global__ __launch_bounds__(256) void kv_attend(AttendArgs A) {
 #pragma unroll
     for (int d = 0; d < DT; ++d) acc[rt][d] = float4v{0, 0, 0, 0};
   }
-  const Cache& C = A.cache;
   const float scale = A.scale * kLog2e;
 
-  for (uint32_t base = begin + wave * 64; base < end; base += 256) {
-    // The lane's block of 16 tokens for K (by its row) and for V (by j).
-    const uint32_t tk = base + (i >> 2) * 16, tv = base + j * 16;
-    const uint32_t pk = tk / C.page, pv = tv / C.page;
-    int32_t page_k = -1, page_v = -1;
-    if (tk < end) page_k = A.table[(size_t)seq * A.table_stride + pk];
-    if (tv < end) page_v = A.table[(size_t)seq * A.table_stride + pv];
-    const bool ok_k = fronk::page_there(page_k, C.pages), ok_v = fronk::page_there(page_v, C.pages);
-    if (tv < end && !ok_v && A.status) atomicOr(A.status, FR_HIP_BAD_PAGE);
-    uint4v kc[4][SEG], vc[DT], ke = {0, 0, 0, 0}, ve = {0, 0, 0, 0};
-    {
-      const uint8_t* p = C.k_codes + (ok_k ? exp_at(C, (uint32_t)page_k, head, tk - pk * C.page + (i & 3)) * D : 0) + j * 16;
-#pragma unroll
-      for (int t = 0; t < 4; ++t)
-#pragma unroll
-        for (int s = 0; s < SEG; ++s) {
-          kc[t][s] = uint4v{0, 0, 0, 0};
-          if (ok_k) kc[t][s] = *reinterpret_cast<const uint4v*>(p + t * 4 * D + s * 64);
-        }
+  // One tile. Its K's registers take the next tile's as soon as the scores are
+  // there (at dim 256, where they would be too many, with V's), V's as soon as the
+  // outputs are; the tile after that is looked up.
+  auto tile = [&](auto more) {
+    constexpr bool kMore = decltype(more)::value;
+    Tile next = now;
+    if constexpr (kMore) {
+      next = locate(base + 256, pages);
+      pages = look_up(base + 512);
     }
-    {
-      const size_t e = ok_v ? exp_at(C, (uint32_t)page_v, head, tv - pv * C.page) : 0;
-      if (ok_v) ke = *reinterpret_cast<const uint4v*>(C.k_exp + e), ve = *reinterpret_cast<const uint4v*>(C.v_exp + e);
-      const uint8_t* p = C.v_codes + e * D + i * 16;
-#pragma unroll
-      for (int d = 0; d < DT; ++d) {
-        vc[d] = uint4v{0, 0, 0, 0};
-        if (ok_v) vc[d] = *reinterpret_cast<const uint4v*>(p + d * 256);
-      }
-    }
-    // What lies past the end in a page was never written: its codes may be
-    // NaN, which no zero weight would take away.
-    if (base + 64 > end) {
-#pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        const uint32_t mask = fronk::first_bytes((int)end - (int)(tv + 4 * w));
-#pragma unroll
-        for (int d = 0; d < DT; ++d) vc[d][w] &= mask;
-      }
-    }
-
     float4v st[RT][4] = {};
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
@@ -332,25 +377,53 @@ __global__ __launch_bounds__(256) void kv_attend(AttendArgs A) {
           for (int p = QP - 1; p >= 0; --p) st[rt][t] = mma(a, qf[rt][p], st[rt][t]);
       }
     }
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const float x = power(ke[t] >> (8 * r) & 255) * scale;
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) st[rt][t][r] *= x;
+      }
+    if constexpr (kMore && D < 256) load_k(next);
 
+    // The tile's end, pages that are not there and tokens that a row does not
+    // see: weights of zero, and codes of zero, as they may be NaN.
+    const uint32_t tv = base + j * 16;
+    const bool masked = !__all(now.there) || base + 64 > all_see;
+    if (masked) {
+      const bool ok = now.there;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const uint32_t mask = ok ? fronk::first_bytes((int)end - (int)(tv + 4 * w)) : 0;
+#pragma unroll
+        for (int d = 0; d < DT; ++d) vc[d][w] &= mask;
+        ve[w] &= mask;
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (!ok || tv + 4 * w + r >= limit[rt]) st[rt][w][r] = -INFINITY;
+      }
+    }
     bf16x8 pf[RT][2][PP];
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-      float now = -INFINITY;
-      bool seen[4][4];
+    for (int rt = RT - 1; rt >= 0; --rt) {
+      // A token with infinities is nothing to a row that does not see it. Rows see
+      // more the later they are, so the last ones go first.
+      if (masked) {
+#pragma unroll
+        for (int t = 0; t < 4; ++t) ve[t] &= fronk::first_bytes((int)(limit[rt] - (tv + 4 * t)));
+      }
+      float most = -INFINITY;
 #pragma unroll
       for (int t = 0; t < 4; ++t)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          seen[t][r] = ok_v && tv + 4 * t + r < limit[rt];
-          const float x = st[rt][t][r] * power(ke[t] >> (8 * r) & 255) * scale;
-          st[rt][t][r] = seen[t][r] ? x : -INFINITY;
-          now = fmaxf(now, st[rt][t][r]);
-        }
-      now = fmaxf(top[rt], max_xor32(max_xor16(now)));
-      const float base_m = now == -INFINITY ? 0.f : now;
+        for (int r = 0; r < 4; ++r) most = fmaxf(most, st[rt][t][r]);
+      most = fmaxf(top[rt], max_xor32(max_xor16(most)));
+      const float base_m = most == -INFINITY ? 0.f : most;
       const float alpha = __builtin_amdgcn_exp2f(top[rt] - base_m);
-      top[rt] = now;
+      top[rt] = most;
       float total = 0, w[2][8];
 #pragma unroll
       for (int t = 0; t < 4; ++t)
@@ -358,7 +431,7 @@ __global__ __launch_bounds__(256) void kv_attend(AttendArgs A) {
         for (int r = 0; r < 4; ++r) {
           const float p = __builtin_amdgcn_exp2f(st[rt][t][r] - base_m);
           total += p;
-          w[t / 2][t % 2 * 4 + r] = seen[t][r] ? p * power(ve[t] >> (8 * r) & 255) : 0.f;
+          w[t / 2][t % 2 * 4 + r] = p * power(ve[t] >> (8 * r) & 255);
         }
       sum[rt] = sum[rt] * alpha + total;
       split8<PP>(w[0], pf[rt][0]);
@@ -378,6 +451,15 @@ __global__ __launch_bounds__(256) void kv_attend(AttendArgs A) {
 #pragma unroll
           for (int p = PP - 1; p >= 0; --p) acc[rt][d] = mma(a, pf[rt][s][p], acc[rt][d]);
       }
+    if constexpr (kMore && D == 256) load_k(next);
+    if constexpr (kMore) load_v(next);
+    now = next;
+    base += 256;
+  };
+  if (base < end) {
+    while (base + 256 < end) tile(std::true_type{});
+    tile(std::false_type{});
+    if (bad && A.status) atomicOr(A.status, FR_HIP_BAD_PAGE);
   }
 
   // Join the four wavefronts.
@@ -443,16 +525,18 @@ __global__ __launch_bounds__(256) void kv_attend(AttendArgs A) {
   }
 }
 
-// The stretches of one row joined, in their order.
-template <typename T, int D>
+// The stretches of one row joined, in their order; one workgroup takes L * 4 of
+// its dims.
+template <typename T, int D, int L>
 __global__ __launch_bounds__(256) void kv_merge(AttendArgs A, uint32_t R) {
-  constexpr uint32_t L = D / 4, G = 256 / L;
+  constexpr uint32_t G = 256 / L, kSlices = D / 4 / L;
   __shared__ float weight[256], red[4];
   __shared__ float4v part[G][L];
-  const uint32_t rows = A.burst * A.per;
-  const uint32_t row = blockIdx.x % rows, head = blockIdx.x / rows % A.cache.heads, seq = blockIdx.x / rows / A.cache.heads;
+  const uint32_t rows = A.burst * A.per, at_row = blockIdx.x / kSlices;
+  const uint32_t row = at_row % rows, head = at_row / rows % A.cache.heads, seq = at_row / rows / A.cache.heads;
   const uint32_t item = (seq * A.cache.heads + head) * A.row_blocks + row / R, at = row % R;
   const uint32_t s = threadIdx.x, wave = s >> 6;
+  const uint32_t c = s % L, g = s / L, d = (blockIdx.x % kSlices * L + c) * 4;
   float m = -INFINITY, l = 0;
   if (s < A.splits) {
     const float* p = A.part_ml + (((size_t)item * A.splits + s) * R + at) * 2;
@@ -472,18 +556,18 @@ __global__ __launch_bounds__(256) void kv_merge(AttendArgs A, uint32_t R) {
   if ((s & 63) == 0) red[wave] = l;
   __syncthreads();
   l = (red[0] + red[1]) + (red[2] + red[3]);
-  const uint32_t c = threadIdx.x % L, g = threadIdx.x / L;
   float4v x = {0, 0, 0, 0};
+#pragma unroll 4
   for (uint32_t k = g; k < A.splits; k += G) {
     const float w = weight[k];
-    if (w != 0.f) x += w * *reinterpret_cast<const float4v*>(A.part_o + (((size_t)item * A.splits + k) * R + at) * D + c * 4);
+    if (w != 0.f) x += w * *reinterpret_cast<const float4v*>(A.part_o + (((size_t)item * A.splits + k) * R + at) * D + d);
   }
   part[g][c] = x;
   __syncthreads();
   if (g) return;
   for (uint32_t k = 1; k < G; ++k) x += part[k][c];
   T* out = static_cast<T*>(A.o) + (int64_t)(seq * A.burst + row / A.per) * A.o_token +
-           (int64_t)(head * A.per + row % A.per) * A.o_head + c * 4;
+           (int64_t)(head * A.per + row % A.per) * A.o_head + d;
 #pragma unroll
   for (int e = 0; e < 4; ++e) out[e] = (T)(l == 0.f ? 0.f : x[e] / l);
 }
@@ -589,8 +673,11 @@ void launch_attend(const AttendArgs& A, const Cut& c, hipStream_t s) {
   const dim3 grid((uint32_t)(c.items * c.splits)), block(256);
   if (c.rt == 1) hipLaunchKernelGGL((kv_attend<T, D, 1>), grid, block, 0, s, A);
   else hipLaunchKernelGGL((kv_attend<T, D, 2>), grid, block, 0, s, A);
-  if (c.splits > 1)
-    hipLaunchKernelGGL((kv_merge<T, D>), dim3(A.sequences * A.burst * A.heads), block, 0, s, A, 16 * c.rt);
+  if (c.splits <= 1) return;
+  // Many stretches of few rows: several workgroups a row.
+  const uint32_t merges = A.sequences * A.burst * A.heads;
+  if (c.splits > 32) hipLaunchKernelGGL((kv_merge<T, D, 4>), dim3(merges * (D / 16)), block, 0, s, A, 16 * c.rt);
+  else hipLaunchKernelGGL((kv_merge<T, D, D / 4>), dim3(merges), block, 0, s, A, 16 * c.rt);
 }
 
 template <typename T>
@@ -644,6 +731,7 @@ int fr_hip_kv_attend(const fr_hip_kv_query* r, void* workspace, size_t bytes, vo
   A.q_token = r->q_token, A.q_head = r->q_head, A.o_token = r->o_token, A.o_head = r->o_head;
   A.sequences = r->sequences, A.burst = r->burst, A.heads = r->heads, A.per = r->heads / r->cache.heads;
   A.max_context = r->max_context, A.table_stride = r->table_stride;
+  A.page16 = r->cache.page / 16, A.reciprocal = 0xffffffffu / A.page16;
   A.splits = c.splits, A.chunk = c.chunk, A.row_blocks = c.row_blocks, A.scale = r->scale;
   A.wide = rows_wide(r->type, r->q, r->q, r->q_token, r->q_head, 0, 0);
   switch (r->type) {
