@@ -208,8 +208,13 @@ template <int N> __device__ __forceinline__ void split8(const float (&x)[8], bf1
     }
 }
 
+// Workgroups a compute unit that the registers are for: at dim 256, and with
+// fp32's parts at 32 rows, one that prefetches beats two that spill (131072
+// tokens at dim 256: 28 us against 33).
 template <typename T, int D, int RT>
-__global__ __launch_bounds__(256, D * RT * (sizeof(T) == 4 ? 2 : 1) <= 256 ? 2 : 1) void kv_attend(AttendArgs A) {
+constexpr int kResident = D == 256 || D * RT * (int)sizeof(T) > 512 ? 1 : 2;
+template <typename T, int D, int RT>
+__global__ __launch_bounds__(256, (kResident<T, D, RT>)) void kv_attend(AttendArgs A) {
   typedef Query<T> Q;
   typedef typename Q::frag frag;
   constexpr int QP = Q::kParts, PP = Q::kP, KS = D / 32, SEG = D / 64, DT = D / 16, R = 16 * RT;
@@ -351,8 +356,9 @@ __global__ __launch_bounds__(256, D * RT * (sizeof(T) == 4 ? 2 : 1) <= 256 ? 2 :
   const float scale = A.scale * kLog2e;
 
   // One tile. Its K's registers take the next tile's as soon as the scores are
-  // there (at dim 256, where they would be too many, with V's), V's as soon as the
-  // outputs are; the tile after that is looked up.
+  // there (with 32 rows of dim 256, where they would be too many, with V's), V's as
+  // soon as the outputs are; the tile after that is looked up.
+  constexpr bool kEarly = D * RT < 512;
   auto tile = [&](auto more) {
     constexpr bool kMore = decltype(more)::value;
     Tile next = now;
@@ -385,7 +391,7 @@ __global__ __launch_bounds__(256, D * RT * (sizeof(T) == 4 ? 2 : 1) <= 256 ? 2 :
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) st[rt][t][r] *= x;
       }
-    if constexpr (kMore && D < 256) load_k(next);
+    if constexpr (kMore && kEarly) load_k(next);
 
     // The tile's end, pages that are not there and tokens that a row does not
     // see: weights of zero, and codes of zero, as they may be NaN.
@@ -451,7 +457,7 @@ __global__ __launch_bounds__(256, D * RT * (sizeof(T) == 4 ? 2 : 1) <= 256 ? 2 :
 #pragma unroll
           for (int p = PP - 1; p >= 0; --p) acc[rt][d] = mma(a, pf[rt][s][p], acc[rt][d]);
       }
-    if constexpr (kMore && D == 256) load_k(next);
+    if constexpr (kMore && !kEarly) load_k(next);
     if constexpr (kMore) load_v(next);
     now = next;
     base += 256;
@@ -652,12 +658,14 @@ struct Cut {
 Cut cut_of(const fr_hip_kv_query* r) {
   Cut c;
   const uint32_t rows = r->burst * (r->heads / r->cache.heads);
-  c.rt = rows > 16 ? 2 : 1;
+  // fp32's parts of 32 rows of dim 256 would not fit the registers.
+  c.rt = rows > 16 && !(r->type == FR_HIP_F32 && r->cache.dim == 256) ? 2 : 1;
   c.row_blocks = (rows + 16 * c.rt - 1) / (16 * c.rt);
   c.items = (uint64_t)r->sequences * r->cache.heads * c.row_blocks;
-  // About two workgroups for each of 256 compute units, none with less than a
-  // tile for each of its wavefronts.
-  const uint64_t want = c.items ? (512 + c.items - 1) / c.items : 1, most = (r->max_context + 255) / 256;
+  // About one workgroup for each of 256 compute units (two: 131072 tokens of one
+  // stream 34 + 6 us against 28 + 5, a ragged batch of 32 the same), none with less
+  // than a tile for each of its wavefronts.
+  const uint64_t want = c.items ? (256 + c.items - 1) / c.items : 1, most = (r->max_context + 255) / 256;
   uint64_t n = want < most ? want : most;
   n = n < 1 ? 1 : n > 256 ? 256 : n;
   c.chunk = (uint32_t)((r->max_context + n * 256 - 1) / (n * 256)) * 256;
@@ -671,8 +679,12 @@ Cut cut_of(const fr_hip_kv_query* r) {
 template <typename T, int D>
 void launch_attend(const AttendArgs& A, const Cut& c, hipStream_t s) {
   const dim3 grid((uint32_t)(c.items * c.splits)), block(256);
-  if (c.rt == 1) hipLaunchKernelGGL((kv_attend<T, D, 1>), grid, block, 0, s, A);
-  else hipLaunchKernelGGL((kv_attend<T, D, 2>), grid, block, 0, s, A);
+  if constexpr (!(std::is_same<T, float>::value && D == 256)) {
+    if (c.rt == 1) hipLaunchKernelGGL((kv_attend<T, D, 1>), grid, block, 0, s, A);
+    else hipLaunchKernelGGL((kv_attend<T, D, 2>), grid, block, 0, s, A);
+  } else {
+    hipLaunchKernelGGL((kv_attend<T, D, 1>), grid, block, 0, s, A);
+  }
   if (c.splits <= 1) return;
   // Many stretches of few rows: several workgroups a row.
   const uint32_t merges = A.sequences * A.burst * A.heads;
