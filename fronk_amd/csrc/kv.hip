@@ -45,93 +45,179 @@ struct KvArgs {
   bool wide;
 };
 
-__device__ __forceinline__ int place(const KvArgs& A, uint32_t t, uint32_t* page, uint32_t* at) {
-  return fronk::locate(A.slot[t], A.cache.page, A.cache.pages, page, at);
-}
-
-// One vector (token, head, k or v) to D / 4 lanes, four values each.
-template <typename T, int D>
-__global__ __launch_bounds__(256) void kv_append(KvArgs A) {
-  constexpr uint32_t L = D / 4;
-  const uint64_t item = ((uint64_t)blockIdx.x * 256 + threadIdx.x) / L;
-  const uint32_t lane = threadIdx.x % L;
-  const uint32_t h = (uint32_t)(item / 2 % A.cache.heads);
-  const uint64_t t = item / 2 / A.cache.heads;
-  const bool is_v = item & 1;
-  if (t >= A.tokens) return;   // whole rows of 16 lanes: their reductions stay whole
-  uint32_t page, at;
-  const int there = place(A, (uint32_t)t, &page, &at);
-  if (there != 1) {
-    if (there == 2 && A.status && lane == 0) atomicOr(A.status, FR_HIP_BAD_SLOT);
-    return;
-  }
-  const T* src = is_v ? static_cast<const T*>(A.v) + (int64_t)t * A.v_token + h * A.v_head
-                      : static_cast<const T*>(A.k) + (int64_t)t * A.k_token + h * A.k_head;
-  float x[4];
-  load_row<4>(src + lane * 4, A.wide, x);
-  // The largest magnitude as bits, which order like it and put infinity and
-  // NaN on top.
+// Four of a vector's values as codes, the vector being in L lanes; its exponent.
+template <uint32_t L> __device__ __forceinline__ uint32_t quantize(const float (&x)[4], uint32_t* exponent) {
+  // The largest magnitude as bits, which order like it and put infinity and NaN
+  // on top.
   uint32_t top = 0;
 #pragma unroll
   for (int e = 0; e < 4; ++e) top = max(top, __builtin_bit_cast(uint32_t, x[e]) & 0x7fffffffu);
   top = umax_rotate(top);
   if constexpr (L > 16) top = max(top, (uint32_t)__shfl_xor((int)top, 16));
   if constexpr (L > 32) top = max(top, (uint32_t)__shfl_xor((int)top, 32));
-  const bool finite = top < 0x7f800000u;
   const int raw = (int)(top >> 23) - 8 + ((top & 0x7fffffu) > 0x600000u);
-  const uint32_t e = finite ? (uint32_t)max(raw, 1) : 255u;
-  const float m = finite ? __builtin_bit_cast(float, (254u - e) << 23) : 0.f;
-  uint32_t codes = 0;
-  if (finite) {
-    codes = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(x[0] * m, x[1] * m, 0, false);
-    codes = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(x[2] * m, x[3] * m, (int)codes, true);
+  *exponent = (uint32_t)max(raw, 1);
+  if (top >= 0x7f800000u) {
+    *exponent = 255;
+    return 0;
   }
-  const Cache& C = A.cache;
-  if (is_v) {
-    uint8_t* out = C.v_codes + v_at(C, page, h, at) + lane * 64;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) out[16 * i] = (uint8_t)(codes >> (8 * i));
+  const float m = __builtin_bit_cast(float, (254u - *exponent) << 23);
+  const int codes = __builtin_amdgcn_cvt_pk_fp8_f32(x[0] * m, x[1] * m, 0, false);
+  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(x[2] * m, x[3] * m, codes, true);
+}
+// ... and as values, at a row of the output.
+template <typename T>
+__device__ __forceinline__ void put_values(T* out, uint32_t codes, uint32_t exponent, bool wide) {
+  const float m = power(exponent);
+  const auto a = __builtin_amdgcn_cvt_pk_f32_fp8(codes, false), b = __builtin_amdgcn_cvt_pk_f32_fp8(codes, true);
+  typedef T vec4 __attribute__((ext_vector_type(4)));
+  const vec4 y = {(T)(a[0] * m), (T)(a[1] * m), (T)(b[0] * m), (T)(b[1] * m)};
+  if (wide) {
+    *reinterpret_cast<vec4*>(out) = y;
   } else {
-    *reinterpret_cast<uint32_t*>(C.k_codes + exp_at(C, page, h, at) * D + lane * 4) = codes;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) out[i] = y[i];
   }
-  if (lane == 0) (is_v ? C.v_exp : C.k_exp)[exp_at(C, page, h, at)] = (uint8_t)e;
 }
 
-template <typename T, int D>
-__global__ __launch_bounds__(256) void kv_read(KvArgs A) {
+// One vector (token, head, k or v) to D / 4 lanes: all reads, and writes of few
+// tokens.
+template <typename T, int D, bool READ>
+__global__ __launch_bounds__(256) void kv_single(KvArgs A) {
   constexpr uint32_t L = D / 4;
-  const uint64_t item = ((uint64_t)blockIdx.x * 256 + threadIdx.x) / L;
-  const uint32_t lane = threadIdx.x % L;
-  const uint32_t h = (uint32_t)(item / 2 % A.cache.heads);
-  const uint64_t t = item / 2 / A.cache.heads;
-  const bool is_v = item & 1;
-  if (t >= A.tokens || !(is_v ? A.v : A.k)) return;
-  uint32_t page = 0, at = 0;
-  const int there = place(A, (uint32_t)t, &page, &at);
-  if (there == 2 && A.status && lane == 0) atomicOr(A.status, FR_HIP_BAD_SLOT);
   const Cache& C = A.cache;
-  uint32_t codes = 0;
-  float m = 0;
-  if (there == 1) {
-    if (is_v) {
-      const uint8_t* in = C.v_codes + v_at(C, page, h, at) + lane * 64;
+  const uint64_t item = ((uint64_t)blockIdx.x * 256 + threadIdx.x) / L, t = item / 2 / C.heads;
+  const uint32_t lane = threadIdx.x % L, h = (uint32_t)(item / 2 % C.heads);
+  const bool is_v = item & 1;
+  if (t >= A.tokens || !(is_v ? A.v : A.k)) return;   // whole rows of 16 lanes: their reductions stay whole
+  uint32_t page = 0, at = 0;
+  const int there = fronk::locate(A.slot[t], C.page, C.pages, &page, &at);
+  if (there == 2 && A.status && lane == 0) atomicOr(A.status, FR_HIP_BAD_SLOT);
+  if (!READ && there != 1) return;
+  T* row = (is_v ? static_cast<T*>(A.v) + (int64_t)t * A.v_token + h * A.v_head
+                 : static_cast<T*>(A.k) + (int64_t)t * A.k_token + h * A.k_head) + lane * 4;
+  uint8_t* v = C.v_codes + v_at(C, page, h, at) + lane * 64;
+  uint32_t* k = reinterpret_cast<uint32_t*>(C.k_codes + exp_at(C, page, h, at) * D + lane * 4);
+  uint8_t* exponent = (is_v ? C.v_exp : C.k_exp) + exp_at(C, page, h, at);
+  if constexpr (READ) {
+    uint32_t codes = 0, e = 1;
+    if (there == 1) {
+      e = *exponent;
+      if (is_v) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) codes |= (uint32_t)in[16 * i] << (8 * i);
-    } else {
-      codes = *reinterpret_cast<const uint32_t*>(C.k_codes + exp_at(C, page, h, at) * D + lane * 4);
+        for (int i = 0; i < 4; ++i) codes |= (uint32_t)v[16 * i] << (8 * i);
+      } else {
+        codes = *k;
+      }
     }
-    m = power((is_v ? C.v_exp : C.k_exp)[exp_at(C, page, h, at)]);
-  }
-  T* out = is_v ? static_cast<T*>(A.v) + (int64_t)t * A.v_token + h * A.v_head
-                : static_cast<T*>(A.k) + (int64_t)t * A.k_token + h * A.k_head;
-  const auto a = __builtin_amdgcn_cvt_pk_f32_fp8(codes, false), b = __builtin_amdgcn_cvt_pk_f32_fp8(codes, true);
-  typedef T vec __attribute__((ext_vector_type(4)));
-  const vec y = {(T)(a[0] * m), (T)(a[1] * m), (T)(b[0] * m), (T)(b[1] * m)};
-  if (A.wide) {
-    *reinterpret_cast<vec*>(out + lane * 4) = y;
+    put_values(row, codes, e, A.wide);
   } else {
+    float x[4];
+    load_row<4>(row, A.wide, x);
+    uint32_t e;
+    const uint32_t codes = quantize<L>(x, &e);
+    if (is_v) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) out[lane * 4 + i] = y[i];
+      for (int i = 0; i < 4; ++i) v[16 * i] = (uint8_t)(codes >> (8 * i));
+    } else {
+      *k = codes;
+    }
+    if (lane == 0) *exponent = (uint8_t)e;
+  }
+}
+
+// A prompt: one workgroup writes 16 tokens of one head. The V codes of one dim
+// of 16 neighbouring tokens lie together, and those of a token 16 bytes apart, so
+// they go through LDS: where the 16 slots are one block of the cache, a lane
+// writes a dim's 16 bytes at once; where they are not, four bytes where four
+// slots follow each other from a multiple of four, and single bytes otherwise.
+// (Reads share their lines in the caches and gain nothing from it.)
+constexpr int kWindow = 16;
+
+struct Window {
+  uint32_t page[kWindow], at[kWindow];
+  int there[kWindow];     // as of fronk::locate
+  int run[kWindow];       // 4: first of four that lie together, 1: by itself, 0: one of four, or not there
+  bool block;             // all 16 are one block
+};
+// By the workgroup's first wavefront; to be followed by a barrier.
+__device__ __forceinline__ void look_up(const KvArgs& A, uint32_t t0, Window& w) {
+  if (threadIdx.x >= 64) return;
+  const uint32_t t = threadIdx.x;
+  uint32_t page = 0, at = 0;
+  const int32_t slot = t < kWindow && t0 + t < A.tokens ? A.slot[t0 + t] : -1;
+  const int there = fronk::locate(slot, A.cache.page, A.cache.pages, &page, &at);
+  if (there == 2 && A.status) atomicOr(A.status, FR_HIP_BAD_SLOT);
+  // Slots that follow each other from a multiple of 4 (16) are of one page.
+  const int32_t first = __shfl(slot, (int)(t & ~15u));
+  const bool block = __all(t >= kWindow || (there == 1 && slot == first + (int32_t)t && first % kWindow == 0));
+  bool four = t + 3 < kWindow && there == 1 && slot % 4 == 0;
+  bool of_four = false;
+#pragma unroll
+  for (int e = 1; e < 4; ++e) four &= __shfl_down(there, e) == 1 && __shfl_down(slot, e) == slot + e;
+#pragma unroll
+  for (int e = 1; e < 4; ++e) {
+    const bool before = __shfl_up((int)four, e);
+    of_four |= t >= (uint32_t)e && before;
+  }
+  if (t < kWindow) {
+    w.page[t] = page, w.at[t] = at, w.there[t] = there;
+    w.run[t] = there != 1 || of_four ? 0 : four ? 4 : 1;
+    if (t == 0) w.block = block;
+  }
+}
+
+// A vector (token, k or v) to D / 4 lanes, four values each.
+template <typename T, int D>
+__global__ __launch_bounds__(256) void kv_append(KvArgs A) {
+  constexpr uint32_t L = D / 4, kAtOnce = 256 / L, kPasses = 2 * kWindow / kAtOnce;
+  __shared__ Window w;
+  __shared__ __attribute__((aligned(16))) uint8_t v_tile[D][kWindow];
+  const Cache& C = A.cache;
+  const uint32_t h = blockIdx.x % C.heads, t0 = blockIdx.x / C.heads * kWindow, lane = threadIdx.x % L;
+  float x[kPasses][4];
+#pragma unroll
+  for (uint32_t p = 0; p < kPasses; ++p) {
+    const uint32_t vec = p * kAtOnce + threadIdx.x / L, t = vec % kWindow;
+    const int64_t token = t0 + t < A.tokens ? t0 + t : A.tokens - 1;
+    const T* src = vec / kWindow ? static_cast<const T*>(A.v) + token * A.v_token + h * A.v_head
+                                 : static_cast<const T*>(A.k) + token * A.k_token + h * A.k_head;
+    load_row<4>(src + lane * 4, A.wide, x[p]);
+  }
+  look_up(A, t0, w);
+  __syncthreads();
+#pragma unroll
+  for (uint32_t p = 0; p < kPasses; ++p) {
+    const uint32_t vec = p * kAtOnce + threadIdx.x / L, t = vec % kWindow;
+    const bool is_v = vec / kWindow;
+    uint32_t e;
+    const uint32_t codes = quantize<L>(x[p], &e);
+    if (is_v) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v_tile[lane * 4 + i][t] = (uint8_t)(codes >> (8 * i));
+    }
+    if (w.there[t] != 1) continue;
+    const size_t at = exp_at(C, w.page[t], h, w.at[t]);
+    if (!is_v) *reinterpret_cast<uint32_t*>(C.k_codes + at * D + lane * 4) = codes;
+    if (lane == 0) (is_v ? C.v_exp : C.k_exp)[at] = (uint8_t)e;
+  }
+  __syncthreads();
+  if (w.block) {
+    if (threadIdx.x < D)
+      *reinterpret_cast<uint4v*>(C.v_codes + v_at(C, w.page[0], h, w.at[0]) + threadIdx.x * 16) =
+          *reinterpret_cast<const uint4v*>(v_tile[threadIdx.x]);
+    return;
+  }
+  for (uint32_t u = threadIdx.x; u < D * kWindow; u += 256) {
+    const uint32_t d = u % D, t = u / D;
+    if (!w.run[t]) continue;
+    uint8_t* out = C.v_codes + v_at(C, w.page[t], h, w.at[t]) + d * 16;
+    if (w.run[t] == 4) {
+      const uint8_t* in = &v_tile[d][t];
+      *reinterpret_cast<uint32_t*>(out) = in[0] | in[1] << 8 | in[2] << 16 | (uint32_t)in[3] << 24;
+    } else {
+      *out = v_tile[d][t];
+    }
   }
 }
 
@@ -605,17 +691,32 @@ int check_tokens(const fr_hip_kv_cache* c, unsigned tokens, unsigned type, const
   if (tokens > INT_MAX || (tokens && (!slot || (both ? !k || !v : !k && !v)))) return FR_HIP_INVALID;
   if (((uintptr_t)k | (uintptr_t)v) % elem_size(type)) return FR_HIP_INVALID;
   if (rc) return rc;
+  // (heads, tokens and dims of a call in one-dimensional grids, with room to spare)
   return (uint64_t)tokens * c->heads * 2 * (c->dim / 4) / 256 >= INT_MAX ? FR_HIP_UNSUPPORTED : FR_HIP_OK;
 }
 
+// From this many values of K on, 16 tokens are written together. Measured, single
+// against together in us: 3.3, 6.9 (256 tokens, 2 heads of 256), 5.8, 4.7 (512, 8
+// of 128: 2^19 values), 10.2, 4.5 (4096, 4 of 64), 15.1, 8.5 (4096, 2 of 256).
+constexpr uint64_t kTogether = 1 << 19;
+
+template <typename T, int D, bool READ>
+void launch_dim(const KvArgs& A, hipStream_t s) {
+  const uint64_t vectors = (uint64_t)A.tokens * A.cache.heads;
+  const dim3 block(256);
+  if constexpr (!READ)
+    if (vectors * D >= kTogether) {
+      hipLaunchKernelGGL((kv_append<T, D>), dim3((A.tokens + kWindow - 1) / kWindow * A.cache.heads), block, 0, s, A);
+      return;
+    }
+  hipLaunchKernelGGL((kv_single<T, D, READ>), dim3((uint32_t)((vectors * 2 * (D / 4) + 255) / 256)), block, 0, s, A);
+}
 template <typename T, bool READ>
 void launch_tokens(const KvArgs& A, hipStream_t s) {
-  const uint64_t threads = (uint64_t)A.tokens * A.cache.heads * 2 * (A.cache.dim / 4);
-  const dim3 grid((uint32_t)((threads + 255) / 256)), block(256);
   switch (A.cache.dim) {
-    case 64: hipLaunchKernelGGL((READ ? kv_read<T, 64> : kv_append<T, 64>), grid, block, 0, s, A); break;
-    case 128: hipLaunchKernelGGL((READ ? kv_read<T, 128> : kv_append<T, 128>), grid, block, 0, s, A); break;
-    default: hipLaunchKernelGGL((READ ? kv_read<T, 256> : kv_append<T, 256>), grid, block, 0, s, A); break;
+    case 64: launch_dim<T, 64, READ>(A, s); break;
+    case 128: launch_dim<T, 128, READ>(A, s); break;
+    default: launch_dim<T, 256, READ>(A, s); break;
   }
 }
 

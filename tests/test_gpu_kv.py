@@ -61,6 +61,33 @@ def test_append_and_read(heads, page, dim, tokens, dtype):
         near(rv, vv.to(out_type), 0.0, "v")
 
 
+@pytest.mark.parametrize("dim,heads,tokens", [(64, 3, 130), (64, 64, 130), (128, 32, 131), (256, 16, 129)])
+@pytest.mark.parametrize("first", [0, 1, 4, 14, 16, 33])
+def test_runs_of_slots(first, dim, heads, tokens):
+    """Streams that begin at any place of a page, with a hole, a slot out of
+    order and pages in any order, written and read as whole blocks, in fours or
+    singly: the bytes of a search among all codes, and no others."""
+    r = gen(6)
+    page, pages = 48, 6
+    k, v = torch.randn(tokens, heads, dim, generator=r), torch.randn(tokens, heads, dim, generator=r)
+    order = torch.tensor([4, 1, 5, 0])
+    place = torch.arange(tokens) + first
+    slots = order[place // page] * page + place % page
+    slots[60], slots[[82, 83]] = -1, slots[[83, 82]]
+    cache = noise(dense.KVCache.empty(pages, heads, page, dim), 7)
+    want_k, want_v = (t.cpu().clone() for t in cache[:2])
+    dense.kv_append(cache, k.cuda(), v.cuda(), slots.to(torch.int32).cuda())
+    live = slots >= 0
+    pg, at = slots[live] // page, slots[live] % page
+    (kv, kq, _), (vv, vq, _) = held(k[live]), held(v[live])
+    want_k[pg, :, at], want_v[pg, :, at // 16, :, at % 16] = kq, vq
+    assert torch.equal(cache[0].cpu() & 0x7f, want_k & 0x7f) and torch.equal(cache[1].cpu() & 0x7f, want_v & 0x7f)
+    rk, rv = dense.kv_read(cache, slots.to(torch.int32).cuda(), F32)
+    near(rk[live], kv.float(), 0.0, "k")
+    near(rv[live], vv.float(), 0.0, "v")
+    assert (rk[~live] == 0).all() and (rv[~live] == 0).all()
+
+
 def test_append_extremes():
     """Zeros, subnormals, the largest, ties between codes, borders of the
     exponent, infinities and NaN."""
