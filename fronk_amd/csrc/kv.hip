@@ -56,14 +56,11 @@ template <uint32_t L> __device__ __forceinline__ uint32_t quantize(const float (
   if constexpr (L > 16) top = max(top, (uint32_t)__shfl_xor((int)top, 16));
   if constexpr (L > 32) top = max(top, (uint32_t)__shfl_xor((int)top, 32));
   const int raw = (int)(top >> 23) - 8 + ((top & 0x7fffffu) > 0x600000u);
-  *exponent = (uint32_t)max(raw, 1);
-  if (top >= 0x7f800000u) {
-    *exponent = 255;
-    return 0;
-  }
-  const float m = __builtin_bit_cast(float, (254u - *exponent) << 23);
+  const bool finite = top < 0x7f800000u;
+  *exponent = finite ? (uint32_t)max(raw, 1) : 255u;
+  const float m = __builtin_bit_cast(float, (254u - (uint32_t)max(raw, 1)) << 23);
   const int codes = __builtin_amdgcn_cvt_pk_fp8_f32(x[0] * m, x[1] * m, 0, false);
-  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(x[2] * m, x[3] * m, codes, true);
+  return finite ? (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(x[2] * m, x[3] * m, codes, true) : 0u;
 }
 // ... and as values, at a row of the output.
 template <typename T>
