@@ -90,17 +90,21 @@ def _need(ok, what):
         raise ValueError(what)
 
 
+# A call of one token is bounded by the host, so what is checked on every call
+# is checked in place, and messages are made only for a refusal.
+
 def _type(t, what):
-    _need(t.is_cuda, f"{what} is on the GPU")
     code = _TYPES.get(t.dtype)
-    _need(code is not None, f"{what} is float32, float16 or bfloat16")
+    if code is None or not t.is_cuda:
+        raise ValueError(f"{what} is float32, float16 or bfloat16, on the GPU")
     return code
 
 
 def _row(t, what):
-    """(strides, address) of a tensor whose last axis is contiguous."""
+    """The strides of a tensor whose last axis is contiguous."""
     s = t.stride()
-    _need(s[-1] == 1 or t.shape[-1] == 1, f"{what}'s last axis is contiguous")
+    if s[-1] != 1 and t.shape[-1] != 1:
+        raise ValueError(f"{what}'s last axis is contiguous")
     return s
 
 
@@ -108,13 +112,31 @@ def _ints(t, n, what):
     """The address of an int32 tensor of n elements."""
     if t is None:
         return None
-    _need(t.is_cuda and t.dtype == torch.int32 and t.is_contiguous() and t.numel() == n,
-          f"{what} is a contiguous int32 tensor of {n} on the GPU")
+    if t.dtype is not torch.int32 or t.numel() != n or not t.is_cuda or not t.is_contiguous():
+        raise ValueError(f"{what} is a contiguous int32 tensor of {n} on the GPU")
     return t.data_ptr()
 
 
-def _scratch(bytes_, device):
-    return torch.empty(bytes_, dtype=torch.uint8, device=device) if bytes_ else None
+def _pool(s, heads, key_dim, value_dim, what):
+    """(address, rows) of a state pool."""
+    if s is None:
+        return None, None
+    shape = s.shape
+    if (len(shape) != 4 or shape[1:] != (heads, key_dim, value_dim) or s.dtype is not torch.float32
+            or not s.is_cuda or not s.is_contiguous()):
+        raise ValueError(f"{what} is a contiguous fp32 [rows, heads, key_dim, value_dim]")
+    return s.data_ptr(), shape[0]
+
+
+def _run(name, workspace, request, device):
+    """The call with the workspace that it asks for."""
+    L, at = lib(), C.addressof(request)
+    n = getattr(L, workspace)(at)
+    if n:
+        w = torch.empty(n, dtype=torch.uint8, device=device)
+        _call(getattr(L, name), name, device.index, at, w.data_ptr(), n)
+    else:
+        _call(getattr(L, name), name, device.index, at, None, 0)
 
 
 def delta_rule(q, k, v, g, beta, state_in=None, state_out=None, *, scale=None, offsets=None, slots=None,
@@ -133,50 +155,53 @@ def delta_rule(q, k, v, g, beta, state_in=None, state_out=None, *, scale=None, o
     zeros / dropped. slots (int32, sequences): the pool row of each sequence,
     -1 to skip one; default row i."""
     code = _type(v, "v")
-    _need(q.dim() == 3 and k.shape == q.shape and v.dim() == 3 and v.shape[0] == q.shape[0],
-          "q and k are [tokens, key_heads, key_dim], v [tokens, heads, value_dim]")
-    _need(q.dtype == v.dtype and k.dtype == v.dtype and q.is_cuda and k.is_cuda, "q, k and v have one type and device")
-    tokens, key_heads, key_dim = q.shape
-    _, heads, value_dim = v.shape
-    _need(key_dim > 0, "key_dim is positive")
-    for t, what in ((g, "g"), (beta, "beta")):
-        _need(t.dtype == torch.float32 and t.is_cuda and t.shape == (tokens, heads), f"{what} is fp32 [tokens, heads]")
+    qshape, vshape = q.shape, v.shape
+    if len(qshape) != 3 or k.shape != qshape or len(vshape) != 3 or vshape[0] != qshape[0]:
+        raise ValueError("q and k are [tokens, key_heads, key_dim], v [tokens, heads, value_dim]")
+    if q.dtype is not v.dtype or k.dtype is not v.dtype or not q.is_cuda or not k.is_cuda:
+        raise ValueError("q, k and v have one type and device")
+    tokens, key_heads, key_dim = qshape
+    _, heads, value_dim = vshape
+    if key_dim <= 0:
+        raise ValueError("key_dim is positive")
+    scalars = (tokens, heads)
+    if (g.shape != scalars or beta.shape != scalars or g.dtype is not torch.float32
+            or beta.dtype is not torch.float32 or not g.is_cuda or not beta.is_cuda):
+        raise ValueError("g and beta are fp32 [tokens, heads]")
     if max_tokens is None:
         max_tokens = tokens
     if offsets is not None:
         sequences = offsets.numel() - 1
-        _need(sequences >= 0, "offsets has sequences + 1 elements")
+        if sequences < 0:
+            raise ValueError("offsets has sequences + 1 elements")
     else:
         _need(tokens == 0 or (max_tokens and tokens % max_tokens == 0), "without offsets, max_tokens divides tokens")
         sequences = tokens // max_tokens if tokens else 0
-    rows = None
-    for s, what in ((state_in, "state_in"), (state_out, "state_out")):
-        if s is None:
-            continue
-        _need(s.dtype == torch.float32 and s.is_cuda and s.is_contiguous() and s.dim() == 4
-              and s.shape[1:] == (heads, key_dim, value_dim),
-              f"{what} is a contiguous fp32 [rows, heads, key_dim, value_dim]")
-        _need(rows is None or rows == s.shape[0], "both state pools have the same rows")
-        rows = s.shape[0]
+    before, rows = _pool(state_in, heads, key_dim, value_dim, "state_in")
+    if state_out is state_in:
+        after = before
+    else:
+        after, others = _pool(state_out, heads, key_dim, value_dim, "state_out")
+        if rows is None:
+            rows = others
+        elif others is not None and others != rows:
+            raise ValueError("both state pools have the same rows")
     if rows is None:
         rows = sequences
+    device = v.device
     if out is None:
-        out = torch.empty_like(v, memory_format=torch.contiguous_format)
-    else:
-        _need(out.shape == v.shape and out.dtype == v.dtype and out.is_cuda, "out is like v")
+        out = torch.empty(vshape, dtype=v.dtype, device=device)
+    elif out.shape != vshape or out.dtype is not v.dtype or not out.is_cuda:
+        raise ValueError("out is like v")
     qs, ks, vs, os_ = _row(q, "q"), _row(k, "k"), _row(v, "v"), _row(out, "out")
     gs, bs = _row(g, "g"), _row(beta, "beta")
     r = DeltaRequest(sequences, tokens, max_tokens, key_heads, heads, key_dim, value_dim, code,
                      DELTA_NORMALIZE if normalize else 0, rows, key_dim ** -0.5 if scale is None else scale,
                      q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(), beta.data_ptr(), out.data_ptr(),
                      qs[0], qs[1], ks[0], ks[1], vs[0], vs[1], os_[0], os_[1], gs[0], bs[0],
-                     _ints(offsets, sequences + 1, "offsets"), _ints(slots, sequences, "slots"),
-                     None if state_in is None else state_in.data_ptr(),
-                     None if state_out is None else state_out.data_ptr(), _ints(status, 1, "status"))
-    L, at = lib(), C.addressof(r)
-    n = L.fr_hip_delta_workspace(at)
-    w = _scratch(n, v.device)
-    _call(L.fr_hip_delta_rule, "fr_hip_delta_rule", v.device.index, at, w.data_ptr() if n else None, n)
+                     _ints(offsets, sequences + 1, "offsets"), _ints(slots, sequences, "slots"), before, after,
+                     _ints(status, 1, "status"))
+    _run("fr_hip_delta_rule", "fr_hip_delta_workspace", r, device)
     return out
 
 
@@ -186,28 +211,31 @@ def q4_product(x, codes, scales, zeros=None, *, out=None):
     and 2j+1 high; scales fp16 or bf16 [rows, cols / group], zeros uint8 of the
     same shape or None (8). group is cols / scales' columns: 32, 64 or 128."""
     code = _type(x, "x")
-    _need(x.dim() == 2 and codes.dim() == 2 and scales.dim() == 2, "x, codes and scales are matrices")
-    tokens, cols = x.shape
-    rows, groups = scales.shape
-    _need(codes.dtype == torch.uint8 and codes.is_cuda and codes.is_contiguous() and codes.shape[0] == rows
-          and codes.shape[1] * 2 == cols, "codes is a contiguous uint8 [rows, cols / 2]")
-    _need(scales.dtype in (torch.float16, torch.bfloat16) and scales.is_cuda and scales.is_contiguous(),
-          "scales is a contiguous fp16 or bf16 [rows, cols / group]")
-    _need(groups > 0 and cols % groups == 0, "scales' columns divide cols")
-    if zeros is not None:
-        _need(zeros.dtype == torch.uint8 and zeros.is_cuda and zeros.is_contiguous() and zeros.shape == scales.shape,
-              "zeros is a contiguous uint8 tensor like scales")
+    xshape, wshape, sshape = x.shape, codes.shape, scales.shape
+    if len(xshape) != 2 or len(wshape) != 2 or len(sshape) != 2:
+        raise ValueError("x, codes and scales are matrices")
+    tokens, cols = xshape
+    rows, groups = sshape
+    if (wshape[0] != rows or wshape[1] * 2 != cols or codes.dtype is not torch.uint8 or not codes.is_cuda
+            or not codes.is_contiguous()):
+        raise ValueError("codes is a contiguous uint8 [rows, cols / 2]")
+    scale_type = scales.dtype
+    if scale_type not in (torch.float16, torch.bfloat16) or not scales.is_cuda or not scales.is_contiguous():
+        raise ValueError("scales is a contiguous fp16 or bf16 [rows, cols / group]")
+    if groups <= 0 or cols % groups:
+        raise ValueError("scales' columns divide cols")
+    if zeros is not None and (zeros.dtype is not torch.uint8 or zeros.shape != sshape or not zeros.is_cuda
+                              or not zeros.is_contiguous()):
+        raise ValueError("zeros is a contiguous uint8 tensor like scales")
+    device = x.device
     if out is None:
-        out = torch.empty((tokens, rows), dtype=x.dtype, device=x.device)
-    else:
-        _need(out.shape == (tokens, rows) and out.dtype == x.dtype and out.is_cuda, "out is [tokens, rows] of x's type")
-    xs, ys = _row(x, "x"), _row(out, "out")
-    r = Q4Request(tokens, rows, cols, cols // groups, code, _TYPES[scales.dtype], x.data_ptr(), codes.data_ptr(),
-                  scales.data_ptr(), None if zeros is None else zeros.data_ptr(), out.data_ptr(), xs[0], ys[0])
-    L, at = lib(), C.addressof(r)
-    n = L.fr_hip_q4_workspace(at)
-    w = _scratch(n, x.device)
-    _call(L.fr_hip_q4_product, "fr_hip_q4_product", x.device.index, at, w.data_ptr() if n else None, n)
+        out = torch.empty((tokens, rows), dtype=x.dtype, device=device)
+    elif out.shape != (tokens, rows) or out.dtype is not x.dtype or not out.is_cuda:
+        raise ValueError("out is [tokens, rows] of x's type")
+    r = Q4Request(tokens, rows, cols, cols // groups, code, _TYPES[scale_type], x.data_ptr(), codes.data_ptr(),
+                  scales.data_ptr(), None if zeros is None else zeros.data_ptr(), out.data_ptr(), _row(x, "x")[0],
+                  _row(out, "out")[0])
+    _run("fr_hip_q4_product", "fr_hip_q4_workspace", r, device)
     return out
 
 
@@ -229,31 +257,30 @@ class KVCache(NamedTuple):
 
 def _cache(cache):
     k, v, ke, ve = cache
-    _need(k.dim() == 4, "k_codes is [pages, heads, page, dim]")
-    pages, heads, page, dim = k.shape
-    _need(v.shape == (pages, heads, page // 16, dim, 16) and page % 16 == 0,
-          "v_codes is [pages, heads, page / 16, dim, 16]")
-    _need(ke.shape == (pages, heads, page) and ve.shape == ke.shape, "k_exp and v_exp are [pages, heads, page]")
-    for t in cache:
-        _need(t.dtype == torch.uint8 and t.is_cuda and t.is_contiguous(), "the cache is of contiguous uint8 tensors")
+    shape = k.shape
+    if len(shape) != 4:
+        raise ValueError("k_codes is [pages, heads, page, dim]")
+    pages, heads, page, dim = shape
+    if page % 16 or v.shape != (pages, heads, page // 16, dim, 16):
+        raise ValueError("v_codes is [pages, heads, page / 16, dim, 16]")
+    if ke.shape != shape[:3] or ve.shape != shape[:3]:
+        raise ValueError("k_exp and v_exp are [pages, heads, page]")
+    for t in (k, v, ke, ve):
+        if t.dtype is not torch.uint8 or not t.is_cuda or not t.is_contiguous():
+            raise ValueError("the cache is of contiguous uint8 tensors")
     return CacheRequest(pages, heads, page, dim, k.data_ptr(), v.data_ptr(), ke.data_ptr(), ve.data_ptr())
 
 
 def _tokens(c, k, v, slots, status):
-    t = v if k is None else k
-    code = _type(t, "k and v")
-    tokens = t.shape[0]
-    at = []
-    for x in (k, v):
-        if x is None:
-            at.append((None, (0, 0)))
-            continue
-        _need(x.dim() == 3 and x.shape == (tokens, c.heads, c.dim) and x.dtype == t.dtype and x.is_cuda,
-              "k and v are [tokens, heads, dim] of one type")
-        at.append((x.data_ptr(), _row(x, "k and v")))
-    (kp, ks), (vp, vs) = at
-    return TokensRequest(c, tokens, code, kp, vp, ks[0], ks[1], vs[0], vs[1], _ints(slots, tokens, "slots"),
-                         _ints(status, 1, "status"))
+    """The request for k and v, two tensors [tokens, heads, dim] alike."""
+    code = _type(k, "k and v")
+    shape = k.shape
+    if (len(shape) != 3 or shape[1] != c.heads or shape[2] != c.dim or v.shape != shape or v.dtype is not k.dtype
+            or not v.is_cuda):
+        raise ValueError("k and v are [tokens, heads, dim] of one type")
+    ks, vs = _row(k, "k and v"), _row(v, "k and v")
+    return TokensRequest(c, shape[0], code, k.data_ptr(), v.data_ptr(), ks[0], ks[1], vs[0], vs[1],
+                         _ints(slots, shape[0], "slots"), _ints(status, 1, "status"))
 
 
 def kv_append(cache, k, v, slots, *, status=None):
@@ -266,9 +293,7 @@ def kv_append(cache, k, v, slots, *, status=None):
 def kv_read(cache, slots, dtype=torch.bfloat16, *, status=None):
     """The values held at slots as (k, v) [tokens, heads, dim]; zeros for -1."""
     c = _cache(cache)
-    shape = (slots.numel(), c.heads, c.dim)
-    k = torch.empty(shape, dtype=dtype, device=slots.device)
-    v = torch.empty(shape, dtype=dtype, device=slots.device)
+    k, v = torch.empty((2, slots.numel(), c.heads, c.dim), dtype=dtype, device=slots.device)
     r = _tokens(c, k, v, slots, status)
     _call(lib().fr_hip_kv_read, "fr_hip_kv_read", k.device.index, C.addressof(r))
     return k, v
@@ -283,9 +308,11 @@ def kv_attend(cache, q, table, lengths, *, scale=None, max_context=None, out=Non
     unless given."""
     code = _type(q, "q")
     c = _cache(cache)
-    _need(q.dim() == 3 and q.shape[2] == c.dim, "q is [sequences * burst, heads, dim]")
-    _need(table.dim() == 2 and table.dtype == torch.int32 and table.is_cuda and (table.stride(1) == 1 or
-          table.shape[1] <= 1), "table is an int32 matrix")
+    if q.dim() != 3 or q.shape[2] != c.dim:
+        raise ValueError("q is [sequences * burst, heads, dim]")
+    if (table.dim() != 2 or table.dtype is not torch.int32 or not table.is_cuda
+            or (table.stride(1) != 1 and table.shape[1] > 1)):
+        raise ValueError("table is an int32 matrix")
     sequences = table.shape[0]
     _need(q.shape[0] % sequences == 0 if sequences else q.shape[0] == 0, "q has the same burst of every sequence")
     most = table.shape[1] * c.page
@@ -293,9 +320,9 @@ def kv_attend(cache, q, table, lengths, *, scale=None, max_context=None, out=Non
         max_context = most
     _need(0 <= max_context <= most, "max_context is within a table row's pages")
     if out is None:
-        out = torch.empty_like(q, memory_format=torch.contiguous_format)
-    else:
-        _need(out.shape == q.shape and out.dtype == q.dtype and out.is_cuda, "out is like q")
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    elif out.shape != q.shape or out.dtype is not q.dtype or not out.is_cuda:
+        raise ValueError("out is like q")
     if not sequences or not q.shape[0]:
         return out
     qs, os_ = _row(q, "q"), _row(out, "out")
@@ -303,9 +330,5 @@ def kv_attend(cache, q, table, lengths, *, scale=None, max_context=None, out=Non
                      max(table.stride(0), table.shape[1]) if sequences == 1 else table.stride(0),
                      c.dim ** -0.5 if scale is None else scale, q.data_ptr(), out.data_ptr(), qs[0], qs[1], os_[0],
                      os_[1], table.data_ptr(), _ints(lengths, sequences, "lengths"), _ints(status, 1, "status"))
-    L, at = lib(), C.addressof(r)
-    n = L.fr_hip_kv_workspace(at)
-    w = _scratch(n, q.device)
-    _call(L.fr_hip_kv_attend, "fr_hip_kv_attend", q.device.index, at, w.data_ptr() if n else None, n)
+    _run("fr_hip_kv_attend", "fr_hip_kv_workspace", r, q.device)
     return out
-
