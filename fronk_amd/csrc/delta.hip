@@ -182,6 +182,8 @@ template <typename T, int DK> struct Room {
   static constexpr int kN = Parts<T>::kIn, kSteps = DK / 32;
   static constexpr size_t kRows = (size_t)4 * kSteps * kN;     // K (and Q) with tokens as rows
   static constexpr size_t kKey = 3 * kRows;                    // ... K, Q, and K with dims as rows
+  static constexpr size_t kMatrix = (size_t)kChunk * (kChunk + 4) * sizeof(float);   // in LDS
+  static constexpr size_t kShared = kRows * 1024 > kMatrix ? kRows * 1024 : kMatrix;
   static constexpr size_t kT = 6 * 3, kP = 6 * Parts<T>::kOut; // lower triangles: 1, 1, 2, 2 steps
   static constexpr size_t kHead = kT + kP + 1;                 // ... and 256 floats
   static size_t bytes(const fr_hip_delta* r) {
@@ -195,6 +197,7 @@ __device__ __forceinline__ int triangle(int w) { return w < 2 ? w : 2 * w - 2; }
 struct ChunkArgs {
   DeltaArgs d;
   uint4v *key, *head;   // [slot][key head][Room::kKey][64], [slot][head][Room::kHead][64]
+  uint32_t each;        // value heads of a workgroup of delta_prepare
 };
 // Floats of a head's last kilobyte.
 enum { kRowK = 0, kRowQ = 64, kColU = 128, kLast = 192 };
@@ -228,8 +231,8 @@ __device__ __forceinline__ void lds_barrier() {
 }
 __device__ __forceinline__ bf16x8 frag(uint4v x) { return __builtin_bit_cast(bf16x8, x); }
 
-// One workgroup: one chunk and key head, and the value heads that share it;
-// wavefront w holds tokens 16 w .. 16 w + 15 as rows.
+// One workgroup: one chunk and key head, and `each` of the value heads that share
+// it; wavefront w holds tokens 16 w .. 16 w + 15 as rows.
 template <typename T, int DK>
 __global__ __launch_bounds__(256) void delta_prepare(ChunkArgs C) {
   typedef Room<T, DK> W;
@@ -237,12 +240,13 @@ __global__ __launch_bounds__(256) void delta_prepare(ChunkArgs C) {
   const DeltaArgs& A = C.d;
   extern __shared__ uint4v lds[];
   uint4v* kf = lds;                                            // [4][KS][N][64]
-  float(*m1)[kPitch] = reinterpret_cast<float(*)[kPitch]>(lds + W::kRows * 64);
-  float(*m2)[kPitch] = m1 + kChunk;
+  float(*m1)[kPitch] = reinterpret_cast<float(*)[kPitch]>(lds);   // in kf's place, once that is read
+  float(*m2)[kPitch] = reinterpret_cast<float(*)[kPitch]>(lds + W::kShared / 16);
   __shared__ double total[kChunk];
   __shared__ __attribute__((aligned(16))) float kn[kChunk], qn[kChunk], bt[kChunk];
 
   const uint32_t chunks = (A.max_tokens + kChunk - 1) / kChunk;
+  const uint32_t group = A.heads / A.key_heads, first_head = blockIdx.y * C.each;
   const uint32_t kh = blockIdx.x % A.key_heads, chunk = blockIdx.x / A.key_heads % chunks;
   const uint32_t seq = blockIdx.x / A.key_heads / chunks;
   uint32_t first, count;
@@ -279,14 +283,16 @@ __global__ __launch_bounds__(256) void delta_prepare(ChunkArgs C) {
 #pragma unroll
     for (int p = 0; p < N; ++p) {
       const int at = ((w * KS + s) * N + p) * 64 + lane;
-      kf[at] = key[at] = __builtin_bit_cast(uint4v, ka[s][p]);
+      kf[at] = __builtin_bit_cast(uint4v, ka[s][p]);
+      if (first_head) continue;   // the first heads' workgroup writes for all
+      key[at] = kf[at];
       key[W::kRows * 64 + at] = __builtin_bit_cast(uint4v, qa[s][p]);
     }
-  __syncthreads();
+  lds_barrier();
 
   // K with dims as rows: dim 16 t + i, tokens 32 s + 16 (e / 4) + 4 j + e % 4.
   const __bf16* k16 = reinterpret_cast<const __bf16*>(kf);
-  for (int f = w; f < DK / 16 * 2 * N; f += 4) {
+  for (int f = w; f < DK / 16 * 2 * N && !first_head; f += 4) {
     const int p = f % N, s = f / N % 2, t = f / N / 2;
     bf16x8 x;
 #pragma unroll
@@ -315,16 +321,16 @@ __global__ __launch_bounds__(256) void delta_prepare(ChunkArgs C) {
       }
   }
 
-  const int group = (int)(A.heads / A.key_heads);
-  for (int r = 0; r < group; ++r) {
+  for (uint32_t r = first_head; r < first_head + C.each && r < group; ++r) {
     const uint32_t head = kh * group + r;
     uint4v* out = C.head + ((size_t)slot * A.heads + head) * W::kHead * 64;
     float* scalars = reinterpret_cast<float*>(out + (W::kT + W::kP) * 64);
     if (w == 0) {
       // In 64 bits: a sum of far decays would take the near ones' differences
-      // with it. One of -1e5 empties the state as -infinity does.
+      // with it. One of -1e5 empties the state as -infinity does. In powers of
+      // two: exp2 of a difference d is off by |d| 2^-24 of itself, at most 2^-24.
       double x = lane < n ? (double)A.g[(int64_t)(first + lane) * A.g_token + head] : 0.0;
-      if (x < -1e5) x = -1e5;
+      x = (x < -1e5 ? -1e5 : x) * 1.4426950408889634;
       for (int d = 1; d < 64; d *= 2) {
         const double y = __shfl_up(x, d);
         if (lane >= d) x += y;
@@ -332,13 +338,13 @@ __global__ __launch_bounds__(256) void delta_prepare(ChunkArgs C) {
       total[lane] = x;
       bt[lane] = lane < n ? A.beta[(int64_t)(first + lane) * A.beta_token + head] : 0.f;
       const double last = __shfl(x, 63);
-      const float gamma = expf((float)x);
+      const float gamma = __builtin_amdgcn_exp2f((float)x);
       scalars[kRowK + lane] = gamma * kn[lane];
       scalars[kRowQ + lane] = gamma * qn[lane] * A.scale;
-      scalars[kColU + lane] = expf((float)(last - x)) * kn[lane];
-      if (lane == 0) scalars[kLast] = expf((float)last);
+      scalars[kColU + lane] = __builtin_amdgcn_exp2f((float)(last - x)) * kn[lane];
+      if (lane == 0) scalars[kLast] = __builtin_amdgcn_exp2f((float)last);
     }
-    __syncthreads();
+    lds_barrier();
     // P row by row, then A, through m1.
     float decay[4][4];
 #pragma unroll
@@ -346,10 +352,11 @@ __global__ __launch_bounds__(256) void delta_prepare(ChunkArgs C) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int a = 16 * w + 4 * j + e, b = 16 * u + i;
-        decay[u][e] = a >= b ? expf((float)(total[a] - total[b])) * kn[b] : 0.f;
+        const float d = __builtin_amdgcn_exp2f((float)(total[a] - total[b])) * kn[b];
+        decay[u][e] = a >= b ? d : 0.f;
         m1[a][b] = a >= b ? qk[u][e] * decay[u][e] * (qn[a] * A.scale) : 0.f;
       }
-    __syncthreads();
+    lds_barrier();
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
       if (s > w / 2) continue;
@@ -360,7 +367,7 @@ __global__ __launch_bounds__(256) void delta_prepare(ChunkArgs C) {
       for (int p = 0; p < PO; ++p)
         out[(W::kT + (triangle(w) + s) * PO + p) * 64 + lane] = __builtin_bit_cast(uint4v, x[p]);
     }
-    __syncthreads();
+    lds_barrier();
 #pragma unroll
     for (int u = 0; u < 4; ++u)
 #pragma unroll
@@ -369,7 +376,7 @@ __global__ __launch_bounds__(256) void delta_prepare(ChunkArgs C) {
         m1[a][b] = a > b ? kk[u][e] * decay[u][e] * (bt[a] * kn[a]) : 0.f;
         m2[a][b] = 0.f;
       }
-    __syncthreads();
+    lds_barrier();
     // (I + A)^-1 in m2 by blocks of 16: the diagonal ones by substitution
     // (lane i column i; products of powers of A would lose digits where keys
     // are alike), then those below by the distance from it, each from blocks
@@ -389,7 +396,7 @@ __global__ __launch_bounds__(256) void delta_prepare(ChunkArgs C) {
       }
     }
     for (int dist = 1; dist < 4; ++dist) {
-      __syncthreads();
+      lds_barrier();
       if (w >= dist) {
         const int u = w - dist;
         float4v c = {0, 0, 0, 0};
@@ -410,7 +417,7 @@ __global__ __launch_bounds__(256) void delta_prepare(ChunkArgs C) {
         for (int e = 0; e < 4; ++e) m2[16 * w + 4 * j + e][16 * u + i] = -y[e];
       }
     }
-    __syncthreads();
+    lds_barrier();
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
       if (s > w / 2) continue;
@@ -421,7 +428,7 @@ __global__ __launch_bounds__(256) void delta_prepare(ChunkArgs C) {
 #pragma unroll
       for (int p = 0; p < 3; ++p) out[((triangle(w) + s) * 3 + p) * 64 + lane] = __builtin_bit_cast(uint4v, x[p]);
     }
-    __syncthreads();
+    lds_barrier();
   }
 }
 
@@ -733,14 +740,18 @@ bool in_chunks(const fr_hip_delta* r) { return r->max_tokens >= kChunkFrom; }
 template <typename T, int DK>
 int launch_chunks(const fr_hip_delta* r, const DeltaArgs& A, void* workspace, hipStream_t s) {
   typedef Room<T, DK> W;
-  constexpr size_t kLds = W::kRows * 1024 + 2 * kChunk * (kChunk + 4) * sizeof(float);
+  constexpr size_t kLds = W::kShared + W::kMatrix;
   const size_t slots = (size_t)r->tokens / kChunk + r->sequences;
-  const ChunkArgs C = {A, static_cast<uint4v*>(workspace), static_cast<uint4v*>(workspace) + slots * W::kKey * r->key_heads * 64};
+  ChunkArgs C = {A, static_cast<uint4v*>(workspace), static_cast<uint4v*>(workspace) + slots * W::kKey * r->key_heads * 64, 1};
   static const hipError_t wide = hipFuncSetAttribute(reinterpret_cast<const void*>(&delta_prepare<T, DK>),
                                                      hipFuncAttributeMaxDynamicSharedMemorySize, (int)kLds);
   FRONK_CK(wide);
   const uint32_t chunks = (A.max_tokens + kChunk - 1) / kChunk;
-  hipLaunchKernelGGL((delta_prepare<T, DK>), dim3(r->sequences * chunks * r->key_heads), dim3(256), kLds, s, C);
+  // The heads of a key head share its products where there are enough chunks to
+  // fill the card without.
+  const uint32_t prepares = r->sequences * chunks * r->key_heads, group = r->heads / r->key_heads;
+  if (prepares >= 3 * 256) C.each = group;
+  hipLaunchKernelGGL((delta_prepare<T, DK>), dim3(prepares, (group + C.each - 1) / C.each), dim3(256), kLds, s, C);
   hipLaunchKernelGGL((delta_scan<T, DK>), dim3(r->sequences * r->heads * (r->value_dim / 16)), dim3(512), 0, s, C);
   return FR_HIP_OK;
 }
