@@ -1,6 +1,8 @@
 """Build the MI355X libraries in-tree (no JIT cache, no site-packages).
 
 libfronk_hip.so      HIP kernels + C ABI (include/fronk_hip.h), gfx950 only.
+_dense.so            fronk_amd.dense's side of it over torch tensors
+                     (host/dense_module.cpp).
 libfr_hip.so         the "hip" fr_backend vtable (host/hip.c, plain C11),
                      compiled against the reference's own src/ headers where
                      they lie (hidden size fixed there at 2560) and linked
@@ -10,6 +12,7 @@ libfr_hip.so         the "hip" fr_backend vtable (host/hip.c, plain C11),
 """
 import os
 import subprocess
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
@@ -19,6 +22,8 @@ HIP_SRCS = [os.path.join(HERE, "csrc", n) for n in ("fronk_hip.hip", "delta.hip"
 HIP_LIB = os.path.join(HERE, "libfronk_hip.so")
 VTABLE_SRC = os.path.join(HERE, "host", "hip.c")
 VTABLE_LIB = os.path.join(HERE, "libfr_hip.so")
+DENSE_SRC = os.path.join(HERE, "host", "dense_module.cpp")
+DENSE_LIB = os.path.join(HERE, "_dense.so")
 REFERENCE_SRC = os.path.join(os.environ.get("FRONK_REFERENCE", "/root/reference"), "src")
 
 # Packed-FP32 instructions are disabled for every HIP translation unit.
@@ -52,8 +57,24 @@ def build_vtable(verbose=False):
     return VTABLE_LIB
 
 
+def build_dense(verbose=False):
+    """The torch side of the dense operators, linked to libfronk_hip.so."""
+    import torch
+    at = os.path.dirname(torch.__file__)
+    include = [os.path.join(ROOT, "include"), os.path.join(at, "include"),
+               os.path.join(at, "include", "torch", "csrc", "api", "include"), sysconfig.get_paths()["include"]]
+    cmd = ["g++", "-std=c++17", "-O2", "-fPIC", "-shared", *("-I" + i for i in include),
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", DENSE_SRC, "-o", DENSE_LIB + ".tmp",
+           "-L" + HERE, "-lfronk_hip", "-Wl,-rpath,$ORIGIN", "-L" + os.path.join(at, "lib"), "-ltorch_python",
+           "-ltorch_cpu", "-lc10"]
+    subprocess.run(cmd, check=True, capture_output=not verbose)
+    os.replace(DENSE_LIB + ".tmp", DENSE_LIB)
+    return DENSE_LIB
+
+
 def build_all(verbose=False):
     build_hip(verbose)
+    build_dense(verbose)
     if os.path.isdir(REFERENCE_SRC):
         build_vtable(verbose)
 
