@@ -33,7 +33,12 @@ __device__ __forceinline__ bool sequence(const DeltaArgs& A, uint32_t i, uint32_
   const int32_t s = A.slot ? A.slot[i] : (int32_t)i;
   const int32_t a = A.offsets ? A.offsets[i] : (int32_t)(i * A.max_tokens);
   const int32_t b = A.offsets ? A.offsets[i + 1] : (int32_t)((i + 1) * A.max_tokens);
-  const uint32_t bad = fronk::bad_sequence(s, A.slots, a, b, A.tokens, A.max_tokens);
+  uint32_t bad = fronk::bad_sequence(s, A.slots, a, b, A.tokens, A.max_tokens);
+  // Behind offsets that go down, a sequence could share tokens with one before.
+  bool below = false;
+  if (A.offsets)
+    for (uint32_t e = threadIdx.x & 63; e < i; e += 64) below |= A.offsets[e] > a;
+  if (__any(below)) bad |= FR_HIP_BAD_OFFSET;
   *first = (uint32_t)a;
   *count = (uint32_t)(b - a);
   *row = (size_t)(s < 0 ? 0 : s);
@@ -48,7 +53,9 @@ __device__ __forceinline__ bool sequence(const DeltaArgs& A, uint32_t i, uint32_
 // products over dk are taken of the state before the token,
 //     p = S^T k,  w = S^T q,  o = scale (a w + (q . k) u),
 // so that a token needs one reduction over the 16 row lanes: two row rotations
-// and the two row swaps, no LDS and no barrier.
+// and the two row swaps, no LDS and no barrier. Bound by reading and writing the
+// states: 64 streams of 32 heads of 128 x 128 (268 MB) in 58.8 us, 4.6 TB/s; one
+// stream's in 4.5 us, a launch and a memory latency.
 template <typename T, int DK>
 __global__ __launch_bounds__(256) void delta_step(DeltaArgs A) {
   constexpr int R = DK / 16;
@@ -232,7 +239,9 @@ __device__ __forceinline__ void lds_barrier() {
 __device__ __forceinline__ bf16x8 frag(uint4v x) { return __builtin_bit_cast(bf16x8, x); }
 
 // One workgroup: one chunk and key head, and `each` of the value heads that share
-// it; wavefront w holds tokens 16 w .. 16 w + 15 as rows.
+// it; wavefront w holds tokens 16 w .. 16 w + 15 as rows. A head takes about 6 us:
+// decays and P 2.5, the inverse 2, the barriers between them the rest. 4096 tokens
+// of 32 heads: 41 us, 113 MB written; 5 sequences with 33 chunks of 9 heads: 16 us.
 template <typename T, int DK>
 __global__ __launch_bounds__(256) void delta_prepare(ChunkArgs C) {
   typedef Room<T, DK> W;
@@ -436,7 +445,9 @@ __global__ __launch_bounds__(256) void delta_prepare(ChunkArgs C) {
 // Wavefronts 0..3 carry the state: wavefront w has tokens 16 w .. of the chunk
 // and dims w * dk / 4 .. of S (in registers, fp32), and three times a chunk they
 // exchange operands through LDS: S, then V - e^G K S, then U. Wavefronts 4..7
-// form the outputs of the same tokens beside them.
+// form the outputs of the same tokens beside them. 64 chunks of 32 heads of 128 x
+// 128 in 98 us, 1.5 us a chunk, of which the chain's products, splits and LDS
+// exchanges by themselves are 1.3 and memory hardly any.
 //
 // A chunk costs three barriers and the products between them, so nothing may
 // wait for memory there: each operand's registers are filled for the next chunk

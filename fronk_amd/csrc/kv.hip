@@ -128,7 +128,8 @@ __global__ __launch_bounds__(256) void kv_single(KvArgs A) {
 // they go through LDS: where the 16 slots are one block of the cache, a lane
 // writes a dim's 16 bytes at once; where they are not, four bytes where four
 // slots follow each other from a multiple of four, and single bytes otherwise.
-// (Reads share their lines in the caches and gain nothing from it.)
+// (Reads share their lines in the caches and gain nothing from it.) 4096 tokens of
+// 2 heads of 256: 8.5 us in a row of writes, 16.4 by single vectors.
 constexpr int kWindow = 16;
 
 struct Window {
@@ -237,6 +238,10 @@ __global__ __launch_bounds__(256) void kv_append(KvArgs A) {
 // Codes times one are exact in bf16 and fp16. Q is an exact operand too (fp32:
 // three bf16 parts); P 2^e is fp32 in two bf16 parts (error 2^-17 of it, below
 // a 16-bit output's own rounding), three for fp32 outputs.
+//
+// 131072 tokens of 2 heads of 256 (134 MB): 26 us, 5.1 TB/s, and 5 to join 128
+// stretches. 32 streams of 4 to 8192 tokens, 32 rows of dim 128: 26 us, bound by the
+// vector work on the scores.
 struct AttendArgs {
   Cache cache;
   const void* q;

@@ -270,7 +270,8 @@ enum { FR_HIP_BAD_OFFSET = 1, FR_HIP_BAD_SLOT = 2, FR_HIP_BAD_PAGE = 4, FR_HIP_B
  * pools (slot NULL: row i); slot -1: the sequence is skipped, nothing of it is
  * read or written. Slots are distinct. state_in NULL: states begin as zeros;
  * state_out NULL: final states are dropped; both may be one pool. A sequence
- * of no tokens passes its state on.
+ * of no tokens passes its state on. Offsets do not go down: a sequence that
+ * begins below an offset before it is bad, as is one that ends below its start.
  * key_dim 64, 128 or 256; value_dim a multiple of 16 up to 1024; key_heads
  * divides heads. State rows are [heads][key_dim][value_dim], 16-byte aligned. */
 enum { FR_HIP_DELTA_NORMALIZE = 1 };
@@ -300,7 +301,8 @@ int fr_hip_delta_rule(const fr_hip_delta *req, void *workspace, size_t bytes, vo
  * one; 16-byte aligned, rows cols / 2 bytes apart. scales fp16 or bf16, zeros
  * uint8 or NULL (8), both [rows][cols / group] dense. group 32, 64 or 128;
  * cols a multiple of group, up to 65536. A token with a non-finite x gets
- * non-finite outputs (inf or NaN). */
+ * non-finite outputs (inf or NaN); fp32 values above bf16's largest (3.39e38)
+ * may count as infinite. */
 typedef struct {
     unsigned tokens, rows, cols, group;
     unsigned type, scale_type;        /* scale_type FR_HIP_F16 or FR_HIP_BF16 */

@@ -212,6 +212,26 @@ def test_bad_entries_touch_nothing(n):
     assert torch.equal(p[0], good[0]) and torch.equal(p[1], pool[1])
 
 
+@pytest.mark.parametrize("n", [3, 100])
+def test_offsets_that_go_down(n):
+    """Sequences behind an offset that goes down may not share tokens with one
+    before: they are left out, each time alike."""
+    q, k, v, g, beta = (x.cuda() for x in delta_inputs(97, [2 * n], 1, 2, 64, 32, BF16))
+    pool = torch.randn(70, 2, 64, 32, generator=gen(98)).cuda()
+    good = pool[:1].clone()
+    o = dense.delta_rule(q, k, v, g, beta, good, good, normalize=True)
+    # The second sequence ends below its start; the later ones begin below 2 n, the
+    # last of them only after 64 others of no tokens.
+    offsets = torch.tensor([0, 2 * n, 1] + [2] * 67 + [2 * n], dtype=torch.int32).cuda()
+    for _ in range(3):
+        p, out = pool.clone(), torch.full_like(v, 3.0)
+        status = torch.zeros(1, dtype=torch.int32, device="cuda")
+        dense.delta_rule(q, k, v, g, beta, p, p, normalize=True, max_tokens=2 * n, out=out, status=status,
+                         offsets=offsets)
+        assert status.item() == dense.BAD_OFFSET
+        assert torch.equal(out, o) and torch.equal(p[0], good[0]) and torch.equal(p[1:], pool[1:])
+
+
 @pytest.mark.parametrize("n", [4, 200])
 def test_stream_and_graph(n):
     """On a stream of its own, and replayed from a graph with eager work in
