@@ -450,10 +450,9 @@ __global__ __launch_bounds__(256) void delta_prepare(ChunkArgs C) {
 // exchanges by themselves are 1.3 and memory hardly any.
 //
 // A chunk costs three barriers and the products between them, so nothing may
-// wait for memory there: each operand's registers are filled for the next chunk
-// in the phase after the product that read them, behind that phase's LDS reads
-// (kAhead; with fp32's 54 operands at dk 256, which do not fit, K's rows and
-// dims take turns). The two kinds of wavefronts have loops of their own, so that
+// wait for memory there: each operand's registers are filled anew in the phase
+// after the product that read them, two phases before the next (kAhead; with
+// fp32's 54 operands at dk 256, which do not fit, K's rows and dims take turns). The two kinds of wavefronts have loops of their own, so that
 // neither's loads are waited for on account of the other's.
 template <typename T, int DK>
 __global__ __launch_bounds__(512) void delta_scan(ChunkArgs C) {
@@ -552,7 +551,6 @@ __global__ __launch_bounds__(512) void delta_scan(ChunkArgs C) {
     if (chunks) {
       load1(0), load_v(0), load2(0, three);
       col_scale = scalars(0, kColU);
-      if constexpr (kAhead) load3(0);
     }
     float4v state[TPW];
     const size_t at = ((row * A.heads + head) * DK + 16 * w * TPW + 4 * j) * A.dv + col;
@@ -569,6 +567,7 @@ __global__ __launch_bounds__(512) void delta_scan(ChunkArgs C) {
       lds_barrier();   // S is there
       float4v x[3] = {};
       bf16x8 y[3][2];
+      if constexpr (kAhead) load3(c);
 #pragma unroll
       for (int s = 0; s < KS; ++s)
 #pragma unroll
@@ -583,7 +582,7 @@ __global__ __launch_bounds__(512) void delta_scan(ChunkArgs C) {
       for (int e = 0; e < 4; ++e) r[e] = token + e < count ? (float)v[e] : 0.f;
       r -= row_scale * (x[0] + (x[1] + x[2]));
       put(&rf[0][w / 2][0], 2 * 64, j, w % 2, r, three);
-      lds_barrier();   // V - e^G K S is there, and S is read
+      lds_barrier();   // V - e^G K S is there
 #pragma unroll
       for (int b = 2; b >= 0; --b)
 #pragma unroll
@@ -626,8 +625,7 @@ __global__ __launch_bounds__(512) void delta_scan(ChunkArgs C) {
         state[t] = last * state[t] + (z[0] + (z[1] + z[2]));
         put_state(t, state[t]);
       }
-      if constexpr (kAhead) load3(next);
-      else load1(next);
+      if constexpr (!kAhead) load1(next);
     }
     __builtin_amdgcn_s_setprio(0);
     if (A.state_out) {
@@ -648,6 +646,7 @@ __global__ __launch_bounds__(512) void delta_scan(ChunkArgs C) {
     for (uint32_t c = 0; c < chunks; ++c) {
       const uint32_t next = c + 1 < chunks ? c + 1 : c;
       lds_barrier();   // S is there
+      lds_barrier();   // ... and read by the chain, which now leaves LDS to these
       float4v acc[3] = {};
 #pragma unroll
       for (int s = 0; s < KS; ++s)
@@ -660,8 +659,7 @@ __global__ __launch_bounds__(512) void delta_scan(ChunkArgs C) {
       acc[0] = row_scale * (acc[0] + (acc[1] + acc[2]));
       acc[1] = acc[2] = float4v{0, 0, 0, 0};
       rows_of(next);
-      lds_barrier();   // S is read
-      lds_barrier();   // U is there
+      lds_barrier();   // U is there, and S is read
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
         if (s >= steps) continue;
