@@ -313,7 +313,7 @@ typedef struct {
     void *y;                          /* [tokens][rows] */
     int64_t x_token, y_token;
 } fr_hip_q4;
-size_t fr_hip_q4_workspace(const fr_hip_q4 *req);
+size_t fr_hip_q4_workspace(const fr_hip_q4 *req);   /* as fr_hip_delta_workspace */
 int fr_hip_q4_product(const fr_hip_q4 *req, void *workspace, size_t bytes, void *stream);
 
 /* A key/value cache in 8 bits, in pages of `page` tokens. A token's vector of
@@ -371,7 +371,7 @@ typedef struct {
     const int32_t *table, *length;
     uint32_t *status;
 } fr_hip_kv_query;
-size_t fr_hip_kv_workspace(const fr_hip_kv_query *req);
+size_t fr_hip_kv_workspace(const fr_hip_kv_query *req);   /* as fr_hip_delta_workspace */
 int fr_hip_kv_attend(const fr_hip_kv_query *req, void *workspace, size_t bytes, void *stream);
 
 /* Launch timing for measurement (no reference counterpart): after
