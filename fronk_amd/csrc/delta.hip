@@ -683,6 +683,10 @@ __global__ __launch_bounds__(512) void delta_scan(ChunkArgs C) {
 
 // ---------------------------------------------------------------------- host
 
+// Bursts go token by token; from this many tokens on, chunks.
+constexpr unsigned kChunkFrom = 33;
+bool in_chunks(const fr_hip_delta* r) { return r->max_tokens >= kChunkFrom; }
+
 int check(const fr_hip_delta* r) {
   if (!r || r->type > FR_HIP_BF16 || (r->flags & ~(unsigned)FR_HIP_DELTA_NORMALIZE)) return FR_HIP_INVALID;
   if (!r->key_heads || !r->heads || r->heads % r->key_heads || !r->key_dim || !r->value_dim) return FR_HIP_INVALID;
@@ -695,9 +699,11 @@ int check(const fr_hip_delta* r) {
   if (((uintptr_t)r->q | (uintptr_t)r->k | (uintptr_t)r->v | (uintptr_t)r->o) % elem_size(r->type)) return FR_HIP_INVALID;
   if (r->key_dim != 64 && r->key_dim != 128 && r->key_dim != 256) return FR_HIP_UNSUPPORTED;
   if (r->value_dim % 16 || r->value_dim > 1024 || r->heads > 65535) return FR_HIP_UNSUPPORTED;
-  // One-dimensional grids of (sequence, head, 16 columns) and (sequence, chunk, key head).
-  if ((uint64_t)r->sequences * r->heads * (r->value_dim / 16) > INT_MAX) return FR_HIP_UNSUPPORTED;
-  if ((uint64_t)r->sequences * ((uint64_t)r->max_tokens / kChunk + 1) * r->key_heads > INT_MAX) return FR_HIP_UNSUPPORTED;
+  // One-dimensional grids of (sequence, head, 16 columns) and (sequence, chunk, key
+  // head), of less than 2^32 threads.
+  const uint64_t columns = (uint64_t)r->sequences * r->heads * (r->value_dim / 16), longest = r->max_tokens < r->tokens ? r->max_tokens : r->tokens;
+  if (columns > UINT32_MAX / (in_chunks(r) ? 512 : 128)) return FR_HIP_UNSUPPORTED;
+  if (r->sequences * (longest / kChunk + 1) > UINT32_MAX / 256 / r->key_heads) return FR_HIP_UNSUPPORTED;
   return FR_HIP_OK;
 }
 
@@ -741,10 +747,6 @@ void launch_step(const fr_hip_delta* r, const DeltaArgs& A, hipStream_t s) {
     default: hipLaunchKernelGGL((delta_step<T, 256>), grid, block, 0, s, A); break;
   }
 }
-
-// Bursts go token by token; from this many tokens on, chunks.
-constexpr unsigned kChunkFrom = 33;
-bool in_chunks(const fr_hip_delta* r) { return r->max_tokens >= kChunkFrom; }
 
 template <typename T, int DK>
 int launch_chunks(const fr_hip_delta* r, const DeltaArgs& A, void* workspace, hipStream_t s) {

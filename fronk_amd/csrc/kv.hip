@@ -693,8 +693,8 @@ int check_tokens(const fr_hip_kv_cache* c, unsigned tokens, unsigned type, const
   if (tokens > INT_MAX || (tokens && (!slot || (both ? !k || !v : !k && !v)))) return FR_HIP_INVALID;
   if (((uintptr_t)k | (uintptr_t)v) % elem_size(type)) return FR_HIP_INVALID;
   if (rc) return rc;
-  // (heads, tokens and dims of a call in one-dimensional grids, with room to spare)
-  return (uint64_t)tokens * c->heads * 2 * (c->dim / 4) / 256 >= INT_MAX ? FR_HIP_UNSUPPORTED : FR_HIP_OK;
+  // Grids of less than 2^32 threads.
+  return (uint64_t)tokens * c->heads * 2 * (c->dim / 4) > UINT32_MAX - 256 ? FR_HIP_UNSUPPORTED : FR_HIP_OK;
 }
 
 // From this many values of K on, 16 tokens are written together. Measured, single

@@ -564,6 +564,8 @@ int check(const fr_hip_q4* r) {
   if ((uintptr_t)r->codes % 16 || (uintptr_t)r->scales % 2) return FR_HIP_INVALID;
   if (((uintptr_t)r->x | (uintptr_t)r->y) % elem_size(r->type)) return FR_HIP_INVALID;
   if (r->tokens > 4096 || r->cols > 65536 || r->rows > (1u << 28)) return FR_HIP_UNSUPPORTED;
+  // Grids of less than 2^32 threads: 512 for 64 tokens and 128 rows.
+  if ((uint64_t)(r->rows / 128 + 8) * (r->tokens / 64 + 1) > UINT32_MAX / 512) return FR_HIP_UNSUPPORTED;
   return FR_HIP_OK;
 }
 

@@ -300,7 +300,8 @@ int fr_hip_delta_rule(const fr_hip_delta *req, void *workspace, size_t bytes, vo
  * codes: byte j of row n holds code 2j in its low nibble and 2j+1 in its high
  * one; 16-byte aligned, rows cols / 2 bytes apart. scales fp16 or bf16, zeros
  * uint8 or NULL (8), both [rows][cols / group] dense. group 32, 64 or 128;
- * cols a multiple of group, up to 65536. A token with a non-finite x gets
+ * cols a multiple of group, up to 65536; rows up to 2^28, and with many tokens
+ * tokens * rows up to about 2^36. A token with a non-finite x gets
  * non-finite outputs (inf or NaN); fp32 values above bf16's largest (3.39e38)
  * may count as infinite. */
 typedef struct {

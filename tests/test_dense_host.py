@@ -232,3 +232,25 @@ def test_sequences(shim):
     for a, b in ((-1, 5), (5, 4), (10, 21), (9, 20), (-2 ** 31, 2 ** 31 - 1), (0, -1)):
         assert shim.bad(3, 4, a, b, 20, 10) == dense.BAD_OFFSET
     assert shim.bad(9, 4, 5, 4, 20, 10) == dense.BAD_SLOT | dense.BAD_OFFSET
+
+
+@pytest.mark.parametrize("change,rc", [
+    # 4 heads of 128 columns: 32 workgroups a sequence, of 512 threads in chunks.
+    (dict(sequences=1 << 18, tokens=1 << 18, slots=1 << 18, max_tokens=64), fa.UNSUPPORTED),
+    (dict(sequences=(1 << 18) - 1, tokens=1 << 18, slots=1 << 18, max_tokens=64), None),
+    (dict(sequences=1 << 20, tokens=1 << 20, slots=1 << 20, max_tokens=8), fa.UNSUPPORTED),
+    (dict(sequences=(1 << 20) - 1, tokens=1 << 20, slots=1 << 20, max_tokens=8), None)])
+def test_delta_grids_end_below_2_32_threads(change, rc):
+    """None: accepted, up to the engine that is not open."""
+    no_engine()
+    r = delta_request(**change)
+    n = fa.lib().fr_hip_delta_workspace(C.addressof(r))
+    assert fa.lib().fr_hip_delta_rule(C.addressof(r), P if n else None, n, None) == (fa.STATE if rc is None else rc)
+
+
+@pytest.mark.parametrize("tokens,rows,rc", [(4096, 1 << 24, fa.UNSUPPORTED), (4096, 1 << 23, None), (64, 1 << 28, None)])
+def test_q4_grids_end_below_2_32_threads(tokens, rows, rc):
+    no_engine()
+    r = q4_request(tokens=tokens, rows=rows)
+    n = fa.lib().fr_hip_q4_workspace(C.addressof(r))
+    assert fa.lib().fr_hip_q4_product(C.addressof(r), P if n else None, n, None) == (fa.STATE if rc is None else rc)
