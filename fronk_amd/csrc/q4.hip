@@ -6,6 +6,7 @@
 #include <type_traits>
 
 #include "dense.h"
+#include "q4_order.h"
 
 namespace {
 
@@ -367,7 +368,6 @@ __global__ __launch_bounds__(512) void q4_tiles(TileArgs C, uint32_t token_block
   constexpr int P = Packed<T>::kParts, GPB = 128 / G, SPG = G / 32;
   constexpr int kPitch = 64 * NT + 4;
   constexpr bool kAhead = P == 1 && G > 32;
-  constexpr uint32_t kLead = kAhead ? 2 : 1;   // blocks from x's load to its product
   extern __shared__ uint4v lds[];   // [half][2][P * 1024], then the sums [64][kPitch]
   const int lane = threadIdx.x & 63, i = lane & 15, j = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = wave >> 2, w = wave & 3;
@@ -463,25 +463,17 @@ __global__ __launch_bounds__(512) void q4_tiles(TileArgs C, uint32_t token_block
   };
 #pragma unroll
   for (int n = 0; n < NT; ++n) load_w(0, n);
-  load_x(0);
-  store_x(0);
-  if constexpr (kAhead) {
-    load_x(1);
-    store_x(1);
-    __syncthreads();
+  auto barrier = [] { __syncthreads(); };
+  auto read_block = [&](uint32_t k) {
 #pragma unroll
-    for (int s = 0; s < 4; ++s) read_x(0, s);
-  }
+    for (int s = 0; s < 4; ++s) read_x(k, s);
+  };
+  fronk::tiles_first<kAhead>(load_x, store_x, barrier, read_block);
   decode(0, 0);
   load_w(1, 0);
   __builtin_amdgcn_s_waitcnt(0x0f70);   // vmcnt(0): the loop's own waits are then for its own loads
   for (uint32_t k = 0; k < count; ++k) {
-    if constexpr (!kAhead) {
-      __syncthreads();   // this block's x is there, and the last one's is read
-#pragma unroll
-      for (int s = 0; s < 4; ++s) read_x(k, s);
-    }
-    load_x(k + kLead);
+    fronk::tiles_before<kAhead>(k, load_x, barrier, read_block);
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       constexpr bool kBeside = NT > 1;   // else the rows just multiplied make way first
@@ -515,8 +507,7 @@ __global__ __launch_bounds__(512) void q4_tiles(TileArgs C, uint32_t token_block
         }
       }
     }
-    store_x(k + kLead);
-    if constexpr (kAhead) __syncthreads();   // x of the block after the next is there, that of the next in registers
+    fronk::tiles_after<kAhead>(k, store_x, barrier);
   }
   add(NT - 1);
 
