@@ -17,8 +17,8 @@ from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
-# The expert engine, and the dense operators around it.
-HIP_SRCS = [os.path.join(HERE, "csrc", n) for n in ("fronk_hip.hip", "delta.hip", "q4.hip", "kv.hip")]
+# The expert engine (fronk_hip.hip within engine.hip), and the dense operators around it.
+HIP_SRCS = [os.path.join(HERE, "csrc", n) for n in ("engine.hip", "delta.hip", "q4.hip", "kv.hip")]
 HIP_LIB = os.path.join(HERE, "libfronk_hip.so")
 VTABLE_SRC = os.path.join(HERE, "host", "hip.c")
 VTABLE_LIB = os.path.join(HERE, "libfr_hip.so")

@@ -34,7 +34,6 @@
 #include <type_traits>
 #include <vector>
 
-#include "dense.h"
 #include "fronk_hip.h"
 
 namespace {
@@ -7862,15 +7861,3 @@ int fr_hip_debug_quantize_staged(const float* x, unsigned n, unsigned form, floa
 }
 
 }  // extern "C"
-
-// What the dense operators (dense.h) ask of the engine: its device made
-// current and `stream` as they take it.
-namespace fronk {
-int enter(void* stream, hipStream_t* out, unsigned* cus) {
-  if (!g_open) return FR_HIP_STATE;
-  CK(hipSetDevice(E.device));
-  *out = !stream ? E.stream : stream == FR_HIP_STREAM_DEFAULT ? hipStream_t(nullptr) : static_cast<hipStream_t>(stream);
-  *cus = E.cus;
-  return FR_HIP_OK;
-}
-}  // namespace fronk
