@@ -56,28 +56,13 @@ __device__ __forceinline__ bool sequence(const DeltaArgs& A, uint32_t i, uint32_
 // and the two row swaps, no LDS and no barrier. Bound by reading and writing the
 // states: 64 streams of 32 heads of 128 x 128 (268 MB) in 58.8 us, 4.6 TB/s; one
 // stream's in 4.5 us, a launch and a memory latency.
+
+// `count` tokens from `first` on of 16 columns (`tile`) of a head, s being its state.
 template <typename T, int DK>
-__global__ __launch_bounds__(256) void delta_step(DeltaArgs A) {
+__device__ __forceinline__ void walk(const DeltaArgs& A, uint32_t first, uint32_t count, uint32_t head, uint32_t tile,
+                                     float (&s)[DK / 16][4]) {
   constexpr int R = DK / 16;
-  const uint32_t lane = threadIdx.x & 63, waves = blockDim.x >> 6, wave = threadIdx.x >> 6;
-  const uint32_t tiles = A.dv / 16, groups = (tiles + waves - 1) / waves;
-  const uint32_t tile = blockIdx.x % groups * waves + wave;
-  const uint32_t head = blockIdx.x / groups % A.heads, seq = blockIdx.x / groups / A.heads;
-  uint32_t first, count;
-  size_t row;
-  if (!sequence(A, seq, &first, &count, &row) || tile >= tiles) return;
-  const uint32_t r = lane >> 2, col = tile * 16 + (lane & 3) * 4, kh = head / (A.heads / A.key_heads);
-
-  const size_t at = ((row * A.heads + head) * DK + r * R) * A.dv + col;
-  float s[R][4];
-#pragma unroll
-  for (int i = 0; i < R; ++i) {
-    float4v x = {0, 0, 0, 0};
-    if (A.state_in) x = *reinterpret_cast<const float4v*>(A.state_in + at + (size_t)i * A.dv);
-#pragma unroll
-    for (int c = 0; c < 4; ++c) s[i][c] = x[c];
-  }
-
+  const uint32_t lane = threadIdx.x & 63, r = lane >> 2, col = tile * 16 + (lane & 3) * 4, kh = head / (A.heads / A.key_heads);
   const T* q = static_cast<const T*>(A.q) + (int64_t)first * A.q_token + kh * A.q_head + r * R;
   const T* k = static_cast<const T*>(A.k) + (int64_t)first * A.k_token + kh * A.k_head + r * R;
   const T* v = static_cast<const T*>(A.v) + (int64_t)first * A.v_token + head * A.v_head + col;
@@ -142,6 +127,24 @@ __global__ __launch_bounds__(256) void delta_step(DeltaArgs A) {
       for (int c = 0; c < 4; ++c) o[(int64_t)t * A.o_token + c] = (T)out[c];
     }
   }
+}
+
+// All `count` tokens of a sequence, from its state to its state.
+template <typename T, int DK>
+__device__ __forceinline__ void walk_all(const DeltaArgs& A, uint32_t first, uint32_t count, size_t row, uint32_t head,
+                                         uint32_t tile) {
+  constexpr int R = DK / 16;
+  const uint32_t lane = threadIdx.x & 63, r = lane >> 2, col = tile * 16 + (lane & 3) * 4;
+  const size_t at = ((row * A.heads + head) * DK + r * R) * A.dv + col;
+  float s[R][4];
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    float4v x = {0, 0, 0, 0};
+    if (A.state_in) x = *reinterpret_cast<const float4v*>(A.state_in + at + (size_t)i * A.dv);
+#pragma unroll
+    for (int c = 0; c < 4; ++c) s[i][c] = x[c];
+  }
+  walk<T, DK>(A, first, count, head, tile, s);
   if (A.state_out) {
 #pragma unroll
     for (int i = 0; i < R; ++i) {
@@ -149,6 +152,18 @@ __global__ __launch_bounds__(256) void delta_step(DeltaArgs A) {
       *reinterpret_cast<float4v*>(A.state_out + at + (size_t)i * A.dv) = x;
     }
   }
+}
+
+template <typename T, int DK>
+__global__ __launch_bounds__(256) void delta_step(DeltaArgs A) {
+  const uint32_t waves = blockDim.x >> 6, wave = threadIdx.x >> 6;
+  const uint32_t tiles = A.dv / 16, groups = (tiles + waves - 1) / waves;
+  const uint32_t tile = blockIdx.x % groups * waves + wave;
+  const uint32_t head = blockIdx.x / groups % A.heads, seq = blockIdx.x / groups / A.heads;
+  uint32_t first, count;
+  size_t row;
+  if (!sequence(A, seq, &first, &count, &row) || tile >= tiles) return;
+  walk_all<T, DK>(A, first, count, row, head, tile);
 }
 
 // ------------------------------------------------------------ chunk by chunk
@@ -175,7 +190,19 @@ __global__ __launch_bounds__(256) void delta_step(DeltaArgs A) {
 // a result's registers are the next product's operand: a lane (i, j) of a result
 // holds rows 4j .. 4j+3 of a tile of 16, so operand element e of lane row j
 // stands for token 32 s + 16 (e / 4) + 4 j + e % 4 of step s.
+//
+// Sums over a chunk's tokens meet zeros where a token is not seen, and zero times
+// infinity is NaN; and e^G may pass fp32 where the recurrence, whose decays meet
+// smaller values one by one, does not. Both leave the final state non-finite: what an
+// infinity or NaN in S, U, T or the scalars gets into is every row of its columns, for
+// good (P, and the scalars of Q, are looked at by themselves). So where a final state
+// has a number of 2^127 or more, or NaN, the sequence is gone through again token by
+// token, and tokens before a non-finite one keep their values.
 constexpr int kChunk = 64;
+__device__ __forceinline__ bool huge(float x) { return !(fabsf(x) < 0x1p127f); }
+__device__ __forceinline__ bool huge(float4v x, float4v y) {   // one of them, or their sum
+  return huge((fabsf(x[0]) + fabsf(x[1])) + (fabsf(x[2]) + fabsf(x[3])) + ((fabsf(y[0]) + fabsf(y[1])) + (fabsf(y[2]) + fabsf(y[3]))));
+}
 
 template <typename T> struct Parts;
 template <> struct Parts<__bf16> { static constexpr int kIn = 1, kOut = 2; };
@@ -206,7 +233,8 @@ struct ChunkArgs {
   uint4v *key, *head;   // [slot][key head][Room::kKey][64], [slot][head][Room::kHead][64]
   uint32_t each;        // value heads of a workgroup of delta_prepare
 };
-// Floats of a head's last kilobyte.
+// Floats of a head's last kilobyte. kLast NaN makes the state NaN, and so sends the
+// sequence through `walk`.
 enum { kRowK = 0, kRowQ = 64, kColU = 128, kLast = 192 };
 
 template <int N> __device__ __forceinline__ void split4(float4v x, bf16x4 (&out)[N]) {
@@ -252,6 +280,7 @@ __global__ __launch_bounds__(256) void delta_prepare(ChunkArgs C) {
   float(*m1)[kPitch] = reinterpret_cast<float(*)[kPitch]>(lds);   // in kf's place, once that is read
   float(*m2)[kPitch] = reinterpret_cast<float(*)[kPitch]>(lds + W::kShared / 16);
   __shared__ double total[kChunk];
+  __shared__ int odd;   // a huge number in this head's P or scalars
   __shared__ __attribute__((aligned(16))) float kn[kChunk], qn[kChunk], bt[kChunk];
 
   const uint32_t chunks = (A.max_tokens + kChunk - 1) / kChunk;
@@ -348,10 +377,13 @@ __global__ __launch_bounds__(256) void delta_prepare(ChunkArgs C) {
       bt[lane] = lane < n ? A.beta[(int64_t)(first + lane) * A.beta_token + head] : 0.f;
       const double last = __shfl(x, 63);
       const float gamma = __builtin_amdgcn_exp2f((float)x);
-      scalars[kRowK + lane] = gamma * kn[lane];
-      scalars[kRowQ + lane] = gamma * qn[lane] * A.scale;
-      scalars[kColU + lane] = __builtin_amdgcn_exp2f((float)(last - x)) * kn[lane];
-      if (lane == 0) scalars[kLast] = __builtin_amdgcn_exp2f((float)last);
+      const float row_k = gamma * kn[lane], row_q = gamma * qn[lane] * A.scale;
+      const float col_u = __builtin_amdgcn_exp2f((float)(last - x)) * kn[lane], all = __builtin_amdgcn_exp2f((float)last);
+      scalars[kRowK + lane] = row_k;
+      scalars[kRowQ + lane] = row_q;
+      scalars[kColU + lane] = col_u;
+      const bool any = __any(huge(row_k) | huge(row_q) | huge(col_u) | huge(all));
+      if (lane == 0) scalars[kLast] = all, odd = any;
     }
     lds_barrier();
     // P row by row, then A, through m1.
@@ -370,8 +402,10 @@ __global__ __launch_bounds__(256) void delta_prepare(ChunkArgs C) {
     for (int s = 0; s < 2; ++s) {
       if (s > w / 2) continue;
       bf16x8 x[PO];
-      split8<PO>(*reinterpret_cast<const float4v*>(&m1[16 * w + i][32 * s + 4 * j]),
-                 *reinterpret_cast<const float4v*>(&m1[16 * w + i][32 * s + 16 + 4 * j]), x);
+      const float4v y = *reinterpret_cast<const float4v*>(&m1[16 * w + i][32 * s + 4 * j]);
+      const float4v z = *reinterpret_cast<const float4v*>(&m1[16 * w + i][32 * s + 16 + 4 * j]);
+      if (huge(y, z)) odd = 1;
+      split8<PO>(y, z, x);
 #pragma unroll
       for (int p = 0; p < PO; ++p)
         out[(W::kT + (triangle(w) + s) * PO + p) * 64 + lane] = __builtin_bit_cast(uint4v, x[p]);
@@ -432,12 +466,14 @@ __global__ __launch_bounds__(256) void delta_prepare(ChunkArgs C) {
       if (s > w / 2) continue;
       const int c = 32 * s + 4 * j;
       bf16x8 x[3];
-      split8<3>(*reinterpret_cast<const float4v*>(&m2[16 * w + i][c]) * *reinterpret_cast<const float4v*>(&bt[c]),
-                *reinterpret_cast<const float4v*>(&m2[16 * w + i][c + 16]) * *reinterpret_cast<const float4v*>(&bt[c + 16]), x);
+      const float4v y = *reinterpret_cast<const float4v*>(&m2[16 * w + i][c]) * *reinterpret_cast<const float4v*>(&bt[c]);
+      const float4v z = *reinterpret_cast<const float4v*>(&m2[16 * w + i][c + 16]) * *reinterpret_cast<const float4v*>(&bt[c + 16]);
+      split8<3>(y, z, x);
 #pragma unroll
       for (int p = 0; p < 3; ++p) out[((triangle(w) + s) * 3 + p) * 64 + lane] = __builtin_bit_cast(uint4v, x[p]);
     }
     lds_barrier();
+    if (threadIdx.x == 0 && odd) scalars[kLast] = NAN;   // behind its own store of the same place
   }
 }
 
@@ -461,6 +497,7 @@ __global__ __launch_bounds__(512) void delta_scan(ChunkArgs C) {
   constexpr bool kAhead = KS * N + TPW * 2 * N <= 32;
   const DeltaArgs& A = C.d;
   __shared__ uint4v sf[3][KS][64], rf[3][2][64], uf[PO][2][64], wf[3][2][64];
+  __shared__ int odd;   // a huge number in the final state
   const int lane = threadIdx.x & 63, i = lane & 15, j = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), w = wave & 3;
   const bool chain = wave < 4;
@@ -474,6 +511,7 @@ __global__ __launch_bounds__(512) void delta_scan(ChunkArgs C) {
   if (!sequence(A, seq, &first, &count, &row)) return;
   const uint32_t slot = first / kChunk + seq, chunks = (count + kChunk - 1) / kChunk;
   const uint32_t col = tile * 16 + i;
+  if (threadIdx.x == 0) odd = 0;
   const int steps = w < 2 ? 1 : 2;   // of T's and P's row tile w
 
   // Four values of lane row r into half h of an operand's parts.
@@ -628,6 +666,15 @@ __global__ __launch_bounds__(512) void delta_scan(ChunkArgs C) {
       if constexpr (!kAhead) load1(next);
     }
     __builtin_amdgcn_s_setprio(0);
+    bool any = false;
+#pragma unroll
+    for (int t = 0; t < TPW; ++t) any |= huge(state[t], float4v{0, 0, 0, 0});
+    if (chunks && any) odd = 1;
+    __syncthreads();   // the outputs are written, too
+    if (odd) {
+      if (w == 0) walk_all<T, DK>(A, first, count, row, head, tile);
+      return;
+    }
     if (A.state_out) {
 #pragma unroll
       for (int t = 0; t < TPW; ++t)
@@ -678,6 +725,7 @@ __global__ __launch_bounds__(512) void delta_scan(ChunkArgs C) {
       for (int e = 0; e < 4; ++e)
         if (token + e < count) out[(int64_t)(token + e) * A.o_token] = (T)acc[0][e];
     }
+    __syncthreads();   // the chain's last one
   }
 }
 

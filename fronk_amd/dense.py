@@ -79,7 +79,8 @@ def delta_rule(q, k, v, g, beta, state_in=None, state_out=None, *, scale=None, o
         u = beta (v - a S^T k);  S <- a S + k u^T;  o = scale S^T q,  a = exp(g)
     q, k [tokens, key_heads, key_dim], v [tokens, heads, value_dim], g and beta
     [tokens, heads] fp32. normalize: q and k are divided by sqrt(sum of squares
-    + 1e-6) first; scale: key_dim ** -0.5 unless given.
+    + 1e-6) first; scale: key_dim ** -0.5 unless given. Non-finite inputs reach
+    no token before theirs.
 
     offsets (int32, sequences + 1): sequence i is tokens offsets[i] ..
     offsets[i+1]-1, at most max_tokens (default: all tokens; the work is laid

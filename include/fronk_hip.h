@@ -263,8 +263,15 @@ enum { FR_HIP_BAD_OFFSET = 1, FR_HIP_BAD_SLOT = 2, FR_HIP_BAD_PAGE = 4, FR_HIP_B
  * a = exp(g), b = beta:
  *     u = b (v - a S^T k);   S <- a S + k u^T;   o = scale S^T q
  * and with FR_HIP_DELTA_NORMALIZE k and q are first divided by
- * sqrt(sum of squares + 1e-6). g <= 0 (a decay) keeps the state bounded; any
- * finite g is computed.
+ * sqrt(sum of squares + 1e-6). g <= 0 (a decay) keeps the state bounded; above
+ * 0 it grows, and any g whose a is an fp32 number (up to 88.7) is computed.
+ * A token with a non-finite q has non-finite outputs, of the heads that it
+ * reaches; one with a non-finite k, beta or g (but g of -infinity empties the
+ * state) or, by columns, v has non-finite outputs from it on, and leaves such a
+ * state. Tokens before it and other sequences are computed as without it.
+ * (fp32 magnitudes above 3.38e38 may count as infinite.) o shares no memory with
+ * an input: a sequence that leaves fp32 as long sequences are computed is gone
+ * through a second time.
  * Sequence i is tokens offsets[i] .. offsets[i+1]-1, at most max_tokens of
  * them (offsets NULL: max_tokens each), and its state is row slot[i] of the
  * pools (slot NULL: row i); slot -1: the sequence is skipped, nothing of it is
