@@ -85,6 +85,7 @@ SIGNATURES = {
                                                C.POINTER(C.c_double)]),
     "fr_hip_debug_partials": (C.c_int, [C.c_uint, C.c_uint, C.POINTER(C.c_float)]),
     "fr_hip_debug_read": (C.c_int, [C.c_uint, C.c_uint64, C.c_void_p, C.c_uint64]),
+    "fr_hip_device": (C.c_int, []),
     # The dense operators (request structures: fronk_amd.dense).
     "fr_hip_delta_workspace": (C.c_size_t, [C.c_void_p]),
     "fr_hip_delta_rule": (C.c_int, [C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]),

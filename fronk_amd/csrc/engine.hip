@@ -15,3 +15,5 @@ int enter(void* stream, hipStream_t* out, unsigned* cus) {
   return FR_HIP_OK;
 }
 }  // namespace fronk
+
+extern "C" int fr_hip_device(void) { return g_open ? E.device : FR_HIP_STATE; }

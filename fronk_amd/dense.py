@@ -1,8 +1,8 @@
 """The dense operators over torch tensors: thin calls of the C ABI
 (include/fronk_hip.h, through host/dense_module.cpp), enqueued on torch's current
 stream, no compute and no fallback of their own. Tensors are on the open engine's
-device (fr_hip_open; the first call here opens theirs) and may have any strides
-but for a contiguous last axis.
+device (fr_hip_open; the first call here opens theirs, and tensors on another one
+are refused) and may have any strides but for a contiguous last axis.
 
   delta_rule   the gated delta rule, decode bursts to prompts
   q4_product   products with 4-bit weights and group scales

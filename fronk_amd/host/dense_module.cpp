@@ -7,6 +7,7 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <ATen/ATen.h>
+#include <c10/core/DeviceGuard.h>
 
 #include <math.h>
 
@@ -69,9 +70,20 @@ at::Tensor make(const at::Tensor* out, at::IntArrayRef shape, const at::Tensor& 
   return *out;
 }
 
+// The engine is one GPU's: on another one's tensors it would work out of order with
+// what made them, or not at all.
+void on_engine(const at::Tensor& as) {
+  const int device = fr_hip_device();
+  if (device >= 0 && device != as.get_device())
+    refuse("the tensors are on GPU " + std::to_string(as.get_device()) + ", the open engine on GPU " + std::to_string(device));
+}
+
 // The call on torch's current stream (HIP's default stream is 0 there), opening
-// the engine first where nothing has.
+// the engine first where nothing has. The C ABI makes its device current: torch's
+// is put back behind it.
 template <typename F> void call(const char* name, const at::Tensor& as, F f) {
+  on_engine(as);
+  const c10::DeviceGuard guard(as.device());
   PyObject* stream = PyObject_CallFunction(g_stream, "i", (int)as.get_device());
   if (!stream) throw python_error();
   void* s = PyLong_AsVoidPtr(stream);
@@ -91,6 +103,7 @@ template <typename F> void call(const char* name, const at::Tensor& as, F f) {
 }
 template <typename R, typename W, typename F>
 void call(const char* name, const at::Tensor& as, const R& request, W workspace, F f) {
+  on_engine(as);
   const size_t n = workspace(&request);
   at::Tensor w;
   if (n) w = at::empty({(int64_t)n}, as.options().dtype(at::kByte));

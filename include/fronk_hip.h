@@ -73,6 +73,8 @@ typedef struct {
  * FR_HIP_UNSUPPORTED when `device` is not a gfx950 GPU. */
 int fr_hip_open(int device);
 int fr_hip_close(void);
+/* The open engine's device (no reference counterpart); FR_HIP_STATE without one. */
+int fr_hip_device(void);
 /* Name of the open device's architecture ("gfx950"), for probe(). */
 int fr_hip_probe(int device, char *arch, size_t cap);
 
@@ -249,7 +251,8 @@ int fr_hip_batch_output(void *stream, float *y, size_t count, unsigned *status);
  * that the caller clears (NULL: not reported).
  *
  * stream: a hipStream_t, NULL = the library stream (which does not wait for
- * the default stream), FR_HIP_STREAM_DEFAULT = HIP's default stream.
+ * the default stream), FR_HIP_STREAM_DEFAULT = HIP's default stream. It and the
+ * memory are of the engine's device (fr_hip_device), which a call makes current.
  * type: of activations in and out; sums, softmax statistics, norms and states
  * are fp32 whatever it is. Strides are in elements and a row's last axis is
  * contiguous; bases and strides of whole 16 bytes are read fastest, and any
