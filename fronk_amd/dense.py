@@ -8,6 +8,9 @@ are refused) and may have any strides but for a contiguous last axis.
   q4_product   products with 4-bit weights and group scales
   KVCache, kv_append, kv_read, kv_attend   the paged 8-bit key/value cache
 
+They have no backward pass: a tensor that requires a gradient is refused unless
+under torch.no_grad() (or inference_mode), one with a forward-mode tangent always.
+
 A refused call raises ValueError before anything is enqueued. What only the
 device can see (offsets, slots, pages, lengths) is bounds-checked there: a bad
 entry reads and writes nothing and sets its bit (BAD_*) in `status`, an int32

@@ -8,6 +8,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/GradMode.h>
 
 #include <math.h>
 
@@ -24,11 +25,19 @@ PyObject *g_open, *g_stream;   // open the engine on a device; give torch's curr
 
 [[noreturn]] void refuse(const std::string& what) { throw std::invalid_argument(what); }
 
-// A tensor argument; None where that is taken.
+// A tensor argument; None where that is taken. There is no backward pass and no
+// forward-mode one, so one that autograd would follow here is refused.
 const at::Tensor* tensor(PyObject* o, const char* name, bool optional = false) {
   if (o == Py_None && optional) return nullptr;
   if (!THPVariable_Check(o)) refuse(std::string(name) + " is a tensor");
-  return &THPVariable_Unpack(o);
+  const at::Tensor& t = THPVariable_Unpack(o);
+  if ((t.requires_grad() && c10::GradMode::is_enabled()) || t._fw_grad(0).defined())
+    refuse(std::string(name) + " carries a gradient, which is not followed here: detach it, or call under torch.no_grad()");
+  return &t;
+}
+// What a call wrote to, so that autograd sees that it has changed.
+void written(const at::Tensor* t) {
+  if (t && !t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
 }
 
 unsigned type_of(const at::Tensor& t, const char* name) {
@@ -187,6 +196,7 @@ PyObject* delta_rule(PyObject*, Args a, Py_ssize_t n) {
     r.state_out = after ? static_cast<float*>(after->data_ptr()) : nullptr;
     r.status = ints<uint32_t*>(status, 1, v, "status");
     call("fr_hip_delta_rule", v, r, fr_hip_delta_workspace, fr_hip_delta_rule);
+    written(out), written(after), written(status);
     return THPVariable_Wrap(o);
   });
 }
@@ -216,6 +226,7 @@ PyObject* q4_product(PyObject*, Args a, Py_ssize_t n) {
     r.zeros = zeros ? static_cast<const uint8_t*>(zeros->data_ptr()) : nullptr, r.y = y.data_ptr();
     r.x_token = x.stride(0), r.y_token = y.stride(0);
     call("fr_hip_q4_product", x, r, fr_hip_q4_workspace, fr_hip_q4_product);
+    written(out);
     return THPVariable_Wrap(y);
   });
 }
@@ -262,8 +273,11 @@ PyObject* kv_append(PyObject*, Args a, Py_ssize_t n) {
     fr_hip_kv_write r = {};
     const at::Tensor& cache = cache_of(a[0], &r.cache);
     const at::Tensor& k = *tensor(a[1], "k");
-    tokens_of(&r, k, *tensor(a[2], "v"), *tensor(a[3], "slots"), tensor(a[4], "status", true), cache);
+    const at::Tensor* status = tensor(a[4], "status", true);
+    tokens_of(&r, k, *tensor(a[2], "v"), *tensor(a[3], "slots"), status, cache);
     call("fr_hip_kv_append", k, [&](void* s) { return fr_hip_kv_append(&r, s); });
+    for (int i = 0; i < 4; ++i) written(&THPVariable_Unpack(PyTuple_GET_ITEM(a[0], i)));
+    written(status);
     Py_RETURN_NONE;
   });
 }
@@ -278,8 +292,10 @@ PyObject* kv_read(PyObject*, Args a, Py_ssize_t n) {
     const auto options = cache.options().dtype(type);
     const int64_t shape[3] = {slots.numel(), cache.size(1), cache.size(3)};
     const at::Tensor k = at::empty(shape, options), v = at::empty(shape, options);
-    tokens_of(&r, k, v, slots, tensor(a[3], "status", true), cache);
+    const at::Tensor* status = tensor(a[3], "status", true);
+    tokens_of(&r, k, v, slots, status, cache);
     call("fr_hip_kv_read", k, [&](void* s) { return fr_hip_kv_read(&r, s); });
+    written(status);
     return Py_BuildValue("(NN)", THPVariable_Wrap(k), THPVariable_Wrap(v));
   });
 }
@@ -313,6 +329,7 @@ PyObject* kv_attend(PyObject*, Args a, Py_ssize_t n) {
     r.q = q.data_ptr(), r.o = o.data_ptr(), r.table = static_cast<const int32_t*>(table.data_ptr());
     r.q_token = q.stride(0), r.q_head = q.stride(1), r.o_token = o.stride(0), r.o_head = o.stride(1);
     call("fr_hip_kv_attend", q, r, fr_hip_kv_workspace, fr_hip_kv_attend);
+    written(out), written(status);
     return THPVariable_Wrap(o);
   });
 }

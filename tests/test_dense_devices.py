@@ -83,14 +83,42 @@ assert calls.value == 0
 
 
 def test_an_engine_that_is_not_open_refuses_nothing(folder):
-    """Opening it is the call's; here it comes as far as making the device current."""
+    """What opens it is the call itself."""
     run(folder, """
 device.value = -2
+for n, (f, args) in enumerate(made(0).values()):
+    f(*args)
+    assert calls.value == n + 1
+""")
+
+
+def test_what_autograd_would_follow_is_refused(folder):
+    """Each floating-point argument of each call; under no_grad it is not."""
+    run(folder, """
+import torch.autograd.forward_ad as fwd
+seen = 0
 for name, (f, args) in made(0).items():
+    for i, t in enumerate(args):
+        if not torch.is_tensor(t) or not t.is_floating_point():
+            continue
+        seen += 1
+        t.requires_grad_()
+        try:
+            f(*args)
+        except ValueError as e:
+            assert "gradient" in str(e), (name, i, str(e))
+        else:
+            raise AssertionError((name, i))
+        with torch.no_grad():
+            f(*args)
+        t.requires_grad_(False)
+assert (seen, calls.value) == (5 + 2 + 2 + 1, seen), (seen, calls.value)
+with fwd.dual_level():
+    x = fwd.make_dual(torch.zeros(2, 64), torch.ones(2, 64))
     try:
-        f(*args)
+        _dense.q4_product(x, x, x, None, None)
     except ValueError as e:
-        raise AssertionError((name, str(e)))
-    except RuntimeError:
-        pass
+        assert "gradient" in str(e), str(e)
+    else:
+        raise AssertionError("a tangent")
 """)
