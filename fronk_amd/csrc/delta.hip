@@ -787,7 +787,7 @@ void launch_step(const fr_hip_delta* r, const DeltaArgs& A, hipStream_t s) {
   // Single wavefronts while they fit the card's SIMDs once over, so that they
   // spread over all of them; then four neighbouring tiles a workgroup, whose
   // 64-byte rows make whole lines.
-  const uint32_t waves = total <= 1024 ? 1 : tiles < 4 ? tiles : 4;
+  const uint32_t waves = total <= 4 * kUnits ? 1 : tiles < 4 ? tiles : 4;
   const dim3 grid((uint32_t)((uint64_t)r->sequences * r->heads * ((tiles + waves - 1) / waves))), block(64 * waves);
   switch (r->key_dim) {
     case 64: hipLaunchKernelGGL((delta_step<T, 64>), grid, block, 0, s, A); break;
@@ -802,14 +802,13 @@ int launch_chunks(const fr_hip_delta* r, const DeltaArgs& A, void* workspace, hi
   constexpr size_t kLds = W::kShared + W::kMatrix;
   const size_t slots = (size_t)r->tokens / kChunk + r->sequences;
   ChunkArgs C = {A, static_cast<uint4v*>(workspace), static_cast<uint4v*>(workspace) + slots * W::kKey * r->key_heads * 64, 1};
-  static const hipError_t wide = hipFuncSetAttribute(reinterpret_cast<const void*>(&delta_prepare<T, DK>),
-                                                     hipFuncAttributeMaxDynamicSharedMemorySize, (int)kLds);
-  FRONK_CK(wide);
+  static fronk::Devices allowed;
+  if (allow_lds(&delta_prepare<T, DK>, kLds, &allowed)) return FR_HIP_IO;
   const uint32_t chunks = (A.max_tokens + kChunk - 1) / kChunk;
   // The heads of a key head share its products where there are enough chunks to
   // fill the card without.
   const uint32_t prepares = r->sequences * chunks * r->key_heads, group = r->heads / r->key_heads;
-  if (prepares >= 3 * 256) C.each = group;
+  if (prepares >= 3 * kUnits) C.each = group;
   hipLaunchKernelGGL((delta_prepare<T, DK>), dim3(prepares, (group + C.each - 1) / C.each), dim3(256), kLds, s, C);
   hipLaunchKernelGGL((delta_scan<T, DK>), dim3(r->sequences * r->heads * (r->value_dim / 16)), dim3(512), 0, s, C);
   return FR_HIP_OK;
@@ -849,8 +848,7 @@ int fr_hip_delta_rule(const fr_hip_delta* req, void* workspace, size_t bytes, vo
   const size_t need = workspace_bytes(req);
   if (need && (!workspace || bytes < need || (uintptr_t)workspace % 16)) return FR_HIP_INVALID;
   hipStream_t s;
-  unsigned cus;
-  rc = fronk::enter(stream, &s, &cus);
+  rc = fronk::enter(stream, &s);
   if (rc || !req->sequences) return rc;
   const DeltaArgs A = arguments(req);
   switch (req->type) {

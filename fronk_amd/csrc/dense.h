@@ -10,17 +10,20 @@
 
 #include <stdint.h>
 
+#include "devices.h"
 #include "fronk_hip.h"
 
 namespace fronk {
 
 // Makes the open engine's device current and resolves `stream`; FR_HIP_STATE
 // without an open engine.
-__attribute__((visibility("hidden"))) int enter(void* stream, hipStream_t* out, unsigned* cus);
+__attribute__((visibility("hidden"))) int enter(void* stream, hipStream_t* out);
 
 }  // namespace fronk
 
 namespace {
+
+constexpr uint32_t kUnits = 256;   // an MI355X's compute units, of four SIMDs each
 
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
@@ -95,6 +98,14 @@ __device__ __forceinline__ float4v mma(half8v a, half8v b, float4v c) {
 __device__ __forceinline__ bf16x2 to_bf16(float a, float b) {
   const float2v v = {a, b};
   return __builtin_convertvector(v, bf16x2);
+}
+
+// Lets a kernel have `bytes` of dynamic LDS on the engine's device. `done` is the
+// kernel's own.
+template <typename Kernel> int allow_lds(Kernel kernel, size_t bytes, fronk::Devices* done) {
+  return fronk::once_a_device(done, fr_hip_device(), [&] {
+    return (int)hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+  });
 }
 
 #define FRONK_CK(x) do { if ((x) != hipSuccess) return FR_HIP_IO; } while (0)

@@ -7,11 +7,10 @@
 #include "dense.h"
 
 namespace fronk {
-int enter(void* stream, hipStream_t* out, unsigned* cus) {
+int enter(void* stream, hipStream_t* out) {
   if (!g_open) return FR_HIP_STATE;
   CK(hipSetDevice(E.device));
   *out = !stream ? E.stream : stream == FR_HIP_STREAM_DEFAULT ? hipStream_t(nullptr) : static_cast<hipStream_t>(stream);
-  *cus = E.cus;
   return FR_HIP_OK;
 }
 }  // namespace fronk

@@ -725,8 +725,7 @@ void launch_tokens(const KvArgs& A, hipStream_t s) {
 template <bool READ>
 int tokens_call(const KvArgs& A, unsigned type, void* stream) {
   hipStream_t s;
-  unsigned cus;
-  const int rc = fronk::enter(stream, &s, &cus);
+  const int rc = fronk::enter(stream, &s);
   if (rc || !A.tokens) return rc;
   switch (type) {
     case FR_HIP_F32: launch_tokens<float, READ>(A, s); break;
@@ -768,7 +767,7 @@ Cut cut_of(const fr_hip_kv_query* r) {
   // About one workgroup for each of 256 compute units (two: 131072 tokens of one
   // stream 34 + 6 us against 28 + 5, a ragged batch of 32 the same), none with less
   // than a tile for each of its wavefronts.
-  const uint64_t want = c.items ? (256 + c.items - 1) / c.items : 1, most = (r->max_context + 255) / 256;
+  const uint64_t want = c.items ? (kUnits + c.items - 1) / c.items : 1, most = (r->max_context + 255) / 256;
   uint64_t n = want < most ? want : most;
   n = n < 1 ? 1 : n > 256 ? 256 : n;
   c.chunk = (uint32_t)((r->max_context + n * 256 - 1) / (n * 256)) * 256;
@@ -835,8 +834,7 @@ int fr_hip_kv_attend(const fr_hip_kv_query* r, void* workspace, size_t bytes, vo
   const Cut c = cut_of(r);
   if (c.bytes && (!workspace || bytes < c.bytes || (uintptr_t)workspace % 16)) return FR_HIP_INVALID;
   hipStream_t s;
-  unsigned cus;
-  rc = fronk::enter(stream, &s, &cus);
+  rc = fronk::enter(stream, &s);
   if (rc || !r->sequences) return rc;
   AttendArgs A;
   A.cache = cache_of(r->cache);

@@ -572,9 +572,8 @@ template <typename T, int MT, int G, bool ZEROS, bool WHOLE>
 int launch_rows(const RowsArgs& C, dim3 grid, uint32_t waves, hipStream_t s) {
   const size_t x = (size_t)C.segment * 256 * Operand<T>::kParts * (C.a.tokens < MT * 16 ? C.a.tokens : MT * 16);
   const size_t sums = (size_t)waves * MT * 16 * 16 * sizeof(float);
-  static const hipError_t wide = hipFuncSetAttribute(reinterpret_cast<const void*>(&q4_rows<T, MT, G, ZEROS, WHOLE>),
-                                                     hipFuncAttributeMaxDynamicSharedMemorySize, (int)kRowsLds);
-  FRONK_CK(wide);
+  static fronk::Devices allowed;
+  if (allow_lds(&q4_rows<T, MT, G, ZEROS, WHOLE>, kRowsLds, &allowed)) return FR_HIP_IO;
   hipLaunchKernelGGL((q4_rows<T, MT, G, ZEROS, WHOLE>), grid, dim3(64 * waves), x > sums ? x : sums, s, C);
   return FR_HIP_OK;
 }
@@ -589,7 +588,7 @@ int launch_rows(const Q4Args& A, bool whole, hipStream_t s) {
   // the card's compute units, but not below one block for each, nor beyond what
   // LDS holds of x for all of them (at least one split's: 12 KB a block).
   RowsArgs C = {A, 1, 0};
-  while (C.splits < 8 && (uint64_t)tiles * y * C.splits < 2048 && C.splits * 2 <= blocks && 2 * C.splits * block <= kRowsLds)
+  while (C.splits < 8 && (uint64_t)tiles * y * C.splits < 8 * kUnits && C.splits * 2 <= blocks && 2 * C.splits * block <= kRowsLds)
     C.splits *= 2;
   const uint32_t waves = 8, each = waves / C.splits;
   C.segment = (uint32_t)(kRowsLds / block) / C.splits * C.splits;
@@ -624,9 +623,8 @@ template <typename T, int G, int NT, bool ZEROS, bool WHOLE>
 int launch_tiles(const TileArgs& C, uint32_t blocks, hipStream_t s) {
   constexpr size_t x = (size_t)4 * Packed<T>::kParts * 1024 * 16, sums = (size_t)kTokens * (64 * NT + 4) * sizeof(float);
   constexpr size_t lds = x > sums ? x : sums;
-  static const hipError_t wide = hipFuncSetAttribute(reinterpret_cast<const void*>(&q4_tiles<T, G, NT, ZEROS, WHOLE>),
-                                                     hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
-  FRONK_CK(wide);
+  static fronk::Devices allowed;
+  if (allow_lds(&q4_tiles<T, G, NT, ZEROS, WHOLE>, lds, &allowed)) return FR_HIP_IO;
   const uint32_t tiles = (C.a.rows + 64 * NT - 1) / (64 * NT);
   hipLaunchKernelGGL((q4_tiles<T, G, NT, ZEROS, WHOLE>), dim3((tiles + 7) / 8 * 8 * blocks), dim3(512), lds, s, C, blocks);
   return FR_HIP_OK;
@@ -645,9 +643,9 @@ int launch_widest(const TileArgs& C, uint32_t blocks, hipStream_t s) {
   constexpr int P = Packed<T>::kParts, kMost = P == 1 && G == 128 && !ZEROS ? 4 : 2;
   const uint64_t tiles = (uint64_t)((C.a.rows + 63) / 64) * blocks;
   if constexpr (kMost >= 4)
-    if (tiles >= 4 * 256) return launch_tiles<T, G, 4, ZEROS>(C, blocks, s);
+    if (tiles >= 4 * kUnits) return launch_tiles<T, G, 4, ZEROS>(C, blocks, s);
   if constexpr (kMost >= 2)
-    if (tiles >= 2 * 256) return launch_tiles<T, G, 2, ZEROS>(C, blocks, s);
+    if (tiles >= 2 * kUnits) return launch_tiles<T, G, 2, ZEROS>(C, blocks, s);
   return launch_tiles<T, G, 1, ZEROS>(C, blocks, s);
 }
 
@@ -701,8 +699,7 @@ int fr_hip_q4_product(const fr_hip_q4* req, void* workspace, size_t bytes, void*
   const size_t need = workspace_bytes(req);
   if (need && (!workspace || bytes < need || (uintptr_t)workspace % 16)) return FR_HIP_INVALID;
   hipStream_t s;
-  unsigned cus;
-  rc = fronk::enter(stream, &s, &cus);
+  rc = fronk::enter(stream, &s);
   if (rc || !req->tokens || !req->rows) return rc;
   const int64_t n = 16 / (int64_t)elem_size(req->type);
   Q4Args A;
