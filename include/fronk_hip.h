@@ -301,7 +301,12 @@ typedef struct {
     uint32_t *status;
 } fr_hip_delta;
 /* Bytes of device workspace (16-byte aligned) that fr_hip_delta_rule needs for
- * these sizes; 0: none, and also for sizes that it refuses. */
+ * these sizes; 0: none, and also for sizes that it refuses. Sequences that all have
+ * up to 32 tokens need none, or 4 bytes each above 2048 of them. Where one may have
+ * more (max_tokens), there are tokens / 64 + sequences slots for chunks, each of
+ * 3 * 128 * key_dim * parts bytes a key head and 18 KB + 6 KB * parts_out + 1 KB a
+ * head (parts, parts_out: bf16 1 and 2, fp16 2 and 2, fp32 3 and 3): for 16 key heads
+ * of 128 and 32 heads 28 KB a token in bf16, 54 KB in fp32. */
 size_t fr_hip_delta_workspace(const fr_hip_delta *req);
 int fr_hip_delta_rule(const fr_hip_delta *req, void *workspace, size_t bytes, void *stream);
 

@@ -254,3 +254,23 @@ def test_q4_grids_end_below_2_32_threads(tokens, rows, rc):
     r = q4_request(tokens=tokens, rows=rows)
     n = fa.lib().fr_hip_q4_workspace(C.addressof(r))
     assert fa.lib().fr_hip_q4_product(C.addressof(r), P if n else None, n, None) == (fa.STATE if rc is None else rc)
+
+
+def test_delta_workspace_for_the_order_of_many_sequences():
+    """Above 2048 sequences, four bytes of each beside what chunks take."""
+    no_engine()
+
+    def size(**kw):
+        r = delta_request(**kw)
+        return fa.lib().fr_hip_delta_workspace(C.addressof(r))
+
+    n = dict(tokens=5000, sequences=2048, slots=5000)
+    more = {**n, "sequences": 2049}
+    assert size(**n) == 0 and size(**more) == 4 * 2049
+    assert size(sequences=2049, tokens=2049, slots=2049, offsets=None, max_tokens=1) == 0
+    a, b = size(**n, max_tokens=64), size(**more, max_tokens=64)
+    assert a > 0 and a % 1024 == 0 and b % 1024 == (4 * 2049) % 1024
+    r = delta_request(**more)
+    for w, given in ((None, 4 * 2049), (P, 4 * 2049 - 1), (P + 8, 4 * 2049)):
+        assert fa.lib().fr_hip_delta_rule(C.addressof(r), w, given, None) == fa.INVALID
+    assert fa.lib().fr_hip_delta_rule(C.addressof(r), P, 4 * 2049, None) == fa.STATE
