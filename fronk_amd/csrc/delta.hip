@@ -768,9 +768,14 @@ __global__ __launch_bounds__(512) void delta_scan(ChunkArgs C) {
 
 // ---------------------------------------------------------------------- host
 
-// Bursts go token by token; from this many tokens on, chunks.
+// Calls go token by token; where a sequence may have this many, in chunks. Measured,
+// token by token against chunks in us: one stream of 32 heads of 128 x 128 in bf16 21,
+// 19 (16 tokens), 36, 19 (32), 67, 20 (64), in fp32 20, 23 (16), 34, 23 (32); 64 such
+// streams 235, 316 (24), 309, 323 (32), 457, 335 (48), in fp32 305, 487 (32), 452, 493
+// (48), 595, 500 (64). Between the borders of few streams (about 16) and of many (about
+// 33 and, fp32, 50).
 constexpr unsigned kChunkFrom = 33;
-bool in_chunks(const fr_hip_delta* r) { return r->max_tokens >= kChunkFrom; }
+bool in_chunks(const fr_hip_delta* r) { return r->max_tokens >= kChunkFrom && r->tokens >= kChunkFrom; }
 
 int check(const fr_hip_delta* r) {
   if (!r || r->type > FR_HIP_BF16 || (r->flags & ~(unsigned)FR_HIP_DELTA_NORMALIZE)) return FR_HIP_INVALID;
@@ -856,9 +861,8 @@ template <typename T>
 size_t room(const fr_hip_delta* r) {
   return r->key_dim == 64 ? Room<T, 64>::bytes(r) : r->key_dim == 128 ? Room<T, 128>::bytes(r) : Room<T, 256>::bytes(r);
 }
-bool chunked(const fr_hip_delta* r) { return in_chunks(r) && r->tokens; }
 size_t chunk_bytes(const fr_hip_delta* r) {   // a multiple of 1024
-  if (!chunked(r)) return 0;
+  if (!in_chunks(r)) return 0;
   return r->type == FR_HIP_F32 ? room<float>(r) : r->type == FR_HIP_F16 ? room<_Float16>(r) : room<__bf16>(r);
 }
 // With more sequences than this, their order is looked at beforehand. Measured, in
@@ -873,7 +877,7 @@ size_t workspace_bytes(const fr_hip_delta* r) {
 
 template <typename T>
 int launch(const fr_hip_delta* r, const DeltaArgs& A, void* workspace, hipStream_t s) {
-  if (!chunked(r)) {
+  if (!in_chunks(r)) {
     launch_step<T>(r, A, s);
     return FR_HIP_OK;
   }

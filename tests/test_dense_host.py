@@ -274,3 +274,11 @@ def test_delta_workspace_for_the_order_of_many_sequences():
     for w, given in ((None, 4 * 2049), (P, 4 * 2049 - 1), (P + 8, 4 * 2049)):
         assert fa.lib().fr_hip_delta_rule(C.addressof(r), w, given, None) == fa.INVALID
     assert fa.lib().fr_hip_delta_rule(C.addressof(r), P, 4 * 2049, None) == fa.STATE
+
+
+def test_delta_goes_by_the_tokens_there_are():
+    """A generous max_tokens is no reason for chunks, nor their workspace."""
+    no_engine()
+    for tokens, most, chunks in ((10, 4096, False), (32, 33, False), (33, 32, False), (33, 33, True), (0, 64, False)):
+        r = delta_request(tokens=tokens, max_tokens=most)
+        assert (fa.lib().fr_hip_delta_workspace(C.addressof(r)) > 0) == chunks, (tokens, most)
