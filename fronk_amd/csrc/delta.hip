@@ -849,9 +849,15 @@ int launch_chunks(const fr_hip_delta* r, const DeltaArgs& A, void* workspace, hi
   if (allow_lds(&delta_prepare<T, DK>, kLds, &allowed)) return FR_HIP_IO;
   const uint32_t chunks = (A.max_tokens + kChunk - 1) / kChunk;
   // The heads of a key head share its products where there are enough chunks to
-  // fill the card without.
+  // fill the card without: six workgroups a unit, were there one a head. Measured, one
+  // a head against one for all of a call in us, bf16, by workgroups of the first kind:
+  // 16 key heads and 32 heads of 128 44, 48 (512), 75, 72 (1024), 90, 91 (1280), 103,
+  // 102 (1536), 134, 127 (2048); 4 and 16 heads 61, 76 (512), 88, 95 (768), 109, 114
+  // (1024), 158, 156 (1536), 208, 196 (2048); 16 and 48 heads of 64 44, 47 (768), 72, 66
+  // (1536). (Chunks as far as they are known here: no more than the tokens have.)
   const uint32_t prepares = r->sequences * chunks * r->key_heads, group = r->heads / r->key_heads;
-  if (prepares >= 3 * kUnits) C.each = group;
+  const uint64_t there = (uint64_t)r->tokens / kChunk + r->sequences;
+  if ((there < (uint64_t)r->sequences * chunks ? there * r->key_heads : prepares) * group >= 6 * kUnits) C.each = group;
   hipLaunchKernelGGL((delta_prepare<T, DK>), dim3(prepares, (group + C.each - 1) / C.each), dim3(256), kLds, s, C);
   hipLaunchKernelGGL((delta_scan<T, DK>), dim3(r->sequences * r->heads * (r->value_dim / 16)), dim3(512), 0, s, C);
   return FR_HIP_OK;
