@@ -264,7 +264,8 @@ __global__ __launch_bounds__(512) void q4_rows(RowsArgs R) {
 // they are; a bf16 token is scaled by the power of two that brings its largest
 // to 2^14 .. 2^15, which keeps every value down to 2^-32 of the largest exact
 // and the others to 2^-40 of it, below fp32's rounding of their sum; an fp32
-// token takes two such parts (2^-23 of each value).
+// token takes two such parts: 2^-23 of each value down to 2^-16 of the token's
+// largest, and 2^-39 of the largest below.
 constexpr int kTokens = 64;
 
 template <typename T> struct Packed { static constexpr int kParts = std::is_same<T, float>::value ? 2 : 1; };
@@ -635,12 +636,16 @@ int launch_tiles(const TileArgs& C, uint32_t blocks, hipStream_t s) {
     if (!C.whole) return launch_tiles<T, G, NT, ZEROS, false>(C, blocks, s);
   return launch_tiles<T, G, NT, ZEROS, true>(C, blocks, s);
 }
-// The widest tiles that still give every compute unit one, as far as their
-// registers go: 256 rows leave none for a second part of x, zero points or
-// several groups a block (512 x 4096 x 8192 in groups of 32: 92 us, 75 with 128).
+// The widest tiles that still give every compute unit one, up to those that are the
+// fastest of their kind: 256 rows leave no registers for a second part of x, zero
+// points or several groups a block. 512 x 4096 x 8192 in us with 64, 128 and 256 rows:
+// 16 bits in groups of 128 75, 68, 51, of 64 95, 70, of 32 75, 73, 92; with zero points
+// 85, 84 (128), 93, 83 (64), 84, 101 (32); fp32 141, 97 (128), 136, 100 (64), 161, 135
+// (32), with zero points 149, 101, 146, 111, 164, 157, though some of its wide tiles in
+// groups of 32 keep registers in memory.
 template <typename T, int G, bool ZEROS>
 int launch_widest(const TileArgs& C, uint32_t blocks, hipStream_t s) {
-  constexpr int P = Packed<T>::kParts, kMost = P == 1 && G == 128 && !ZEROS ? 4 : 2;
+  constexpr int kMost = Packed<T>::kParts > 1 ? 2 : G == 128 && !ZEROS ? 4 : G == 32 && ZEROS ? 1 : 2;
   const uint64_t tiles = (uint64_t)((C.a.rows + 63) / 64) * blocks;
   if constexpr (kMost >= 4)
     if (tiles >= 4 * kUnits) return launch_tiles<T, G, 4, ZEROS>(C, blocks, s);
