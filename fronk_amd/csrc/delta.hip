@@ -816,7 +816,7 @@ DeltaArgs arguments(const fr_hip_delta* r) {
   A.sequences = r->sequences, A.tokens = r->tokens, A.max_tokens = r->max_tokens < r->tokens ? r->max_tokens : r->tokens;
   A.key_heads = r->key_heads, A.heads = r->heads, A.dv = r->value_dim;
   // Without state pools a slot only says whether the sequence is skipped.
-  A.slots = r->state_in || r->state_out || r->slot ? r->slots : (uint32_t)INT_MAX;
+  A.slots = r->state_in || r->state_out ? r->slots : (uint32_t)INT_MAX;
   A.scale = r->scale;
   A.normalize = r->flags & FR_HIP_DELTA_NORMALIZE;
   A.wide = all16(r);

@@ -279,7 +279,8 @@ enum { FR_HIP_BAD_OFFSET = 1, FR_HIP_BAD_SLOT = 2, FR_HIP_BAD_PAGE = 4, FR_HIP_B
  * them (offsets NULL: max_tokens each), and its state is row slot[i] of the
  * pools (slot NULL: row i); slot -1: the sequence is skipped, nothing of it is
  * read or written. Slots are distinct. state_in NULL: states begin as zeros;
- * state_out NULL: final states are dropped; both may be one pool. A sequence
+ * state_out NULL: final states are dropped; both may be one pool, and without one
+ * a slot that is not negative says no more than that. A sequence
  * of no tokens passes its state on. Offsets do not go down: a sequence that
  * begins below an offset before it is bad, as is one that ends below its start.
  * key_dim 64, 128 or 256; value_dim a multiple of 16 up to 1024; key_heads
