@@ -786,6 +786,10 @@ int check(const fr_hip_delta* r) {
   if (!r->slot && r->slots < r->sequences && (r->state_in || r->state_out)) return FR_HIP_INVALID;
   if (r->tokens && r->sequences && (!r->q || !r->k || !r->v || !r->g || !r->beta || !r->o)) return FR_HIP_INVALID;
   if (((uintptr_t)r->state_in | (uintptr_t)r->state_out) % 16) return FR_HIP_INVALID;
+  if (r->state_in && r->state_out && r->state_in != r->state_out) {   // pools that share some rows, not all
+    const uintptr_t a = (uintptr_t)r->state_in, b = (uintptr_t)r->state_out, apart = a < b ? b - a : a - b;
+    if (apart / ((uint64_t)r->heads * r->key_dim * r->value_dim * sizeof(float)) < r->slots) return FR_HIP_INVALID;
+  }
   if (((uintptr_t)r->q | (uintptr_t)r->k | (uintptr_t)r->v | (uintptr_t)r->o) % elem_size(r->type)) return FR_HIP_INVALID;
   if (r->key_dim != 64 && r->key_dim != 128 && r->key_dim != 256) return FR_HIP_UNSUPPORTED;
   if (r->value_dim % 16 || r->value_dim > 1024 || r->heads > 65535) return FR_HIP_UNSUPPORTED;

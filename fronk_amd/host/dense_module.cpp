@@ -7,6 +7,7 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <ATen/ATen.h>
+#include <ATen/MemoryOverlap.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/core/GradMode.h>
 
@@ -76,7 +77,15 @@ unsigned u32(int64_t n, const char* name) {
 at::Tensor make(const at::Tensor* out, at::IntArrayRef shape, const at::Tensor& as, const char* what) {
   if (!out) return at::empty(shape, as.options());
   if (out->sizes() != shape || out->scalar_type() != as.scalar_type() || out->device() != as.device()) refuse(what);
+  if (at::has_internal_overlap(*out) == at::MemOverlap::Yes) refuse("out has places of its own for all elements");
   return *out;
+}
+// An output whose places are also read, by other workgroups than write them.
+void apart(const at::Tensor* out, const at::Tensor& in, const char* name) {
+  if (!out || !out->numel() || !in.numel()) return;
+  const auto both = at::get_overlap_status(*out, in);
+  if (both == at::MemOverlapStatus::Full || both == at::MemOverlapStatus::Partial || out->data_ptr() == in.data_ptr())
+    refuse(std::string("out shares memory with ") + name);
 }
 
 // The engine is one GPU's: on another one's tensors it would work out of order with
@@ -180,6 +189,7 @@ PyObject* delta_rule(PyObject*, Args a, Py_ssize_t n) {
     }
     const at::Tensor o = make(out, v.sizes(), v, "out is like v");
     row(q, "q"), row(k, "k"), row(v, "v"), row(o, "out"), row(g, "g"), row(beta, "beta");
+    apart(out, q, "q"), apart(out, k, "k"), apart(out, v, "v");
     r.sequences = u32(sequences, "sequences"), r.tokens = u32(tokens, "tokens"), r.max_tokens = u32(longest, "max_tokens");
     r.key_heads = u32(q.size(1), "key_heads"), r.heads = u32(heads, "heads");
     r.key_dim = u32(dk, "key_dim"), r.value_dim = u32(dv, "value_dim"), r.slots = u32(rows, "rows");
@@ -220,6 +230,7 @@ PyObject* q4_product(PyObject*, Args a, Py_ssize_t n) {
     const int64_t shape[2] = {tokens, rows};
     const at::Tensor y = make(out, shape, x, "out is [tokens, rows] of x's type");
     row(x, "x"), row(y, "out");
+    apart(out, x, "x");
     r.tokens = u32(tokens, "tokens"), r.rows = u32(rows, "rows"), r.cols = u32(cols, "cols");
     r.group = u32(cols / groups, "group"), r.scale_type = scales.scalar_type() == at::kHalf ? FR_HIP_F16 : FR_HIP_BF16;
     r.x = x.data_ptr(), r.codes = static_cast<const uint8_t*>(codes.data_ptr()), r.scales = scales.data_ptr();

@@ -279,8 +279,9 @@ enum { FR_HIP_BAD_OFFSET = 1, FR_HIP_BAD_SLOT = 2, FR_HIP_BAD_PAGE = 4, FR_HIP_B
  * them (offsets NULL: max_tokens each), and its state is row slot[i] of the
  * pools (slot NULL: row i); slot -1: the sequence is skipped, nothing of it is
  * read or written. Slots are distinct. state_in NULL: states begin as zeros;
- * state_out NULL: final states are dropped; both may be one pool, and without one
- * a slot that is not negative says no more than that. A sequence
+ * state_out NULL: final states are dropped; both may be one pool (but share no
+ * part of it otherwise), and without one a slot that is not negative says no more
+ * than that. A sequence
  * of no tokens passes its state on. Offsets do not go down: a sequence that
  * begins below an offset before it is bad, as is one that ends below its start.
  * key_dim 64, 128 or 256; value_dim a multiple of 16 up to 1024; key_heads
@@ -319,7 +320,7 @@ int fr_hip_delta_rule(const fr_hip_delta *req, void *workspace, size_t bytes, vo
  * cols a multiple of group, up to 65536; rows up to 2^28, and with many tokens
  * tokens * rows up to about 2^36. A token with a non-finite x gets
  * non-finite outputs (inf or NaN); fp32 values above bf16's largest (3.39e38)
- * may count as infinite. */
+ * may count as infinite. y shares no memory with an input. */
 typedef struct {
     unsigned tokens, rows, cols, group;
     unsigned type, scale_type;        /* scale_type FR_HIP_F16 or FR_HIP_BF16 */

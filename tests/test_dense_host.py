@@ -282,3 +282,14 @@ def test_delta_goes_by_the_tokens_there_are():
     for tokens, most, chunks in ((10, 4096, False), (32, 33, False), (33, 32, False), (33, 33, True), (0, 64, False)):
         r = delta_request(tokens=tokens, max_tokens=most)
         assert (fa.lib().fr_hip_delta_workspace(C.addressof(r)) > 0) == chunks, (tokens, most)
+
+
+@pytest.mark.parametrize("rows,refused", [(-3, False), (-2, False), (-1, True), (0, False), (1, True), (2, False), (3, False)])
+def test_delta_pools_are_one_or_apart(rows, refused):
+    """Two rows each, `rows` rows from one to the other."""
+    no_engine()
+    r = delta_request(state_in=P * 64, state_out=P * 64 + rows * 4 * 128 * 128 * 4)
+    assert fa.lib().fr_hip_delta_rule(C.addressof(r), None, 0, None) == (fa.INVALID if refused else fa.STATE)
+    if rows:
+        r = delta_request(state_in=P * 64, state_out=P * 64 + rows * 4 * 128 * 128 * 4 + (-16 if rows > 0 else 16))
+        assert fa.lib().fr_hip_delta_rule(C.addressof(r), None, 0, None) == (fa.INVALID if abs(rows) < 3 else fa.STATE)
