@@ -741,7 +741,7 @@ int check_query(const fr_hip_kv_query* r) {
   const int rc = check_cache(&r->cache, r->type);
   if (rc == FR_HIP_INVALID) return rc;
   if (!r->burst || !r->heads || r->heads % r->cache.heads || !isfinite(r->scale)) return FR_HIP_INVALID;
-  if (r->sequences && (!r->q || !r->o || !r->length || !r->table)) return FR_HIP_INVALID;
+  if (r->sequences && (!r->q || !r->o || !r->length || (r->max_context && !r->table))) return FR_HIP_INVALID;
   if (((uintptr_t)r->q | (uintptr_t)r->o) % elem_size(r->type)) return FR_HIP_INVALID;
   if (r->max_context > INT_MAX - (1u << 20)) return FR_HIP_INVALID;
   if (r->table_stride < (r->max_context + r->cache.page - 1) / r->cache.page) return FR_HIP_INVALID;

@@ -377,7 +377,7 @@ int fr_hip_kv_read(const fr_hip_kv_values *req, void *stream);
  *     o = sum_j softmax_j(scale q . k_j) v_j ;
  * a token that sees nothing gets zeros. Token j of sequence i lies in page
  * table[i * table_stride + j / page]. length[i] is at most max_context, which
- * bounds the launch. cache.heads divides heads, at most 64 query heads for
+ * bounds the launch (0: nothing is seen, and table may be NULL). cache.heads divides heads, at most 64 query heads for
  * each cache head. A page outside the cache counts as not seen. */
 typedef struct {
     fr_hip_kv_cache cache;

@@ -293,3 +293,11 @@ def test_delta_pools_are_one_or_apart(rows, refused):
     if rows:
         r = delta_request(state_in=P * 64, state_out=P * 64 + rows * 4 * 128 * 128 * 4 + (-16 if rows > 0 else 16))
         assert fa.lib().fr_hip_delta_rule(C.addressof(r), None, 0, None) == (fa.INVALID if abs(rows) < 3 else fa.STATE)
+
+
+def test_attention_over_nothing_needs_no_table():
+    no_engine()
+    r = query_request(max_context=0, table=None, table_stride=0)
+    assert fa.lib().fr_hip_kv_attend(C.addressof(r), None, 0, None) == fa.STATE
+    r = query_request(max_context=1, table=None)
+    assert fa.lib().fr_hip_kv_attend(C.addressof(r), None, 0, None) == fa.INVALID
