@@ -193,7 +193,9 @@ PyObject* delta_rule(PyObject*, Args a, Py_ssize_t n) {
     r.sequences = u32(sequences, "sequences"), r.tokens = u32(tokens, "tokens"), r.max_tokens = u32(longest, "max_tokens");
     r.key_heads = u32(q.size(1), "key_heads"), r.heads = u32(heads, "heads");
     r.key_dim = u32(dk, "key_dim"), r.value_dim = u32(dv, "value_dim"), r.slots = u32(rows, "rows");
-    r.flags = PyObject_IsTrue(a[11]) ? FR_HIP_DELTA_NORMALIZE : 0;
+    const int normalize = PyObject_IsTrue(a[11]);
+    if (normalize < 0) throw python_error();
+    r.flags = normalize ? FR_HIP_DELTA_NORMALIZE : 0;
     r.scale = (float)(a[7] == Py_None ? 1.0 / sqrt((double)dk) : number(a[7]));
     r.q = q.data_ptr(), r.k = k.data_ptr(), r.v = v.data_ptr(), r.o = o.data_ptr();
     r.g = static_cast<const float*>(g.data_ptr()), r.beta = static_cast<const float*>(beta.data_ptr());

@@ -122,3 +122,19 @@ with fwd.dual_level():
     else:
         raise AssertionError("a tangent")
 """)
+
+
+def test_what_has_no_truth_value_is_no_flag(folder):
+    run(folder, """
+f, args = made(0)["delta_rule"]
+args[11] = torch.ones(2)
+try:
+    f(*args)
+except RuntimeError as e:
+    assert "ambiguous" in str(e), str(e)
+else:
+    raise AssertionError("normalize of two elements")
+args[11] = torch.ones(1)
+f(*args)
+assert calls.value == 1
+""")
