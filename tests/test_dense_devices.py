@@ -126,15 +126,21 @@ with fwd.dual_level():
 
 def test_what_has_no_truth_value_is_no_flag(folder):
     run(folder, """
+class Neither:
+    def __bool__(self):
+        raise RuntimeError("ambiguous")
+
+
 f, args = made(0)["delta_rule"]
-args[11] = torch.ones(2)
+args[11] = Neither()
 try:
     f(*args)
 except RuntimeError as e:
     assert "ambiguous" in str(e), str(e)
 else:
-    raise AssertionError("normalize of two elements")
-args[11] = torch.ones(1)
+    raise AssertionError("neither true nor false")
+assert calls.value == 0
+args[11] = 1
 f(*args)
 assert calls.value == 1
 """)
