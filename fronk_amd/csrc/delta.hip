@@ -205,8 +205,10 @@ __global__ __launch_bounds__(256) void delta_step(DeltaArgs A) {
 
 // ------------------------------------------------------------ chunk by chunk
 //
-// Within a chunk of 64 tokens, with G the running sum of g and D_ij =
-// e^(G_i - G_j), the rule's updates u solve a lower triangular system:
+// The published chunk form of the delta rule (Yang et al., Parallelizing Linear
+// Transformers with the Delta Rule over Sequence Length, 2024), with its decays:
+// within a chunk of 64 tokens, with G the running sum of g and D_ij =
+// e^(G_i - G_j), the rule's updates u solve a lower triangular system
 //     A_ij = beta_i (k_i . k_j) D_ij  (j < i),   T = (I + A)^-1 diag(beta)
 //     U = T (V - e^G K S)
 //     O = scale (e^G Q S + (Q K^T . D) U),   S <- e^(G_last) S + (e^(G_last - G) K)^T U
@@ -218,8 +220,8 @@ __global__ __launch_bounds__(256) void delta_step(DeltaArgs A) {
 // the sum of parts: fp32 (T, S, U and fp32 activations) of three (8 + 8 + 8
 // bits), fp16 activations of two; products of parts down to 2^-16 of the
 // largest are taken, so that the state keeps fp32's accuracy. Outputs of 16
-// bits take two parts of S, P and U (2^-17, against their own rounding of 2^-9
-// or 2^-12). fp32 matrix instructions would do without parts at a sixteenth of
+// bits take two parts of S, P and U (2^-17, against their own rounding of 2^-8
+// or 2^-11). fp32 matrix instructions would do without parts at a sixteenth of
 // the rate.
 //
 // The order of the summed index in an operand is free. Over dims it is theirs,

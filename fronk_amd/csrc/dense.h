@@ -35,10 +35,6 @@ typedef float float4v __attribute__((ext_vector_type(4)));
 typedef uint32_t uint2v __attribute__((ext_vector_type(2)));
 typedef uint32_t uint4v __attribute__((ext_vector_type(4)));
 
-template <int TYPE> struct Elem;
-template <> struct Elem<FR_HIP_F32> { typedef float type; };
-template <> struct Elem<FR_HIP_F16> { typedef _Float16 type; };
-template <> struct Elem<FR_HIP_BF16> { typedef __bf16 type; };
 inline size_t elem_size(unsigned type) { return type == FR_HIP_F32 ? 4 : 2; }
 
 // N consecutive elements as floats; `wide`: the address is aligned to the

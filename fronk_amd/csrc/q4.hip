@@ -259,7 +259,7 @@ __global__ __launch_bounds__(512) void q4_rows(RowsArgs R) {
 // operands that all of them share through LDS.
 //
 // Both operands are fp16 here, where two codes are numbers after two packed
-// instructions: 0x6400 | c is 1024 + c, and with c four bits higher 1024 + 16 c,
+// instructions (published by Kim et al., Who Says Elephants Can't Run, 2022): 0x6400 | c is 1024 + c, and with c four bits higher 1024 + 16 c,
 // so that one packed add or fma gives c - zero exactly. fp16 activations go as
 // they are; a bf16 token is scaled by the power of two that brings its largest
 // to 2^14 .. 2^15, which keeps every value down to 2^-32 of the largest exact

@@ -13,8 +13,9 @@ under torch.no_grad() (or inference_mode), one with a forward-mode tangent alway
 
 A refused call raises ValueError before anything is enqueued. What only the
 device can see (offsets, slots, pages, lengths) is bounds-checked there: a bad
-entry reads and writes nothing and sets its bit (BAD_*) in `status`, an int32
-tensor of one element that the caller clears.
+entry reads nothing, leaves what it would write as it was (zeros in kv_read's and
+kv_attend's outputs) and sets its bit (BAD_*) in `status`, an int32 tensor of one
+element that the caller clears. Call once before capturing a graph.
 """
 import ctypes as C
 from typing import NamedTuple
@@ -91,7 +92,7 @@ def delta_rule(q, k, v, g, beta, state_in=None, state_out=None, *, scale=None, o
     unless max_tokens is given). state_in / state_out: pools [rows, heads,
     key_dim, value_dim] fp32, the same tensor to update in place; None: from
     zeros / dropped. slots (int32, sequences): the pool row of each sequence,
-    -1 to skip one; default row i."""
+    -1 to skip one; default row i. out shares no memory with an input."""
     return _dense.delta_rule(q, k, v, g, beta, state_in, state_out, scale, offsets, slots, max_tokens, normalize, out,
                              status)
 

@@ -247,8 +247,10 @@ int fr_hip_batch_output(void *stream, float *y, size_t count, unsigned *status);
  * (FR_HIP_INVALID; FR_HIP_UNSUPPORTED for sizes outside the ranges below;
  * then FR_HIP_STATE without an open engine). What only the device can see
  * (offsets, slots, pages, lengths) is bounds-checked by the kernels: a bad
- * entry reads and writes nothing and sets its bit in *status, a device word
- * that the caller clears (NULL: not reported).
+ * entry reads nothing, writes nothing but the zeros of an output that is said
+ * to have them, and sets its bit in *status, a device word that the caller
+ * clears (NULL: not reported). The engine is opened, and each entry point
+ * called once at the sizes meant, before a capture.
  *
  * stream: a hipStream_t, NULL = the library stream (which does not wait for
  * the default stream), FR_HIP_STREAM_DEFAULT = HIP's default stream. It and the
@@ -361,7 +363,7 @@ typedef struct {
 } fr_hip_kv_write;
 int fr_hip_kv_append(const fr_hip_kv_write *req, void *stream);
 /* The held values of slot[t] as k and v [tokens][heads][dim], rounded to
- * `type`; slot -1 gives zeros. k or v NULL: not read. */
+ * `type`; slot -1, or a bad one, gives zeros. k or v NULL: not read. */
 typedef struct {
     fr_hip_kv_cache cache;
     unsigned tokens, type;
@@ -375,10 +377,13 @@ int fr_hip_kv_read(const fr_hip_kv_values *req, void *stream);
  * the last of its length[i] tokens, token b sees tokens 0 .. length[i] - burst
  * + b, and per query head h (cache head h * cache.heads / heads)
  *     o = sum_j softmax_j(scale q . k_j) v_j ;
- * a token that sees nothing gets zeros. Token j of sequence i lies in page
+ * a token that sees nothing gets zeros, as do those of a bad length. Token j of sequence i lies in page
  * table[i * table_stride + j / page]. length[i] is at most max_context, which
  * bounds the launch (0: nothing is seen, and table may be NULL). cache.heads divides heads, at most 64 query heads for
- * each cache head. A page outside the cache counts as not seen. */
+ * each cache head. A page outside the cache counts as not seen.
+ * Sums are fp32 and come before the division and the keys' powers of two: where
+ * |q| dim 448, or |v| length[i], passes 3.4e38, outputs may be infinite or NaN;
+ * values of a token and head all below 1e-33 are weighed with 8 bits. */
 typedef struct {
     fr_hip_kv_cache cache;
     unsigned sequences, burst, heads, max_context, type, table_stride;
