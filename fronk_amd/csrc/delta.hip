@@ -91,7 +91,7 @@ __global__ __launch_bounds__(1024) void delta_order(const int32_t* offsets, uint
 //     p = S^T k,  w = S^T q,  o = scale (a w + (q . k) u),
 // so that a token needs one reduction over the 16 row lanes: two row rotations
 // and the two row swaps, no LDS and no barrier. Bound by reading and writing the
-// states: 64 streams of 32 heads of 128 x 128 (268 MB) in 58.8 us, 4.6 TB/s; one
+// states: 64 streams of 32 heads of 128 x 128 (268 MB) in 57.7 us, 4.7 TB/s; one
 // stream's in 4.5 us, a launch and a memory latency.
 
 // `count` tokens from `first` on of 16 columns (`tile`) of a head, s being its state.
@@ -308,7 +308,7 @@ __device__ __forceinline__ bf16x8 frag(uint4v x) { return __builtin_bit_cast(bf1
 // One workgroup: one chunk and key head, and `each` of the value heads that share
 // it; wavefront w holds tokens 16 w .. 16 w + 15 as rows. A head takes about 6 us:
 // decays and P 2.5, the inverse 2, the barriers between them the rest. 4096 tokens
-// of 32 heads: 41 us, 113 MB written; 5 sequences with 33 chunks of 9 heads: 16 us.
+// of 32 heads: 43 us, 113 MB written; 5 sequences with 33 chunks of 9 heads: 17 us.
 template <typename T, int DK>
 __global__ __launch_bounds__(256) void delta_prepare(ChunkArgs C) {
   typedef Room<T, DK> W;
@@ -521,7 +521,7 @@ __global__ __launch_bounds__(256) void delta_prepare(ChunkArgs C) {
 // and dims w * dk / 4 .. of S (in registers, fp32), and three times a chunk they
 // exchange operands through LDS: S, then V - e^G K S, then U. Wavefronts 4..7
 // form the outputs of the same tokens beside them. 64 chunks of 32 heads of 128 x
-// 128 in 98 us, 1.5 us a chunk, of which the chain's products, splits and LDS
+// 128 in 100 us, 1.6 us a chunk, of which the chain's products, splits and LDS
 // exchanges by themselves are 1.3 and memory hardly any.
 //
 // A chunk costs three barriers and the products between them, so nothing may

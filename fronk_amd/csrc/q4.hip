@@ -96,7 +96,7 @@ __device__ __forceinline__ float scale_of(uint16_t bits, bool bf16) {
 // for a block's successor as soon as it is multiplied. x is laid out as operands
 // in LDS, `segment` blocks at a time, once for the workgroup (from memory, four
 // of a block's five reads would be x's). 4096 x 65536 of one token: 35 us, 3.9 TB/s
-// (52 with x from memory); 7 fp32 tokens of 2592 x 4099: 13.3; 2560 x 2560: 4.9.
+// (52 with x from memory); 7 fp32 tokens of 2592 x 4099: 13.3; 2560 x 2560: 5.2.
 //
 // x is the A operand (tokens as rows; beyond the last it is repeated), 16 rows of
 // W the B operand, so that a lane's four results belong to its own weight row: one

@@ -2,8 +2,8 @@
 //
 // What fronk_amd.dense documents: arguments checked, the output and workspace
 // allocated, the C ABI called. It is C++ because a call of one token takes the
-// card 3 to 5 us, and the same steps in Python took the host 7 to 12 (this: 5 to
-// 6, of which the launch is 3).
+// card 3 to 5 us, and the same steps in Python took the host 7 to 12 (this: 3 to 5,
+// where torch's zero_ takes 3.6).
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <ATen/ATen.h>
