@@ -377,10 +377,11 @@ int fr_hip_kv_read(const fr_hip_kv_values *req, void *stream);
  * the last of its length[i] tokens, token b sees tokens 0 .. length[i] - burst
  * + b, and per query head h (cache head h * cache.heads / heads)
  *     o = sum_j softmax_j(scale q . k_j) v_j ;
- * a token that sees nothing gets zeros, as do those of a bad length. Token j of sequence i lies in page
- * table[i * table_stride + j / page]. length[i] is at most max_context, which
- * bounds the launch (0: nothing is seen, and table may be NULL). cache.heads divides heads, at most 64 query heads for
- * each cache head. A page outside the cache counts as not seen.
+ * a token that sees nothing gets zeros, as do those of a bad length. Token j of
+ * sequence i lies in page table[i * table_stride + j / page]. length[i] is at
+ * most max_context, which bounds the launch (0: nothing is seen, and table may be
+ * NULL). cache.heads divides heads, at most 64 query heads for each cache head. A
+ * page outside the cache counts as not seen.
  * Sums are fp32 and come before the division and the keys' powers of two: where
  * |q| dim 448, or |v| length[i], passes 3.4e38, outputs may be infinite or NaN;
  * values of a token and head all below 1e-33 are weighed with 8 bits. */

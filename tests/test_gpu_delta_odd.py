@@ -85,6 +85,17 @@ def test_slow_growth(n, dtype):
     compare(q, k, v, g, beta, torch.randn(4, 64, 32, generator=gen(203)))
 
 
+@pytest.mark.parametrize("growth", [0.02, 0.1, 0.3])
+@pytest.mark.parametrize("n", [30, 64, 100])
+def test_growth_that_each_token_takes_back(n, growth):
+    """One key for all tokens and beta 1: what has grown is replaced by the next
+    value. (Rounding errors beside the key are not, and grow.)"""
+    q, k, v, g, beta = delta_inputs(220, [n], 1, 1, 64, 16, F32)
+    k[:] = k[0]
+    g[:], beta[:] = growth, 1.0
+    compare(q, k, v, g, beta, torch.zeros(1, 64, 16))
+
+
 @pytest.mark.parametrize("first", [0, 70])
 def test_small_states_that_grow_past_a_chunks_factors(first):
     """Values near 1e-25 that grow by e^120 within thirty tokens and shrink again."""
