@@ -95,6 +95,13 @@ SIGNATURES = {
     "fr_hip_kv_read": (C.c_int, [C.c_void_p, C.c_void_p]),
     "fr_hip_kv_workspace": (C.c_size_t, [C.c_void_p]),
     "fr_hip_kv_attend": (C.c_int, [C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]),
+    "fr_hip_rotate": (C.c_int, [C.c_void_p, C.c_void_p]),
+    "fr_hip_prompt_workspace": (C.c_size_t, [C.c_void_p]),
+    "fr_hip_prompt_attend": (C.c_int, [C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]),
+    "fr_hip_tree_workspace": (C.c_size_t, [C.c_void_p]),
+    "fr_hip_kv_attend_tree": (C.c_int, [C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]),
+    "fr_hip_kv_move": (C.c_int, [C.c_void_p, C.c_void_p]),
+    "fr_hip_kv_copy": (C.c_int, [C.c_void_p, C.c_void_p]),
 }
 
 _lib = None

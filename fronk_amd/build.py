@@ -1,8 +1,8 @@
 """Build the MI355X libraries in-tree (no JIT cache, no site-packages).
 
 libfronk_hip.so      HIP kernels + C ABI (include/fronk_hip.h), gfx950 only.
-_dense.so            fronk_amd.dense's side of it over torch tensors
-                     (host/dense_module.cpp).
+_dense.so, _attention.so   fronk_amd.dense's side of it over torch tensors
+                     (host/dense_module.cpp, host/attention_module.cpp).
 libfr_hip.so         the "hip" fr_backend vtable (host/hip.c, plain C11),
                      compiled against the reference's own src/ headers where
                      they lie (hidden size fixed there at 2560) and linked
@@ -18,12 +18,13 @@ from concurrent.futures import ThreadPoolExecutor
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
 # The expert engine (fronk_hip.hip within engine.hip), and the dense operators around it.
-HIP_SRCS = [os.path.join(HERE, "csrc", n) for n in ("engine.hip", "delta.hip", "q4.hip", "kv.hip")]
+HIP_SRCS = [os.path.join(HERE, "csrc", n) for n in ("engine.hip", "delta.hip", "q4.hip", "kv.hip", "rotary.hip", "prompt.hip", "tree.hip", "pages.hip")]
 HIP_LIB = os.path.join(HERE, "libfronk_hip.so")
 VTABLE_SRC = os.path.join(HERE, "host", "hip.c")
 VTABLE_LIB = os.path.join(HERE, "libfr_hip.so")
-DENSE_SRC = os.path.join(HERE, "host", "dense_module.cpp")
-DENSE_LIB = os.path.join(HERE, "_dense.so")
+# (source, library) of the dense operators' torch side.
+DENSE_MODULES = [(os.path.join(HERE, "host", n + "_module.cpp"), os.path.join(HERE, "_" + n + ".so"))
+                 for n in ("dense", "attention")]
 REFERENCE_SRC = os.path.join(os.environ.get("FRONK_REFERENCE", "/root/reference"), "src")
 
 # Packed-FP32 instructions are disabled for every HIP translation unit.
@@ -63,13 +64,17 @@ def build_dense(verbose=False):
     at = os.path.dirname(torch.__file__)
     include = [os.path.join(ROOT, "include"), os.path.join(at, "include"),
                os.path.join(at, "include", "torch", "csrc", "api", "include"), sysconfig.get_paths()["include"]]
-    cmd = ["g++", "-std=c++17", "-O2", "-fPIC", "-shared", *("-I" + i for i in include),
-           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", DENSE_SRC, "-o", DENSE_LIB + ".tmp",
-           "-L" + HERE, "-lfronk_hip", "-Wl,-rpath,$ORIGIN", "-L" + os.path.join(at, "lib"), "-ltorch_python",
-           "-ltorch_cpu", "-lc10"]
-    subprocess.run(cmd, check=True, capture_output=not verbose)
-    os.replace(DENSE_LIB + ".tmp", DENSE_LIB)
-    return DENSE_LIB
+    def compile_one(module):
+        src, lib = module
+        cmd = ["g++", "-std=c++17", "-O2", "-fPIC", "-shared", *("-I" + i for i in include),
+               f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", src, "-o", lib + ".tmp",
+               "-L" + HERE, "-lfronk_hip", "-Wl,-rpath,$ORIGIN", "-L" + os.path.join(at, "lib"), "-ltorch_python",
+               "-ltorch_cpu", "-lc10"]
+        subprocess.run(cmd, check=True, capture_output=not verbose)
+        os.replace(lib + ".tmp", lib)
+        return lib
+    with ThreadPoolExecutor(len(DENSE_MODULES)) as pool:
+        return list(pool.map(compile_one, DENSE_MODULES))
 
 
 def build_all(verbose=False):

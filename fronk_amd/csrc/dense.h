@@ -24,6 +24,7 @@ __attribute__((visibility("hidden"))) int enter(void* stream, hipStream_t* out);
 namespace {
 
 constexpr uint32_t kUnits = 256;   // an MI355X's compute units, of four SIMDs each
+constexpr float kLog2e = 1.4426950408889634f;
 
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));

@@ -398,6 +398,102 @@ typedef struct {
 size_t fr_hip_kv_workspace(const fr_hip_kv_query *req);   /* as fr_hip_delta_workspace */
 int fr_hip_kv_attend(const fr_hip_kv_query *req, void *workspace, size_t bytes, void *stream);
 
+/* Rotary positions of q and k. With pair i's angle a = position * frequencies[i]
+ * (radians, formed in 64 bits) and m = magnitude, its two values become
+ *     m (x cos a - y sin a),  m (x sin a + y cos a) ;
+ * pair i is values i and i + pairs of a head, or 2i and 2i + 1 with
+ * FR_HIP_ROTARY_INTERLEAVED. Values from 2 * pairs on stay as they are. q_out
+ * (k_out) is q (k) itself, with its strides, or shares no memory with an input.
+ * dim up to 1024, pairs up to dim / 2; heads or kv_heads 0: that one is not there. */
+enum { FR_HIP_ROTARY_INTERLEAVED = 1 };
+typedef struct {
+    unsigned tokens, heads, kv_heads, dim, pairs, type, flags;
+    float magnitude;
+    const void *q, *k;                /* [tokens][heads][dim], [tokens][kv_heads][dim] */
+    void *q_out, *k_out;
+    int64_t q_token, q_head, k_token, k_head, qo_token, qo_head, ko_token, ko_head;
+    const int32_t *positions;         /* [tokens] */
+    const double *frequencies;        /* [pairs] */
+} fr_hip_rotary;
+int fr_hip_rotate(const fr_hip_rotary *req, void *stream);
+
+/* Causal attention of packed prompts over their keys, per query head h (key head h *
+ * kv_heads / heads)
+ *     o = sum_j softmax_j(scale q . k_j) v_j .
+ * Sequence i is queries offsets[i] .. offsets[i+1]-1, at most max_tokens, and keys
+ * k_offsets[i] .. k_offsets[i+1]-1, at most max_context; its queries are the last of its
+ * keys: query t of n, of m keys, sees keys 0 .. m - n + t. One that sees nothing has
+ * zeros. offsets NULL: max_tokens queries each; k_offsets NULL: the keys are the queries'
+ * own (without offsets, max_context of them each). Offsets do not go down: a sequence that
+ * begins below an offset before it is bad, as is one that ends below its start, is too long or
+ * out of range, and a bad one's outputs are left as they were. max_tokens and max_context
+ * bound the launch. kv_heads divides heads, at most 64 query heads for each; dim 64, 128
+ * or 256. o shares no memory with an input.
+ * A value (v) that is not finite makes its dim not finite (NaN or infinity) in the queries that
+ * see it, and in no others; a key that is not finite may make all of theirs NaN.
+ * Weights are rounded to `type`, their sums are not. */
+typedef struct {
+    unsigned sequences, tokens, k_tokens, max_tokens, max_context;
+    unsigned heads, kv_heads, dim, type;
+    float scale;
+    const void *q;                    /* [tokens][heads][dim] */
+    const void *k, *v;                /* [k_tokens][kv_heads][dim] */
+    void *o;                          /* [tokens][heads][dim] */
+    int64_t q_token, q_head, k_token, k_head, v_token, v_head, o_token, o_head;
+    const int32_t *offsets, *k_offsets;   /* [sequences + 1] */
+    uint32_t *status;
+} fr_hip_prompt;
+/* As fr_hip_delta_workspace; needed where a few rows have many keys (max_context). */
+size_t fr_hip_prompt_workspace(const fr_hip_prompt *req);
+int fr_hip_prompt_attend(const fr_hip_prompt *req, void *workspace, size_t bytes, void *stream);
+
+/* Attention of trees of drafted tokens over the cache. Sequence i's drafts are rows
+ * offsets[i] .. offsets[i+1]-1 of q (offsets NULL: max_tokens each), n of them, at most
+ * max_tokens (up to 64), and the last n of its length[i] tokens in the cache. Draft b
+ * sees the tokens before the drafts, and draft j where bit j of its tree word is set
+ * (its own bit among them, if it sees itself; bits from n on say nothing). One that sees
+ * nothing has zeros, as do those of a bad length (below n, or above max_context); a bad
+ * sequence's (as for fr_hip_prompt_attend) are left as they were. Otherwise as
+ * fr_hip_kv_attend: softmax(scale q k) v per query head, pages by table, a page
+ * outside the cache counts as not seen. o shares no memory with an input.
+ * What is held of drafts that no draft sees may be anything. A draft held with infinity or
+ * NaN makes the drafts that see it NaN, and no others. bf16 outputs: weights are rounded to
+ * bf16, their sums are not. */
+typedef struct {
+    fr_hip_kv_cache cache;
+    unsigned sequences, tokens, max_tokens, heads, max_context, type, table_stride;
+    float scale;
+    const void *q;                    /* [tokens][heads][dim] */
+    void *o;
+    int64_t q_token, q_head, o_token, o_head;
+    const int64_t *tree;              /* [tokens] */
+    const int32_t *offsets, *table, *length;
+    uint32_t *status;
+} fr_hip_kv_tree;
+size_t fr_hip_tree_workspace(const fr_hip_kv_tree *req);   /* as fr_hip_delta_workspace */
+int fr_hip_kv_attend_tree(const fr_hip_kv_tree *req, void *workspace, size_t bytes, void *stream);
+
+/* What slot source[g * moves + i] holds is written to slot target[g * moves + i], bit
+ * for bit, each group's as if all of it were read before any is written (accepted drafts
+ * moved together). -1 in either: that one is skipped. Targets are distinct, and no
+ * group's target is another's source. moves up to 64. */
+typedef struct {
+    fr_hip_kv_cache cache;
+    unsigned groups, moves;
+    const int32_t *source, *target;   /* [groups][moves] */
+    uint32_t *status;
+} fr_hip_kv_moves;
+int fr_hip_kv_move(const fr_hip_kv_moves *req, void *stream);
+/* Pages source[i] copied to pages target[i]; -1 in either: skipped. Targets are
+ * distinct, and none is the source of another. */
+typedef struct {
+    fr_hip_kv_cache cache;
+    unsigned count;
+    const int32_t *source, *target;
+    uint32_t *status;
+} fr_hip_kv_copies;
+int fr_hip_kv_copy(const fr_hip_kv_copies *req, void *stream);
+
 /* Launch timing for measurement (no reference counterpart): after
  * fr_hip_timing(n), the next n launches record HIP events on their stream
  * before the main kernel, after it and after the launch's last kernel (a
