@@ -39,19 +39,33 @@ __device__ __forceinline__ float16v mma32(float4v a, float4v b, float16v c) {
   return c;
 }
 
+// What all lanes have alike, so that the compiler keeps it, and addresses made of it, once.
+__device__ __forceinline__ int32_t same(int32_t x) { return __builtin_amdgcn_readfirstlane(x); }
+
 typedef __attribute__((address_space(3))) char lds_char;
 
 // 64 lanes' 16 bytes to consecutive places of LDS from `at` on. Of the counter of
 // loads in flight that this raises the compiler knows nothing: whoever reads the
 // places waits for it, and then for the other wavefronts.
 __device__ __forceinline__ void to_lds(const char* base, uint32_t offset, uint32_t at) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(at), "v"(offset), "s"(base) : "memory");
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(at), "v"(offset), "s"(base) : "memory", "m0");
 }
-__device__ __forceinline__ void loads_done() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+// The largest of a lane's scores (NaN is none), in four chains.
+template <int N> __device__ __forceinline__ float largest(const float16v (&st)[N]) {
+  float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+  for (int t = 0; t < N; ++t)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) m[r % 4] = fmaxf(m[r % 4], st[t][r]);
+  return fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
+}
+// Waits for this wavefront's loads but the last N, and then for all wavefronts'.
+template <int N> __device__ __forceinline__ void loads_done() {
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
+}
 
-// N operands of READS reads each, one matrix instruction each: a few ahead.
-template <int N, int READS> __device__ __forceinline__ void schedule() {
-  constexpr int kAhead = 4;
+// N operands of READS reads each, one matrix instruction each: kAhead ahead.
+template <int N, int READS, int kAhead> __device__ __forceinline__ void schedule() {
   __builtin_amdgcn_sched_group_barrier(0x100, kAhead * READS, 0);
 #pragma unroll
   for (int n = 0; n < N; ++n) {
@@ -76,21 +90,58 @@ template <typename T> __device__ __forceinline__ void put4(T* p, float4v x, floa
   }
 }
 
-// Four dims of a row from its stretches, in their order: `part` its place in the first.
+// Four dims of a row from its stretches, joined in their order; `part` is the row's
+// place in the first, of `block_rows`. Few stretches: D / 4 lanes a row.
 template <int D>
-__device__ __forceinline__ float4v join(const float* part_o, const float* part_ml, size_t part, uint32_t splits, uint32_t d, float* sum) {
+__device__ __forceinline__ float4v join_few(const float* part_o, const float* part_ml, size_t part, uint32_t splits, uint32_t block_rows, float* sum) {
+  const uint32_t d = threadIdx.x % (D / 4) * 4;
   float top = -INFINITY, total = 0;
-  for (uint32_t s = 0; s < splits; ++s) top = fmaxf(top, part_ml[(part + (size_t)s * R) * 2]);
+  for (uint32_t s = 0; s < splits; ++s) top = fmaxf(top, part_ml[(part + (size_t)s * block_rows) * 2]);
   float4v x = {0, 0, 0, 0};
-  for (uint32_t s = 0; s < splits; ++s, part += R) {
-    const float shift = part_ml[part * 2];
-    if (shift == -INFINITY) continue;   // nothing seen there, and no sums written
-    const float w = __builtin_amdgcn_exp2f(shift - top);
-    total += w * part_ml[part * 2 + 1];
-    x += w * *reinterpret_cast<const float4v*>(part_o + part * D + d);
+#pragma unroll 4
+  for (uint32_t s = 0; s < splits; ++s) {
+    const size_t at = part + (size_t)s * block_rows;
+    const float shift = part_ml[at * 2], l = part_ml[at * 2 + 1], w = __builtin_amdgcn_exp2f(shift - top);
+    const float4v y = *reinterpret_cast<const float4v*>(part_o + at * D + d);
+    if (shift != -INFINITY) total += w * l, x += w * y;   // (else nothing is seen there, and y was not written)
   }
   *sum = total;
   return x;
 }
+// Up to 256 of them: a workgroup of 256 a row; the first D / 4 threads have the result.
+template <int D>
+__device__ __forceinline__ float4v join_many(const float* part_o, const float* part_ml, size_t part, uint32_t splits, uint32_t block_rows, float* sum) {
+  constexpr uint32_t L = D / 4, G = 256 / L;
+  __shared__ float weight[256], red[2][4];
+  __shared__ float4v parts[G][L];
+  const uint32_t s = threadIdx.x, c = s % L, g = s / L;
+  const float m = s < splits ? part_ml[(part + (size_t)s * block_rows) * 2] : -INFINITY;
+  const float l = s < splits ? part_ml[(part + (size_t)s * block_rows) * 2 + 1] : 0.f;
+  float top = m;
+  for (int o = 1; o < 64; o *= 2) top = fmaxf(top, __shfl_xor(top, o));
+  if ((s & 63) == 0) red[0][s >> 6] = top;
+  __syncthreads();
+  top = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
+  const bool seen = m != -INFINITY;
+  const float w = seen ? __builtin_amdgcn_exp2f(m - top) : -1.f;
+  weight[s] = w;
+  float total = seen ? w * l : 0.f;
+  for (int o = 1; o < 64; o *= 2) total += __shfl_xor(total, o);
+  if ((s & 63) == 0) red[1][s >> 6] = total;
+  __syncthreads();
+  *sum = (red[1][0] + red[1][1]) + (red[1][2] + red[1][3]);
+  float4v x = {0, 0, 0, 0};
+#pragma unroll 8
+  for (uint32_t k = g; k < splits; k += G) {
+    const float f = weight[k];
+    const float4v y = *reinterpret_cast<const float4v*>(part_o + (part + (size_t)k * block_rows) * D + c * 4);
+    if (!(f < 0.f)) x += f * y;   // (else nothing is seen there, and y was not written)
+  }
+  parts[g][c] = x;
+  __syncthreads();
+  for (uint32_t k = 1; k < G; ++k) x += parts[k][c];   // (by all, for the first group)
+  return x;
+}
+constexpr uint32_t kFewSplits = 4;
 
 }  // namespace

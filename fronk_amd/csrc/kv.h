@@ -36,6 +36,13 @@ __device__ __forceinline__ half8v codes8(uint32_t lo, uint32_t hi, half8v) {
   return {a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
+// ... and times a power of two.
+__device__ __forceinline__ bf16x8 codes8(uint32_t lo, uint32_t hi, float power, bf16x8) {
+  const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, power, false), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, power, true);
+  const bf16x2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, power, false), d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, power, true);
+  return {a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+
 // x as `N` bf16 parts whose sum it is (up to 2^-8N of it).
 template <int N> __device__ __forceinline__ void split8(const float (&x)[8], bf16x8 (&out)[N]) {
   float rest[8];

@@ -2,6 +2,8 @@
 #include <limits.h>
 #include <math.h>
 
+#include <type_traits>
+
 #include "attend.h"
 #include "bounds.h"
 #include "dense.h"
@@ -28,11 +30,11 @@ struct Prompt {
 __device__ __forceinline__ Prompt prompt_of(const PromptArgs& A, uint32_t seq) {
   int32_t q0 = seq * A.max_tokens, q1 = q0 + A.max_tokens, k0 = seq * A.max_context, k1 = k0 + A.max_context, before = 0;
   if (A.offsets) {
-    q0 = A.offsets[seq], q1 = A.offsets[seq + 1];
+    q0 = same(A.offsets[seq]), q1 = same(A.offsets[seq + 1]);
     for (uint32_t s = threadIdx.x; s < seq; s += blockDim.x) before = max(before, A.offsets[s]);
     if (!A.k_offsets) k0 = q0, k1 = q1;
   }
-  if (A.k_offsets) k0 = A.k_offsets[seq], k1 = A.k_offsets[seq + 1];
+  if (A.k_offsets) k0 = same(A.k_offsets[seq]), k1 = same(A.k_offsets[seq + 1]);
   const uint32_t bad = fronk::bad_sequence(0, 1, q0, q1, A.tokens, A.max_tokens) |
                        fronk::bad_sequence(0, 1, k0, k1, A.k_tokens, A.max_context);
   return Prompt{q0, k0, (uint32_t)(q1 - q0), (uint32_t)(k1 - k0), __syncthreads_or(before > q0 || bad) != 0};
@@ -139,7 +141,7 @@ __global__ __launch_bounds__(64 * kWaves, (kResident<T, D>)) void prompt_attend(
     k_off[l] = lane_row * (uint32_t)k_row + (lane_chunk ^ (r & 7)) * 16;
     v_off[l] = lane_row * (uint32_t)v_row + (lane_chunk ^ 2 * (r & 3)) * 16;
   }
-  auto load = [&](uint32_t base, uint32_t buffer) {
+  auto load = [&](uint32_t base, uint32_t buffer) __attribute__((always_inline)) {
     char* const to = lds + buffer * 2 * kTile;
     if constexpr (WIDE) {
       const uint32_t at = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_char*)to + wave * 1024);
@@ -196,8 +198,10 @@ __global__ __launch_bounds__(64 * kWaves, (kResident<T, D>)) void prompt_attend(
   // A tile: scores, weights, outputs. `masked`: rows see different parts of it. (One
   // body with a branch over the mask alone: as two, the accumulators took twice the
   // registers.)
-  auto compute = [&](uint32_t base, uint32_t buffer, bool masked) {
+  auto compute = [&](uint32_t base, uint32_t buffer, bool masked) __attribute__((always_inline)) {
     const char* const tile = lds + buffer * 2 * kTile;
+    // (The matrix cores' work goes before another wavefront's vector work.)
+    __builtin_amdgcn_s_setprio(1);
     float16v st[ST];
 #pragma unroll
     for (int t = 0; t < ST; ++t) {
@@ -206,7 +210,7 @@ __global__ __launch_bounds__(64 * kWaves, (kResident<T, D>)) void prompt_attend(
       for (int s = 0; s < KS; ++s)
         st[t] = mma32(*reinterpret_cast<const frag*>(tile + k_at[s % 4] + t * 32 * kRow + s / 4 * 128), qf[s], st[t]);
     }
-    schedule<ST * KS, 1>();
+    schedule<ST * KS, 1, 2>();
     if (masked) {
 #pragma unroll
       for (int t = 0; t < ST; ++t)
@@ -214,12 +218,7 @@ __global__ __launch_bounds__(64 * kWaves, (kResident<T, D>)) void prompt_attend(
         for (int r = 0; r < 16; ++r)
           if ((int32_t)(base + t * 32 + 8 * (r / 4) + 4 * h + r % 4) >= limit) st[t][r] = -INFINITY;
     }
-    float most = -INFINITY;
-#pragma unroll
-    for (int t = 0; t < ST; ++t)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) most = fmaxf(most, st[t][r]);
-    most = max_xor32(most);
+    const float most = max_xor32(largest(st));
     // The maximum that weights are taken from moves only where one would pass 2^8:
     // sums and outputs are scaled seldom.
     if (__any(most * scale > top * scale + 8.f)) {
@@ -229,18 +228,20 @@ __global__ __launch_bounds__(64 * kWaves, (kResident<T, D>)) void prompt_attend(
 #pragma unroll
       for (int d = 0; d < DT; ++d) acc[d] *= f;
     }
+    __builtin_amdgcn_s_setprio(0);
     __builtin_amdgcn_sched_barrier(0);
     frag pf[ST][PS];
-    float total = 0;
+    float total[4] = {};
 #pragma unroll
     for (int t = 0; t < ST; ++t)
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(st[t][r], scale, -shift));
-        total += p;
+        total[r % 4] += p;
         pf[t][r / kEach][r % kEach] = (T)p;
       }
-    sum += total;
+    sum += (total[0] + total[1]) + (total[2] + total[3]);
+    __builtin_amdgcn_s_setprio(1);
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int t = 0; t < ST; ++t)
@@ -262,29 +263,31 @@ __global__ __launch_bounds__(64 * kWaves, (kResident<T, D>)) void prompt_attend(
           }
           acc[d] = mma32(a, pf[t][s], acc[d]);
         }
-    schedule<ST * PS * DT, sizeof(T) == 2 ? 2 : 4>();
+    schedule<ST * PS * DT, sizeof(T) == 2 ? 2 : 4, 3>();
   };
 
   // A value that is not finite times a weight of zero is NaN, also in rows that do
   // not see its key. So where outputs are not finite, all is done again with such values
   // as zeros, the first key that has one noted for each dim, and NaN for those
   // outputs whose row sees it.
-  bool again = false;
-  for (;; again = true) {
+  // (as code of its own: in one loop, what the second time needs was spilled)
+  auto pass = [&](auto second) __attribute__((always_inline)) {
+    constexpr bool kSecond = decltype(second)::value;
     top = -INFINITY, shift = 0, sum = 0;
 #pragma unroll
     for (int d = 0; d < DT; ++d) acc[d] = float16v{};
-    if (again) {
+    if constexpr (kSecond)
       for (uint32_t d = threadIdx.x; d < D; d += 64 * kWaves) first_bad[d] = INT_MAX;
-    }
     if (begin < end) load(begin, 0);
     uint32_t buffer = 0;
+#pragma unroll 1
     for (uint32_t base = begin; base < end; base += KT) {
-      if constexpr (WIDE) loads_done();
-      __syncthreads();
+      if constexpr (WIDE) loads_done<0>();
+      else __syncthreads();
       if (base + KT < end) load(base + KT, buffer ^ 1);
-      if (again) {
+      if constexpr (kSecond) {
         char* const v = lds + buffer * 2 * kTile + kTile;
+#pragma unroll 1
         for (uint32_t e = threadIdx.x; e < KT * D; e += 64 * kWaves) {
           const uint32_t r = e / D, d = e % D;
           T* x = reinterpret_cast<T*>(v + r * kRow + ((d / kEach) ^ 2 * (r & 3)) * 16) + d % kEach;
@@ -299,15 +302,15 @@ __global__ __launch_bounds__(64 * kWaves, (kResident<T, D>)) void prompt_attend(
       if ((int32_t)base < any_see) compute(base, buffer, (int32_t)base + KT > all_see);
       buffer ^= 1;
     }
-    if (again) break;
-    float finite = 0;
+  };
+  pass(std::false_type{});
+  float finite = 0;
 #pragma unroll
-    for (int d = 0; d < DT; ++d)
+  for (int d = 0; d < DT; ++d)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) finite = __builtin_fmaf(acc[d][r], 0.f, finite);
-    if (!__syncthreads_or(finite != 0.f)) break;
-  }
-  if (again) {
+    for (int r = 0; r < 16; ++r) finite = __builtin_fmaf(acc[d][r], 0.f, finite);
+  if (__syncthreads_or(finite != 0.f)) {
+    pass(std::true_type{});
 #pragma unroll
     for (int d = 0; d < DT; ++d)
 #pragma unroll
@@ -315,6 +318,7 @@ __global__ __launch_bounds__(64 * kWaves, (kResident<T, D>)) void prompt_attend(
         if (first_bad[d * 32 + r / 4 * 8 + 4 * h + r % 4] < limit) acc[d][r] = NAN;
   }
 
+  __builtin_amdgcn_s_setprio(0);
   sum = add_xor32(sum);
   if (row >= rows) return;
   if (A.splits > 1) {
@@ -338,18 +342,19 @@ __global__ __launch_bounds__(64 * kWaves, (kResident<T, D>)) void prompt_attend(
       put4<T>(p + d * 32 + g * 8, float4v{acc[d][g * 4], acc[d][g * 4 + 1], acc[d][g * 4 + 2], acc[d][g * 4 + 3]}, sum, WIDE);
 }
 
-// The stretches of a row joined, in their order: D / 4 lanes a row.
-template <typename T, int D, bool WIDE>
+// The stretches of rows joined: one row a workgroup, or as many as have D / 4 lanes.
+template <typename T, int D, bool WIDE, bool MANY>
 __global__ __launch_bounds__(256) void prompt_merge(PromptArgs A) {
-  constexpr uint32_t L = D / 4, kAtOnce = 256 / L;
-  const uint32_t item = blockIdx.x / (R / kAtOnce), r = blockIdx.x % (R / kAtOnce) * kAtOnce + threadIdx.x / L;
+  constexpr uint32_t L = D / 4, kAtOnce = MANY ? 1 : 256 / L;
+  const uint32_t item = blockIdx.x / (R / kAtOnce), r = blockIdx.x % (R / kAtOnce) * kAtOnce + (MANY ? 0 : threadIdx.x / L);
   const uint32_t head = item % A.kv_heads, seq = item / A.kv_heads % A.sequences, block = item / A.kv_heads / A.sequences;
   const Prompt P = prompt_of(A, seq);
-  const uint32_t row = block * R + r, d = threadIdx.x % L * 4;
+  const uint32_t row = block * R + r;
   if (P.bad || row >= P.n * A.per) return;
   float sum;
-  const float4v x = join<D>(A.part_o, A.part_ml, ((size_t)item * A.splits) * R + r, A.splits, d, &sum);
-  put4<T>(output_row<T>(A, P, head, row) + d, x, sum, WIDE);
+  const size_t part = (size_t)item * A.splits * R + r;
+  const float4v x = MANY ? join_many<D>(A.part_o, A.part_ml, part, A.splits, R, &sum) : join_few<D>(A.part_o, A.part_ml, part, A.splits, R, &sum);
+  if (!MANY || threadIdx.x < L) put4<T>(output_row<T>(A, P, head, row) + threadIdx.x % L * 4, x, sum, WIDE);
 }
 
 // ---------------------------------------------------------------------- host
@@ -394,7 +399,7 @@ PromptCut prompt_cut(const fr_hip_prompt* r) {
 }
 // Grids of less than 2^32 threads.
 bool prompt_fits(const fr_hip_prompt* r, const PromptCut& c) {
-  return c.items * c.splits * 64 * kWaves <= UINT32_MAX && (c.splits == 1 || c.items * R * (r->dim / 4) <= UINT32_MAX);
+  return c.items * c.splits * 64 * kWaves <= UINT32_MAX && (c.splits == 1 || c.items * R * 256 <= UINT32_MAX);
 }
 
 bool prompt_wide(const fr_hip_prompt* r) {
@@ -414,8 +419,10 @@ int launch_prompt(const PromptArgs& A, const PromptCut& c, hipStream_t s) {
   static fronk::Devices done;
   if (allow_lds(prompt_attend<T, D, WIDE>, kLds, &done)) return FR_HIP_IO;
   hipLaunchKernelGGL((prompt_attend<T, D, WIDE>), dim3((uint32_t)(c.items * c.splits)), dim3(64 * kWaves), kLds, s, A);
-  if (c.splits > 1)
-    hipLaunchKernelGGL((prompt_merge<T, D, WIDE>), dim3((uint32_t)(c.items * R / (1024 / D))), dim3(256), 0, s, A);
+  if (c.splits > kFewSplits)
+    hipLaunchKernelGGL((prompt_merge<T, D, WIDE, true>), dim3((uint32_t)(c.items * R)), dim3(256), 0, s, A);
+  else if (c.splits > 1)
+    hipLaunchKernelGGL((prompt_merge<T, D, WIDE, false>), dim3((uint32_t)(c.items * R / (1024 / D))), dim3(256), 0, s, A);
   FRONK_CK(hipGetLastError());
   return FR_HIP_OK;
 }

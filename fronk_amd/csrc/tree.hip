@@ -12,7 +12,7 @@ struct TreeArgs {
   Cache cache;
   const void* q;
   void* o;
-  float *part_o, *part_ml;       // [item][split][R][D], [item][split][R][2]
+  float *part_o, *part_ml;       // [item][split][block's row][D], [item][split][block's row][2]
   const int64_t* tree;
   const int32_t *offsets, *table, *length;
   uint32_t* status;
@@ -32,10 +32,10 @@ struct Drafts {
 __device__ __forceinline__ Drafts drafts_of(const TreeArgs& A, uint32_t seq) {
   int32_t q0 = seq * A.max_tokens, q1 = q0 + A.max_tokens, before = 0;
   if (A.offsets) {
-    q0 = A.offsets[seq], q1 = A.offsets[seq + 1];
+    q0 = same(A.offsets[seq]), q1 = same(A.offsets[seq + 1]);
     for (uint32_t s = threadIdx.x; s < seq; s += blockDim.x) before = max(before, A.offsets[s]);
   }
-  Drafts d = {q0, (uint32_t)(q1 - q0), (uint32_t)A.length[seq], 0};
+  Drafts d = {q0, (uint32_t)(q1 - q0), (uint32_t)same(A.length[seq]), 0};
   if (__syncthreads_or(before > q0) || fronk::bad_sequence(0, 1, q0, q1, A.tokens, A.max_tokens)) d.bad = FR_HIP_BAD_OFFSET;
   else if ((int32_t)d.length < (int32_t)d.n || d.length > A.max_context) d.bad = FR_HIP_BAD_LENGTH, d.length = 0;
   return d;
@@ -44,240 +44,350 @@ template <typename T> __device__ __forceinline__ T* draft_row(const TreeArgs& A,
   return static_cast<T*>(A.o) + (int64_t)(S.q0 + row / A.per) * A.o_token + (int64_t)(head * A.per + row % A.per) * A.o_head;
 }
 
-// One workgroup: one sequence, one cache head, R of its rows (query heads of that
-// cache head by drafts, draft-major) and one stretch of the context. Products and
-// fragments are those of prompt_attend (attend.h); codes become 16-bit operands on
-// their way to LDS, once for the four wavefronts' 128 rows. Codes times one are exact
-// in bf16 and fp16, a token's powers of two go to its scores and weights.
+// One workgroup: one sequence, one cache head, 32 RG of its rows (query heads of that
+// cache head by drafts, draft-major) and one stretch of the context. Its four
+// wavefronts are RG groups of 32 rows by 4 / RG groups of keys; each takes every
+// (4 / RG)-th tile of KT keys. Products and fragments are those of prompt_attend
+// (attend.h), but that codes become operands as they are read from LDS: there they are
+// as the cache has them, S stages of 4 / RG tiles, loaded that far ahead, as a tile's
+// work (0.5 us) is less than a memory's latency. Codes times one are exact in bf16 and
+// fp16; a token's powers of two go to its scores and weights.
 //
-// K in LDS: [token][dim], chunk c of 16 bytes at c ^ (token & 7). V: [block of 16
-// tokens][dim][16 tokens], in the order 0-3, 8-11, 4-7, 12-15 in which a half's lanes
-// hold weights.
+// K in LDS: [token][dim], chunk c of 16 codes at another place for each of eight
+// tokens, so that a read of one chunk of 32 of them goes to all banks; a lane's 16
+// codes are operands of two steps (Q is laid out alike). V: [block of 16 tokens][dim]
+// [16 tokens], a half's lanes hold weights of tokens 0-3 and 8-11, or 4-7 and 12-15.
 //
 // Q is an exact operand (fp32: three bf16 parts); P 2^e is in bf16 parts, of which there
 // are as many as keep it well below the output's own rounding but for bf16, where
 // half a step of independent weights is no more than that.
 template <typename T> struct Row;
-template <> struct Row<__bf16> {
+template <> struct Row<__bf16> {   // (kFold: K's powers of two go into its operand)
+  static constexpr bool kFold = true;
   typedef bf16x8 frag;
   static constexpr int kQ = 1, kP = 1;
 };
 template <> struct Row<_Float16> {
+  static constexpr bool kFold = false;
   typedef half8v frag;
   static constexpr int kQ = 1, kP = 2;
 };
 template <> struct Row<float> {
+  static constexpr bool kFold = true;
   typedef bf16x8 frag;
   static constexpr int kQ = 3, kP = 3;
 };
 
-// Four codes, those that are no number (which nothing writes) as zeros.
-__device__ __forceinline__ uint32_t numbers(uint32_t codes) {
-  const uint32_t nan = (((codes & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7;
-  return codes & ~(nan * 255u);
+// Wavefronts, keys of a tile, stages, wavefronts a SIMD that the registers are for.
+// Where Q's three parts do not fit them beside the sums, Q is kept in LDS, and split
+// where it is used.
+template <typename T, int D> constexpr bool kTreeQInLds = D * sizeof(T) > 512;
+template <typename T, int D, int RG> constexpr int kTreeWaves = kTreeQInLds<T, D> ? 2 : D == 256 && RG > 1 ? 8 : 4;
+template <int D, int RG> constexpr int kTreeKeys = D == 256 || (D == 128 && RG == 1) ? 32 : 64;
+constexpr int kTreeStages = 2;
+template <typename T, int D> constexpr int kTreeResident = sizeof(T) == 2 && D == 64 ? 3 : 2;
+// LDS: the stages, and Q; at the end the key groups are joined in it.
+template <typename T, int D, int RG> constexpr size_t kTreeTiles =
+    (size_t)kTreeStages * (kTreeWaves<T, D, RG> / RG) * 2 * kTreeKeys<D, RG> * D;
+template <typename T, int D, int RG> constexpr size_t kTreeUsed = kTreeTiles<T, D, RG> + (kTreeQInLds<T, D> ? 128 * RG * D : 0);
+template <typename T, int D, int RG> constexpr size_t kTreeJoin = RG == kTreeWaves<T, D, RG> ? 0 : 64 * kTreeWaves<T, D, RG> * (D + 4);
+template <typename T, int D, int RG> constexpr size_t kTreeLds = kTreeUsed<T, D, RG> > kTreeJoin<T, D, RG> ? kTreeUsed<T, D, RG> : kTreeJoin<T, D, RG>;
+
+// The turn of a token's chunks of K in LDS: another one for each of eight lanes that
+// follow each other, whose tokens differ in bits 0, 1 and 3.
+template <int D> __device__ __forceinline__ uint32_t turn_of(uint32_t token) {
+  return D == 64 ? (token >> 1 & 1) | (token >> 2 & 2) : (token & 3) | (token >> 1 & 4);
 }
 
-template <int D> constexpr int kTreeKeys = D == 64 ? 64 : 32;
-template <typename T, int D> constexpr int kTreeResident = D * sizeof(T) > 512 ? 1 : 2;
+// A lane's four bytes to consecutive places, as to_lds.
+__device__ __forceinline__ void four_to_lds(const void* from, uint32_t at) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(at), "v"(from) : "memory", "m0");
+}
 
-template <typename T, int D>
-__global__ __launch_bounds__(64 * kWaves, (kTreeResident<T, D>)) void kv_attend_tree(TreeArgs A) {
+template <typename T, int D, int RG>
+__global__ __launch_bounds__((64 * kTreeWaves<T, D, RG>), (kTreeResident<T, D>)) void kv_attend_tree(TreeArgs A) {
   typedef Row<T> Q;
   typedef typename Q::frag frag;
-  constexpr int QP = Q::kQ, PP = Q::kP, KT = kTreeKeys<D>, KS = D / 16, ST = KT / 32, DT = D / 32;
-  constexpr uint32_t kRow = D * 2, kTile = KT * kRow, kUnits16 = KT * D / 16 / 256;   // 16 codes each, a thread
-  extern __shared__ __attribute__((aligned(16))) char lds[];   // [2][K, V][kTile]
-  // Per token: the factor of its scores, what is added to them (-infinity: there is no such
-  // token), and the power of two of its values.
-  __shared__ __attribute__((aligned(16))) float per_token[2][3][KT];
-  __shared__ uint32_t bad_drafts[2];   // drafts whose values are not finite
+  constexpr int W = kTreeWaves<T, D, RG>, QP = Q::kQ, PP = Q::kP, KG = W / RG, KT = kTreeKeys<D, RG>, S = kTreeStages;
+  constexpr int KS = D / 32, ST = KT / 32, DT = D / 32, kRows = 32 * RG;
+  constexpr uint32_t kHalf = KT * D, kStage = KG * 2 * kHalf;      // a tile's K, or V; a stage
+  constexpr uint32_t kLoads = kHalf / 1024 / RG;                   // of a wavefront: a tile's K, or V, 64 units of 16 codes each
+  constexpr int kPerStage = 2 * kLoads + 1;
+  constexpr uint32_t kUnits = D / 16;                              // a token's units of K
+  extern __shared__ __attribute__((aligned(16))) char lds[];       // [S][KG][K, V][kHalf]
+  __shared__ __attribute__((aligned(16))) uint8_t exps[S][W][2][KT];
+  __shared__ __attribute__((aligned(16))) float powers[W][Q::kFold ? 1 : 2][KT];   // of a tile's values, and keys
+  __shared__ float stat[W][32][2];
+  __shared__ uint64_t seen_words[W][32];   // the drafts that a row sees (by its own wavefront)
 
   const uint32_t lane = threadIdx.x & 63, i = lane & 31, h = lane >> 5;
-  const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), rg = wave % RG, kg = wave / RG;
   const Cache& C = A.cache;
-  // Stretches vary slowest, so that contexts that end early leave work for all dies.
-  uint32_t at = blockIdx.x;
-  const uint32_t head = at % C.heads;
-  at /= C.heads;
-  const uint32_t block = at % A.blocks;
-  at /= A.blocks;
-  const uint32_t seq = at % A.sequences, split = at / A.sequences;
-  if (threadIdx.x < 2) bad_drafts[threadIdx.x] = 0;
-  const Drafts S = drafts_of(A, seq);
-  if (S.bad) {
-    if (A.status && threadIdx.x == 0) atomicOr(A.status, S.bad);
-    if (S.bad == FR_HIP_BAD_OFFSET) return;
+  // Workgroups go to the eight dies in turn. A stretch's row blocks follow each other on
+  // one die, whose L2 then has the stretch; stretches vary slowest, each turned one die on,
+  // so that neither contexts that end early nor sequences of few rows leave a die without work.
+  const uint32_t of_eight = blockIdx.x / (8 * A.blocks), rest = blockIdx.x % (8 * A.blocks);
+  const uint32_t block = rest / 8, unit = of_eight * 8 + rest % 8, items = A.sequences * C.heads;
+  if (unit >= items * A.splits) return;
+  const uint32_t split = unit / items, item = (unit % items + split) % items;
+  const uint32_t head = item % C.heads, seq = item / C.heads;
+  const Drafts P = drafts_of(A, seq);
+  if (P.bad) {
+    if (A.status && threadIdx.x == 0) atomicOr(A.status, P.bad);
+    if (P.bad == FR_HIP_BAD_OFFSET) return;
   }
-  const uint32_t rows = S.n * A.per, row0 = block * R;
+  const uint32_t rows = P.n * A.per, row0 = block * kRows;
   if (row0 >= rows) return;
-  const uint32_t begin = split * A.chunk, end = max(begin, min(S.length, begin + A.chunk));
-  const uint32_t prefix = S.length - S.n;
-  const uint32_t wave_row = row0 + wave * 32, row = wave_row + i;
-  const uint64_t seen = row < rows ? (uint64_t)A.tree[S.q0 + row / A.per] & (~0ull >> (64 - S.n)) : 0;
+  const uint32_t begin = split * A.chunk, end = max(begin, min(P.length, begin + A.chunk));
+  const uint32_t prefix = P.length - P.n;
+  const uint32_t wave_row = row0 + rg * 32, row = wave_row + i;
   const int32_t* const table = A.table + (size_t)seq * A.table_stride;
-
-  // Q: lane (i, h) of step s holds row i's dims 16 s + 8 h ..
-  frag qf[QP][KS];
-  {
-    const uint32_t r = min(row, rows - 1);
-    const T* p = static_cast<const T*>(A.q) + (int64_t)(S.q0 + r / A.per) * A.q_token +
-                 (int64_t)(head * A.per + r % A.per) * A.q_head + h * 8;
-#pragma unroll
-    for (int s = 0; s < KS; ++s) {
-      float x[8];
-      load_row<8>(p + s * 16, A.wide, x);
-      if constexpr (QP == 3) {
-        bf16x8 parts[3];
-        split8<3>(x, parts);
-#pragma unroll
-        for (int q = 0; q < 3; ++q) qf[q][s] = parts[q];
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) qf[0][s][e] = (T)x[e];
-      }
-    }
-  }
-
-  // A thread's units of a tile: 16 codes of a K token, 16 tokens of a V dim; each
-  // wavefront's are of one block of 16 tokens. Blocks past the end are taken to be the
+  // Where 64 blocks of 16 tokens are (in blocks of the cache; kGone: their page is not
+  // there), a lane each, and the 64 behind them. Blocks past the end are taken to be the
   // last one.
-  struct Pages {
-    int32_t k[kUnits16], v[kUnits16], e;
-  };
-  auto place_of = [&](uint32_t n, uint32_t* page, uint32_t* in) {   // of the n-th block
-    n = min(n, (end - 1) >> 4);
+  constexpr uint32_t kGone = ~0u;
+  uint32_t first_place = begin >> 4;   // the block of `places`' first lane; a stage is of whole ones of 64
+  auto look_up = [&](uint32_t block) {
+    const uint32_t n = min(block + lane, (end - 1) >> 4);
     uint32_t q = __umulhi(n, A.reciprocal), r = n - q * A.page16;   // q or one below
     if (r >= A.page16) ++q, r -= A.page16;
-    *page = q, *in = r * 16;
+    const int32_t page = table[q];
+    return fronk::page_there(page, C.pages) ? ((uint32_t)page * C.heads + head) * A.page16 + r : kGone;
   };
-  const uint32_t e_token = threadIdx.x % KT;
-  auto k_block = [&](uint32_t base, uint32_t u) { return (base >> 4) + (wave * 64 + u * 256) / D; };   // (D / 16 units a token)
-  auto v_block = [&](uint32_t base, uint32_t u) { return (base >> 4) + (wave * 64 + u * 256) / D; };
-  auto look_up = [&](uint32_t base) {
-    Pages p;
-    uint32_t page, in;
+  uint32_t places = 0, places_next = 0;
+  bool missing = false;
+  uint32_t gone = 0;       // four bits a stage: blocks of the tile that are not there
+  // A stage's loads: this wavefront's part of its key group's tile, 64 units of 16 codes
+  // each, and all of the tile's exponents. (Past the end they are the last block's once
+  // more, so that there are always as many in flight.)
+  const uint32_t lane_token = lane / kUnits, lane_unit = lane % kUnits;
+  const uint32_t k_lane = (lane_token * kUnits + (lane_unit ^ turn_of<D>(lane_token))) * 16;
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_char*)lds + kg * 2 * kHalf;
+  const uint32_t exps0 = (uint32_t)(uintptr_t)(lds_char*)reinterpret_cast<char*>(&exps[0][wave][0][0]);
+  const uint8_t* const e_lane = (lane < KT / 4 ? C.k_exp : C.v_exp) + lane % 4 * 4;
+  auto load = [&](uint32_t base, uint32_t stage) __attribute__((always_inline)) {
+    if ((base >> 4) - first_place >= 64) first_place += 64, places = places_next, places_next = look_up(first_place + 64);
+    const uint32_t first = (base >> 4) - first_place + kg * (KT / 16);
+    uint32_t bits = 0;
 #pragma unroll
-    for (uint32_t u = 0; u < kUnits16; ++u) {
-      place_of(k_block(base, u), &page, &in);
-      p.k[u] = table[page];
-      place_of(v_block(base, u), &page, &in);
-      p.v[u] = table[page];
-    }
-    place_of((base + e_token) >> 4, &page, &in);
-    p.e = table[page];
-    return p;
-  };
-  uint4v kc[kUnits16], vc[kUnits16];
-  uint32_t ke, ve;
-  bool k_there[kUnits16], v_there[kUnits16], e_there, missing = false;
-  auto load = [&](uint32_t base, const Pages& p) {
-    uint32_t page, in;
+    for (uint32_t b = 0; b < KT / 16; ++b) bits |= (uint32_t)(__builtin_amdgcn_readlane(places, first + b) == kGone) << b;
+    gone = (gone & ~(15u << 4 * stage)) | bits << 4 * stage, missing |= bits;
+    const uint32_t to_k = lds0 + stage * kStage;
 #pragma unroll
-    for (uint32_t u = 0; u < kUnits16; ++u) {
-      place_of(k_block(base, u), &page, &in);
-      k_there[u] = fronk::page_there(p.k[u], C.pages);
-      const uint32_t unit = threadIdx.x + u * 256;
-      kc[u] = *reinterpret_cast<const uint4v*>(C.k_codes + exp_at(C, k_there[u] ? p.k[u] : 0, head, in) * D + (unit / (D / 16) % 16) * D + unit % (D / 16) * 16);
-      place_of(v_block(base, u), &page, &in);
-      v_there[u] = fronk::page_there(p.v[u], C.pages);
-      vc[u] = *reinterpret_cast<const uint4v*>(C.v_codes + exp_at(C, v_there[u] ? p.v[u] : 0, head, in) * D + unit % D * 16);
+    for (uint32_t l = 0; l < kLoads; ++l) {
+      const uint32_t u = rg * 64 + l * RG * 64, token = u / kUnits % 16;
+      const uint32_t place = __builtin_amdgcn_readlane(places, first + u / D);
+      const size_t from = (size_t)(place == kGone ? 0 : place) * (16 * D);
+      to_lds(reinterpret_cast<const char*>(C.k_codes) + from + token * D, k_lane ^ turn_of<D>(token) * 16, to_k + u * 16);
+      to_lds(reinterpret_cast<const char*>(C.v_codes) + from + u % D * 16, lane * 16, to_k + kHalf + u * 16);
     }
-    place_of((base + e_token) >> 4, &page, &in);
-    e_there = fronk::page_there(p.e, C.pages);
-    const size_t e = exp_at(C, e_there ? p.e : 0, head, in) + e_token % 16;
-    ke = C.k_exp[e], ve = C.v_exp[e];
-    missing |= !e_there;
-  };
-  // ... to LDS, as operands. What is not there, or past the end, is zeros.
-  const float scale = A.scale * kLog2e;
-  auto store = [&](uint32_t base, uint32_t buffer) {
-    char* const to = lds + buffer * 2 * kTile;
-    const bool drafts = base + KT > prefix;
-#pragma unroll
-    for (uint32_t u = 0; u < kUnits16; ++u) {
-      const uint32_t unit = threadIdx.x + u * 256, token = unit / (D / 16), c = unit % (D / 16) * 2;
-      if (!k_there[u] || base + token >= end) kc[u] = uint4v{0, 0, 0, 0};
-      const uint32_t first = unit / D * 16;
-#pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        vc[u][w] &= v_there[u] ? fronk::first_bytes((int)end - (int)(base + first + 4 * w)) : 0;
-        if (drafts) kc[u][w] = numbers(kc[u][w]), vc[u][w] = numbers(vc[u][w]);
-      }
-      *reinterpret_cast<frag*>(to + token * kRow + (c ^ (token & 7)) * 16) = codes8(kc[u][0], kc[u][1], frag{});
-      *reinterpret_cast<frag*>(to + token * kRow + ((c + 1) ^ (token & 7)) * 16) = codes8(kc[u][2], kc[u][3], frag{});
-      char* const v = to + kTile + unit * 32;
-      *reinterpret_cast<bf16x8*>(v) = codes8(vc[u][0], vc[u][2], bf16x8{});
-      *reinterpret_cast<bf16x8*>(v + 16) = codes8(vc[u][1], vc[u][3], bf16x8{});
-    }
-    if (threadIdx.x < KT) {
-      const uint32_t token = base + threadIdx.x;
-      const bool there = e_there && token < end;
-      // A draft whose values are not finite (zero codes) makes the rows that see it NaN at the end.
-      const bool bad = there && token >= prefix && ve == 255;
-      if (bad) atomicOr(&bad_drafts[(token - prefix) / 32], 1u << (token - prefix) % 32);
-      per_token[buffer][0][threadIdx.x] = there ? power(ke) * scale : 0.f;
-      per_token[buffer][1][threadIdx.x] = there ? 0.f : -INFINITY;
-      per_token[buffer][2][threadIdx.x] = there && !bad ? power(ve) : 0.f;
-    }
+    const uint32_t place = __shfl(places, (int)(first + lane % (KT / 4) / 4));
+    if (lane < KT / 2) four_to_lds(e_lane + (size_t)(place == kGone ? 0 : place) * 16, exps0 + stage * (W * 2 * KT));
   };
 
-  uint32_t k_at[4];   // as in prompt_attend
+  if (begin < end) {
+    places = look_up(first_place), places_next = look_up(first_place + 64);
+#pragma unroll 1
+    for (uint32_t k = 0; k < S - 1; ++k) load(begin + k * KG * KT, k);
+  }
+
+  if (h == 0) seen_words[wave][i] = row < rows ? (uint64_t)A.tree[P.q0 + row / A.per] & (~0ull >> (64 - P.n)) : 0;
+  // Drafts that any sees: what is held of others may be anything.
+  uint64_t any_seen = lane < P.n ? (uint64_t)A.tree[P.q0 + lane] : 0;
 #pragma unroll
-  for (uint32_t s = 0; s < 4; ++s) k_at[s] = i * kRow + ((2 * s + h) ^ (i & 7)) * 16;
-  const uint32_t v_at = kTile + i * 32 + h * 16;
+  for (int o = 1; o < 64; o *= 2) any_seen |= __shfl_xor((unsigned long long)any_seen, o);
+  any_seen = (uint32_t)same((int32_t)any_seen) | (uint64_t)(uint32_t)same((int32_t)(any_seen >> 32)) << 32;
+  // Q: lane (i, h) of step 2 s + j holds row i's dims 32 s + 16 h + 8 j ..
+  constexpr bool kQInLds = kTreeQInLds<T, D>;
+  frag qf[kQInLds ? 1 : QP][kQInLds ? 1 : 2 * KS];
+  float4v* const q_lds = reinterpret_cast<float4v*>(lds + kTreeTiles<T, D, RG>) + (rg * 2 * KS * 64 + lane) * 2;   // 128 on for each step
+  {
+    const uint32_t r = min(row, rows - 1);
+    const T* p = static_cast<const T*>(A.q) + (int64_t)(P.q0 + r / A.per) * A.q_token +
+                 (int64_t)(head * A.per + r % A.per) * A.q_head + h * 16;
+    auto take = [&](bool wide) __attribute__((always_inline)) {
+#pragma unroll
+      for (int s = 0; s < 2 * KS; ++s) {
+        float x[8];
+        load_row<8>(p + s / 2 * 32 + s % 2 * 8, wide, x);
+        if constexpr (QP == 3) {
+          bf16x8 parts[3];
+          split8<3>(x, parts);
+#pragma unroll
+          for (int q = 0; q < 3; ++q) qf[q][s] = parts[q];
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) qf[0][s][e] = (T)x[e];
+        }
+      }
+    };
+    if constexpr (kQInLds) {
+      if (kg == 0) {
+#pragma unroll 2
+        for (int s = 0; s < 2 * KS; ++s) {
+          float x[8];
+          load_row<8>(p + s / 2 * 32 + s % 2 * 8, A.wide, x);
+          const float one = A.scale < 0.f ? -1.f : 1.f;
+          q_lds[s * 128] = float4v{x[0], x[1], x[2], x[3]} * one, q_lds[s * 128 + 1] = float4v{x[4], x[5], x[6], x[7]} * one;
+        }
+      }
+    } else if constexpr (QP == 1) {
+      if (A.wide) {
+#pragma unroll
+        for (int s = 0; s < 2 * KS; ++s) qf[0][s] = *reinterpret_cast<const frag*>(p + s / 2 * 32 + s % 2 * 8);
+      } else {
+        take(false);
+      }
+    } else {
+      if (A.wide) take(true);
+      else take(false);
+    }
+    // A negative scale is taken to Q, as in prompt_attend.
+    const uint32_t sign = A.scale < 0.f ? 0x80008000u : 0u;
+#pragma unroll
+    for (int q = 0; q < (kQInLds ? 0 : QP); ++q)
+#pragma unroll
+      for (int s = 0; s < 2 * KS; ++s) qf[q][s] = __builtin_bit_cast(frag, __builtin_bit_cast(uint4v, qf[q][s]) ^ sign);
+  }
+
+  const float scale = fmaxf(fabsf(A.scale) * kLog2e, 1e-37f);
   float top = -INFINITY, shift = 0, sum = 0;
   float16v acc[DT];
 #pragma unroll
   for (int d = 0; d < DT; ++d) acc[d] = float16v{};
+  bool poisoned = false;
+  // Row i of a K operand is the token with bits 2 and 3 of i changed over, which leaves a
+  // lane in half h, in registers 8 s .. 8 s + 7, with tokens 16 s + 8 h ..: eight bytes of V.
+  const uint32_t k_token = (i & ~12u) | (i & 4) << 1 | (i & 8) >> 1;
 
-  auto compute = [&](uint32_t base, uint32_t buffer) {
-    const char* const tile = lds + buffer * 2 * kTile;
-    float16v st[ST];
-#pragma unroll
-    for (int t = 0; t < ST; ++t) {
-      st[t] = float16v{};
-#pragma unroll
-      for (int s = 0; s < KS; ++s) {
-        const frag a = *reinterpret_cast<const frag*>(tile + k_at[s % 4] + t * 32 * kRow + s / 4 * 128);
-#pragma unroll
-        for (int q = QP - 1; q >= 0; --q) st[t] = mma32(a, qf[q][s], st[t]);
-      }
-    }
-#pragma unroll
-    for (int t = 0; t < ST; ++t)
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const float4v f = *reinterpret_cast<const float4v*>(&per_token[buffer][0][t * 32 + 8 * g + 4 * h]);
-        const float4v b = *reinterpret_cast<const float4v*>(&per_token[buffer][1][t * 32 + 8 * g + 4 * h]);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) st[t][g * 4 + e] = __builtin_fmaf(st[t][g * 4 + e], f[e], b[e]);
-      }
-    if (base + KT > prefix) {
+  auto compute = [&](uint32_t base, uint32_t stage) __attribute__((always_inline)) {
+    base += kg * KT;
+    if (base >= end) return;
+    char* const kt = lds + stage * kStage + kg * 2 * kHalf;
+    char* const vt = kt + kHalf;
+    const uint32_t none = gone >> 4 * stage & 15;
+    // A tile of which rows see different parts, or not all is there; and tokens held with
+    // infinities or NaN (as zeros).
+    const uint32_t ke = exps[stage][wave][0][lane % KT], ve = exps[stage][wave][1][lane % KT];
+    const bool masked = base + KT > prefix || base + KT > end || none || __any(ke == 255 || ve == 255);
+    powers[wave][0][lane % KT] = ve == 255 ? 0.f : power(ve);
+    float k_power[ST];
+    if constexpr (Q::kFold) {
 #pragma unroll
       for (int t = 0; t < ST; ++t) {
-        // Which of 32 tokens the row sees: all before the drafts, and its own of those.
-        const int32_t first = (int32_t)(base + t * 32 - prefix);
-        const uint32_t bits = first <= -32 ? ~0u : first >= 64 ? 0u : first < 0 ? (uint32_t)(seen << -first) | ~(~0u << -first) : (uint32_t)(seen >> first);
+        const uint32_t e = exps[stage][wave][0][t * 32 + k_token];
+        k_power[t] = e == 255 ? 1.f : power(e);   // (zero codes)
+      }
+    } else {
+      powers[wave][1][lane % KT] = ke == 255 ? 0.f : power(ke);
+    }
+    uint32_t seen_bits[ST] = {}, bad_bits[ST] = {};
+    if (masked) {
+      const uint64_t bad_k = __ballot(ke == 255), bad_v = __ballot(ve == 255), seen = seen_words[wave][i];
 #pragma unroll
-        for (int r = 0; r < 16; ++r)
-          if (!(bits >> (4 * h) & 1u << (8 * (r / 4) + r % 4))) st[t][r] = -INFINITY;
+      for (int t = 0; t < ST; ++t) {
+        const int32_t left = (int32_t)(end - base) - t * 32, first = (int32_t)(base + t * 32 - prefix);
+        uint32_t there = left >= 32 ? ~0u : left <= 0 ? 0u : ~(~0u << left);
+        if (none >> 2 * t & 1) there &= 0xffff0000u;
+        if (none >> 2 * t & 2) there &= 0x0000ffffu;
+        // Which of 32 tokens are seen: all before the drafts, and of those the words' bits.
+        auto of = [&](uint64_t word) {
+          const uint32_t bits = first <= -32 ? ~0u : first >= 64 ? 0u : first < 0 ? (uint32_t)(word << -first) | ~(~0u << -first) : (uint32_t)(word >> first);
+          return bits & there;
+        };
+        seen_bits[t] = of(seen);
+        bad_bits[t] = seen_bits[t] & (uint32_t)(bad_k >> 32 * t);
+        poisoned |= (seen_bits[t] & (uint32_t)(bad_v >> 32 * t)) || bad_bits[t];
+        // Codes of V that count for nothing may be no numbers: zeros (which all
+        // wavefronts of the tile write alike).
+        const uint32_t any = of(any_seen);
+        if (any != ~0u)
+          for (uint32_t u = lane; u < 2 * D; u += 64) {
+            uint4v* const c = reinterpret_cast<uint4v*>(vt + t * 32 * D) + u;
+            uint4v x = *c;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) x[w] &= ((any >> (u / D * 16 + 4 * w) & 15) * 0x00204081u & 0x01010101u) * 255u;
+            *c = x;
+          }
       }
     }
-    float most = -INFINITY;
+    // Each step's operands are read while the one before it is worked on.
+    float16v st[ST];
+    constexpr int kK = KS < 4 ? 1 : 2, kV = DT < 4 ? DT : 4;   // reads at once
+    uint4v kc[2][kK];
+    auto read_k = [&](int n) __attribute__((always_inline)) {
 #pragma unroll
-    for (int t = 0; t < ST; ++t)
+      for (int k = 0; k < kK; ++k) {
+        const int s = n % (KS / kK) * kK + k;
+        kc[n % 2][k] = *reinterpret_cast<const uint4v*>(kt + (n / (KS / kK) * 32 + k_token) * D + ((2 * s + h) ^ turn_of<D>(k_token)) * 16);
+      }
+    };
+    read_k(0);
 #pragma unroll
-      for (int r = 0; r < 16; ++r) most = fmaxf(most, st[t][r]);
-    most = max_xor32(most);
-    if (__any(most > top + 8.f)) {   // (as in prompt_attend)
-      const float now = fmaxf(top, most), to = now == -INFINITY ? 0.f : now;
-      const float f = __builtin_amdgcn_exp2f(top - to);
+    for (int n = 0; n < ST * KS / kK; ++n) {
+      __builtin_amdgcn_sched_barrier(0);
+      if (n + 1 < ST * KS / kK) read_k(n + 1);
+      const int t = n / (KS / kK);
+      if (n % (KS / kK) == 0) st[t] = float16v{};
+#pragma unroll
+      for (int k = 0; k < kK; ++k) {
+        const uint4v c = kc[n % 2][k];
+        const int step = 2 * (n % (KS / kK) * kK + k);
+        frag a, b;
+        if constexpr (Q::kFold) a = codes8(c[0], c[1], k_power[t], frag{}), b = codes8(c[2], c[3], k_power[t], frag{});
+        else a = codes8(c[0], c[1], frag{}), b = codes8(c[2], c[3], frag{});
+        if constexpr (kQInLds) {
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const float4v x = q_lds[(step + j) * 128], y = q_lds[(step + j) * 128 + 1];
+            const float row[8] = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
+            bf16x8 parts[QP];
+            split8<QP>(row, parts);
+#pragma unroll
+            for (int q = QP - 1; q >= 0; --q) st[t] = mma32(j ? b : a, __builtin_bit_cast(frag, parts[q]), st[t]);
+          }
+        } else {
+#pragma unroll
+          for (int q = QP - 1; q >= 0; --q) st[t] = mma32(a, qf[q][step], st[t]);
+#pragma unroll
+          for (int q = QP - 1; q >= 0; --q) st[t] = mma32(b, qf[q][step + 1], st[t]);
+        }
+      }
+    }
+    uint2v vc[2][kV];
+    auto read_v = [&](int n) __attribute__((always_inline)) {   // of 16 tokens
+#pragma unroll
+      for (int d = 0; d < kV; ++d)
+        vc[n % 2][d] = *reinterpret_cast<const uint2v*>(vt + (n / (DT / kV) * D + (n % (DT / kV) * kV + d) * 32 + i) * 16 + h * 8);
+    };
+    if constexpr (!Q::kFold) {
+#pragma unroll
+      for (int t = 0; t < ST; ++t)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const float4v f = *reinterpret_cast<const float4v*>(&powers[wave][1][t * 32 + g / 2 * 16 + 8 * h + g % 2 * 4]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) st[t][g * 4 + e] *= f[e];
+        }
+    }
+    if (masked) {
+#pragma unroll
+      for (int t = 0; t < ST; ++t)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (!(seen_bits[t] >> (8 * h) & 1u << (16 * (r / 8) + r % 8))) st[t][r] = -INFINITY;
+    }
+    const float most = max_xor32(largest(st));
+    if (__any(most * scale > top * scale + 8.f)) {   // (as in prompt_attend)
+      const float now = fmaxf(top, most), to = now == -INFINITY ? 0.f : now * scale;
+      const float f = __builtin_amdgcn_exp2f(top * scale - to);
       top = now, shift = to, sum *= f;
 #pragma unroll
       for (int d = 0; d < DT; ++d) acc[d] *= f;
     }
+    __builtin_amdgcn_sched_barrier(0);
     bf16x8 pf[ST][2][PP];
-    float total = 0;
+    float total[4] = {};
 #pragma unroll
     for (int t = 0; t < ST; ++t)
 #pragma unroll
@@ -285,53 +395,113 @@ __global__ __launch_bounds__(64 * kWaves, (kTreeResident<T, D>)) void kv_attend_
         float w[8];
 #pragma unroll
         for (int g = 0; g < 2; ++g) {
-          const float4v f = *reinterpret_cast<const float4v*>(&per_token[buffer][2][t * 32 + s * 16 + 8 * g + 4 * h]);
+          const float4v f = *reinterpret_cast<const float4v*>(&powers[wave][0][t * 32 + s * 16 + 8 * h + 4 * g]);
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const float p = __builtin_amdgcn_exp2f(st[t][s * 8 + g * 4 + e] - shift);
-            total += p;
+            const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(st[t][s * 8 + g * 4 + e], scale, -shift));
+            total[e] += p;
             w[g * 4 + e] = p * f[e];
           }
         }
         split8<PP>(w, pf[t][s]);
       }
-    sum += total;
+    sum += (total[0] + total[1]) + (total[2] + total[3]);
+    read_v(0);
 #pragma unroll
-    for (int t = 0; t < ST; ++t)
+    for (int n = 0; n < 2 * ST * (DT / kV); ++n) {
+      __builtin_amdgcn_sched_barrier(0);
+      if (n + 1 < 2 * ST * (DT / kV)) read_v(n + 1);
+      const int s = n / (DT / kV);
 #pragma unroll
-      for (int s = 0; s < 2; ++s)
+      for (int k = 0; k < kV; ++k) {
+        const int d = n % (DT / kV) * kV + k;
+        const bf16x8 a = codes8(vc[n % 2][k][0], vc[n % 2][k][1], bf16x8{});
 #pragma unroll
-        for (int d = 0; d < DT; ++d) {
-          const bf16x8 a = *reinterpret_cast<const bf16x8*>(tile + v_at + ((t * 2 + s) * D + d * 32) * 32);
-#pragma unroll
-          for (int p = PP - 1; p >= 0; --p) acc[d] = mma32(a, pf[t][s][p], acc[d]);
-        }
+        for (int p = PP - 1; p >= 0; --p) acc[d] = mma32(a, pf[s / 2][s % 2][p], acc[d]);
+      }
+    }
   };
 
   if (begin < end) {
-    Pages pages = look_up(begin);
-    load(begin, pages);
-    pages = look_up(begin + KT);
-    store(begin, 0);
-    uint32_t buffer = 0;
-    for (uint32_t base = begin; base < end; base += KT) {
-      __syncthreads();
-      load(base + KT, pages);   // (past the end the last block once more: a load under a condition is waited for)
-      pages = look_up(base + 2 * KT);
-      if (wave_row < rows) compute(base, buffer);
-      if (base + KT < end) store(base + KT, buffer ^ 1);
-      buffer ^= 1;
+    uint32_t stage = 0;
+#pragma unroll 1
+    for (uint32_t base = begin; base < end; base += KG * KT) {
+      loads_done<(S - 2) * kPerStage>();   // and all wavefronts'
+      load(base + (S - 1) * KG * KT, (stage + S - 1) % S);
+      if (wave_row < rows) compute(base, stage);
+      stage = (stage + 1) % S;
     }
     if (missing && A.status) atomicOr(A.status, FR_HIP_BAD_PAGE);
+    loads_done<0>();
   }
-  __syncthreads();   // bad_drafts
 
   sum = add_xor32(sum);
+  if (poisoned) sum = NAN;
+  const bool many = A.splits > 1;
+  if constexpr (KG > 1) {
+    // Join the key groups by halves, in LDS; from there all write the rows.
+    if (h == 0) stat[wave][i][0] = sum == 0.f ? -INFINITY : shift, stat[wave][i][1] = sum;
+    __syncthreads();
+    float all = -INFINITY;
+#pragma unroll
+    for (int g = 0; g < KG; ++g) all = fmaxf(all, stat[g * RG + rg][i][0]);
+    const float to = all == -INFINITY ? 0.f : all, mine = stat[wave][i][0];
+    const float f = mine == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mine - to);
+    float joined = 0;
+#pragma unroll
+    for (int g = 0; g < KG; ++g) {
+      const float m = stat[g * RG + rg][i][0];
+      if (m != -INFINITY) joined += stat[g * RG + rg][i][1] * __builtin_amdgcn_exp2f(m - to);
+    }
+#pragma unroll
+    for (int d = 0; d < DT; ++d) acc[d] *= f;
+    constexpr uint32_t kPitch = D + 4;
+    float* const o = reinterpret_cast<float*>(lds);
+    auto place = [&](uint32_t group, int d, int q) __attribute__((always_inline)) {
+      return reinterpret_cast<float4v*>(o + (group * kRows + rg * 32 + i) * kPitch + d * 32 + q * 8 + 4 * h);
+    };
+#pragma unroll
+    for (int half = KG / 2; half >= 0; half /= 2) {
+      if (kg >= (uint32_t)half && kg < (uint32_t)(half ? 2 * half : 1)) {
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            *place(kg - half, d, q) = float4v{acc[d][q * 4], acc[d][q * 4 + 1], acc[d][q * 4 + 2], acc[d][q * 4 + 3]};
+        if (!half && h == 0) stat[wave][i][0] = joined == 0.f ? -INFINITY : to, stat[wave][i][1] = joined;
+      }
+      __syncthreads();
+      if (!half) break;
+      if (kg < (uint32_t)half) {
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const float4v x = *place(kg, d, q);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[d][q * 4 + e] += x[e];
+          }
+      }
+      __syncthreads();
+    }
+    const size_t part = (((size_t)(seq * A.blocks + block) * C.heads + head) * A.splits + split) * kRows;
+    for (uint32_t e = threadIdx.x; e < kRows * (D / 4); e += 64 * W) {
+      const uint32_t r = e / (D / 4), d = e % (D / 4) * 4;
+      if (row0 + r >= rows) break;
+      const float total = stat[r / 32][r % 32][1];
+      const float4v x = *reinterpret_cast<const float4v*>(o + r * kPitch + d);
+      if (many) {
+        if (d == 0) A.part_ml[(part + r) * 2] = stat[r / 32][r % 32][0], A.part_ml[(part + r) * 2 + 1] = total;
+        if (begin < end) *reinterpret_cast<float4v*>(A.part_o + (part + r) * D + d) = x;
+      } else {
+        put4<T>(draft_row<T>(A, P, head, row0 + r) + d, x, total, A.wide);
+      }
+    }
+    return;
+  }
   if (row >= rows) return;
-  if (seen & (bad_drafts[0] | (uint64_t)bad_drafts[1] << 32)) sum = NAN;
-  if (A.splits > 1) {
-    const uint32_t item = (seq * A.blocks + block) * C.heads + head;
-    const size_t to = ((size_t)item * A.splits + split) * R + (row - row0);
+  if (many) {
+    const size_t to = (((size_t)(seq * A.blocks + block) * C.heads + head) * A.splits + split) * kRows + (row - row0);
     if (h == 0) A.part_ml[to * 2] = sum == 0.f ? -INFINITY : shift, A.part_ml[to * 2 + 1] = sum;
     if (begin == end) return;
 #pragma unroll
@@ -342,7 +512,7 @@ __global__ __launch_bounds__(64 * kWaves, (kTreeResident<T, D>)) void kv_attend_
             float4v{acc[d][g * 4], acc[d][g * 4 + 1], acc[d][g * 4 + 2], acc[d][g * 4 + 3]};
     return;
   }
-  T* const p = draft_row<T>(A, S, head, row) + 4 * h;
+  T* const p = draft_row<T>(A, P, head, row) + 4 * h;
 #pragma unroll
   for (int d = 0; d < DT; ++d)
 #pragma unroll
@@ -350,18 +520,21 @@ __global__ __launch_bounds__(64 * kWaves, (kTreeResident<T, D>)) void kv_attend_
       put4<T>(p + d * 32 + g * 8, float4v{acc[d][g * 4], acc[d][g * 4 + 1], acc[d][g * 4 + 2], acc[d][g * 4 + 3]}, sum, A.wide);
 }
 
-// The stretches of a row joined, in their order: D / 4 lanes a row.
-template <typename T, int D>
-__global__ __launch_bounds__(256) void tree_merge(TreeArgs A) {
-  constexpr uint32_t L = D / 4, kAtOnce = 256 / L;
-  const uint32_t item = blockIdx.x / (R / kAtOnce), r = blockIdx.x % (R / kAtOnce) * kAtOnce + threadIdx.x / L;
+// The stretches of rows joined: one row a workgroup, or as many as have D / 4 lanes.
+template <typename T, int D, bool MANY>
+__global__ __launch_bounds__(256) void tree_merge(TreeArgs A, uint32_t block_rows) {
+  constexpr uint32_t L = D / 4, kAtOnce = MANY ? 1 : 256 / L;
+  const uint32_t parts = block_rows / kAtOnce;
+  const uint32_t item = blockIdx.x / parts, r = blockIdx.x % parts * kAtOnce + (MANY ? 0 : threadIdx.x / L);
   const uint32_t head = item % A.cache.heads, block = item / A.cache.heads % A.blocks, seq = item / A.cache.heads / A.blocks;
-  const Drafts S = drafts_of(A, seq);
-  const uint32_t row = block * R + r, d = threadIdx.x % L * 4;
-  if (S.bad == FR_HIP_BAD_OFFSET || row >= S.n * A.per) return;
+  const Drafts W = drafts_of(A, seq);
+  const uint32_t row = block * block_rows + r;
+  if (W.bad == FR_HIP_BAD_OFFSET || row >= W.n * A.per) return;
   float sum;
-  const float4v x = join<D>(A.part_o, A.part_ml, (size_t)item * A.splits * R + r, A.splits, d, &sum);
-  put4<T>(draft_row<T>(A, S, head, row) + d, x, sum, A.wide);
+  const size_t part = (size_t)item * A.splits * block_rows + r;
+  const float4v x = MANY ? join_many<D>(A.part_o, A.part_ml, part, A.splits, block_rows, &sum)
+                         : join_few<D>(A.part_o, A.part_ml, part, A.splits, block_rows, &sum);
+  if (!MANY || threadIdx.x < L) put4<T>(draft_row<T>(A, W, head, row) + threadIdx.x % L * 4, x, sum, A.wide);
 }
 
 // ---------------------------------------------------------------------- host
@@ -378,52 +551,76 @@ int check_tree(const fr_hip_kv_tree* r) {
   if (r->max_context > INT_MAX - (1u << 20)) return FR_HIP_INVALID;
   if (r->table_stride < (r->max_context + r->cache.page - 1) / r->cache.page) return FR_HIP_INVALID;
   if (rc) return rc;
+  if ((uint64_t)r->cache.pages * r->cache.heads * (r->cache.page / 16) >= UINT32_MAX) return FR_HIP_UNSUPPORTED;
   if (r->max_tokens > 64 || r->heads / r->cache.heads > 64) return FR_HIP_UNSUPPORTED;
   return FR_HIP_OK;
 }
 
-// How a call is cut: blocks of rows of a sequence, stretches of the context.
+// How a call is cut: blocks of 32 `groups` rows of a sequence, stretches of the context.
 struct TreeCut {
-  uint32_t blocks, splits, chunk;
+  uint32_t groups, blocks, splits, chunk;
   uint64_t items;
   size_t bytes;
 };
 TreeCut tree_cut(const fr_hip_kv_tree* r) {
   TreeCut c;
   const uint32_t drafts = r->max_tokens < r->tokens ? r->max_tokens : r->tokens;
-  c.blocks = (drafts * (r->heads / r->cache.heads) + R - 1) / R;
+  const uint32_t rows = drafts * (r->heads / r->cache.heads);
+  // 64 rows, or 32 where there are no more (128: the same to 20 % slower at 16 to 64 drafts).
+  c.groups = rows <= 32 ? 1 : 2;
+  c.blocks = (rows + 32 * c.groups - 1) / (32 * c.groups);
   c.items = (uint64_t)c.blocks * r->sequences * r->cache.heads;
-  const uint64_t want = c.items ? (kUnits + c.items - 1) / c.items : 1, most = (r->max_context + 255) / 256;
-  uint64_t n = want < most ? want : most;
-  n = n < 1 ? 1 : n > 256 ? 256 : n;
+  // Stretches so that workgroups fill all units a whole number of times (two each at
+  // once, one at dim 256), beginning and ending each taking as long as about 300 tokens;
+  // none with less than 256.
+  const uint64_t slots = kUnits * (r->cache.dim == 256 ? 1 : 2), most = (r->max_context + 255) / 256;
+  uint64_t n = 1, best = UINT64_MAX;
+  for (uint64_t rounds = 1; c.items && rounds <= 4; ++rounds) {
+    uint64_t k = rounds * slots / c.items;
+    k = k < 1 ? 1 : k > 256 ? 256 : k;
+    if (k > most) k = most ? most : 1;
+    const uint64_t cost = (c.items * k + slots - 1) / slots * (r->max_context / k + 300);
+    if (cost < best) best = cost, n = k;
+  }
   c.chunk = (uint32_t)((r->max_context + n * 64 - 1) / (n * 64)) * 64;
   if (!c.chunk) c.chunk = 64;
   c.splits = (r->max_context + c.chunk - 1) / c.chunk;
   if (!c.splits) c.splits = 1;
-  c.bytes = c.splits > 1 ? (size_t)c.items * c.splits * R * (r->cache.dim + 2) * sizeof(float) : 0;
+  c.bytes = c.splits > 1 ? (size_t)c.items * c.splits * 32 * c.groups * (r->cache.dim + 2) * sizeof(float) : 0;
   return c;
 }
-// Grids of less than 2^32 threads.
-bool tree_fits(const fr_hip_kv_tree* r, const TreeCut& c) {
-  return c.items * c.splits * 64 * kWaves <= UINT32_MAX && (c.splits == 1 || c.items * R * (r->cache.dim / 4) <= UINT32_MAX);
+// Grids of less than 2^32 threads, stretches rounded up to eight.
+bool tree_fits(const TreeCut& c) {
+  return (c.items * c.splits + 7 * c.blocks) * 512 <= UINT32_MAX && (c.splits == 1 || c.items * 32 * c.groups * 256 <= UINT32_MAX);
 }
 
-template <typename T, int D>
+uint32_t tree_grid(const TreeArgs& A, const TreeCut& c) {
+  return (A.sequences * A.cache.heads * c.splits + 7) / 8 * 8 * c.blocks;
+}
+
+template <typename T, int D, int RG>
 int launch_tree(const TreeArgs& A, const TreeCut& c, hipStream_t s) {
-  constexpr size_t kLds = 8ull * kTreeKeys<D> * D;
   static fronk::Devices done;
-  if (allow_lds(kv_attend_tree<T, D>, kLds, &done)) return FR_HIP_IO;
-  hipLaunchKernelGGL((kv_attend_tree<T, D>), dim3((uint32_t)(c.items * c.splits)), dim3(64 * kWaves), kLds, s, A);
-  if (c.splits > 1) hipLaunchKernelGGL((tree_merge<T, D>), dim3((uint32_t)(c.items * R / (1024 / D))), dim3(256), 0, s, A);
+  if (allow_lds(kv_attend_tree<T, D, RG>, kTreeLds<T, D, RG>, &done)) return FR_HIP_IO;
+  hipLaunchKernelGGL((kv_attend_tree<T, D, RG>), dim3(tree_grid(A, c)), dim3(64 * kTreeWaves<T, D, RG>), (kTreeLds<T, D, RG>), s, A);
+  return FR_HIP_OK;
+}
+template <typename T, int D>
+int launch_dim(const TreeArgs& A, const TreeCut& c, hipStream_t s) {
+  const int rc = c.groups == 1 ? launch_tree<T, D, 1>(A, c, s) : launch_tree<T, D, 2>(A, c, s);
+  if (rc) return rc;
+  const uint32_t rows = 32 * c.groups;
+  if (c.splits > kFewSplits) hipLaunchKernelGGL((tree_merge<T, D, true>), dim3((uint32_t)(c.items * rows)), dim3(256), 0, s, A, rows);
+  else if (c.splits > 1) hipLaunchKernelGGL((tree_merge<T, D, false>), dim3((uint32_t)(c.items * rows / (1024 / D))), dim3(256), 0, s, A, rows);
   FRONK_CK(hipGetLastError());
   return FR_HIP_OK;
 }
 template <typename T>
 int launch_dims(const TreeArgs& A, const TreeCut& c, hipStream_t s) {
   switch (A.cache.dim) {
-    case 64: return launch_tree<T, 64>(A, c, s);
-    case 128: return launch_tree<T, 128>(A, c, s);
-    default: return launch_tree<T, 256>(A, c, s);
+    case 64: return launch_dim<T, 64>(A, c, s);
+    case 128: return launch_dim<T, 128>(A, c, s);
+    default: return launch_dim<T, 256>(A, c, s);
   }
 }
 
@@ -434,14 +631,14 @@ extern "C" {
 size_t fr_hip_tree_workspace(const fr_hip_kv_tree* r) {
   if (check_tree(r)) return 0;
   const TreeCut c = tree_cut(r);
-  return tree_fits(r, c) ? c.bytes : 0;
+  return tree_fits(c) ? c.bytes : 0;
 }
 
 int fr_hip_kv_attend_tree(const fr_hip_kv_tree* r, void* workspace, size_t bytes, void* stream) {
   int rc = check_tree(r);
   if (rc) return rc;
   const TreeCut c = tree_cut(r);
-  if (!tree_fits(r, c)) return FR_HIP_UNSUPPORTED;
+  if (!tree_fits(c)) return FR_HIP_UNSUPPORTED;
   if (c.bytes && (!workspace || bytes < c.bytes || (uintptr_t)workspace % 16)) return FR_HIP_INVALID;
   hipStream_t s;
   rc = fronk::enter(stream, &s);
@@ -451,7 +648,7 @@ int fr_hip_kv_attend_tree(const fr_hip_kv_tree* r, void* workspace, size_t bytes
   A.q = r->q, A.o = r->o, A.tree = r->tree, A.offsets = r->offsets, A.table = r->table, A.length = r->length;
   A.status = r->status;
   A.part_o = static_cast<float*>(workspace);
-  A.part_ml = A.part_o + (c.splits > 1 ? (size_t)c.items * c.splits * R * r->cache.dim : 0);
+  A.part_ml = A.part_o + (c.splits > 1 ? (size_t)c.items * c.splits * 32 * c.groups * r->cache.dim : 0);
   A.q_token = r->q_token, A.q_head = r->q_head, A.o_token = r->o_token, A.o_head = r->o_head;
   A.sequences = r->sequences, A.tokens = r->tokens, A.max_tokens = r->max_tokens, A.per = r->heads / r->cache.heads;
   A.max_context = r->max_context, A.table_stride = r->table_stride, A.splits = c.splits, A.chunk = c.chunk, A.blocks = c.blocks;
