@@ -12,12 +12,14 @@ struct TreeArgs {
   Cache cache;
   const void* q;
   void* o;
-  float *part_o, *part_ml;       // [item][split][block's row][D], [item][split][block's row][2]
+  float *part_o, *part_ml;       // [workgroup][row][D], [workgroup][row][2]
+  uint2v* plan;                  // of each sequence: its first workgroup, stretches
   const int64_t* tree;
   const int32_t *offsets, *table, *length;
   uint32_t* status;
   int64_t q_token, q_head, o_token, o_head;
-  uint32_t sequences, tokens, max_tokens, per, max_context, table_stride, splits, chunk, blocks;
+  uint32_t sequences, tokens, max_tokens, per, max_context, table_stride, blocks;
+  uint32_t slots, at_once;       // workgroups that may have a part (0: nothing is split); that run at once
   uint32_t page16, reciprocal;   // blocks of 16 tokens a page, and 2^32 by it, rounded down
   float scale;
   bool wide;
@@ -39,6 +41,160 @@ __device__ __forceinline__ Drafts drafts_of(const TreeArgs& A, uint32_t seq) {
   if (__syncthreads_or(before > q0) || fronk::bad_sequence(0, 1, q0, q1, A.tokens, A.max_tokens)) d.bad = FR_HIP_BAD_OFFSET;
   else if ((int32_t)d.length < (int32_t)d.n || d.length > A.max_context) d.bad = FR_HIP_BAD_LENGTH, d.length = 0;
   return d;
+}
+// Where a workgroup works: `block` of the rows of one sequence and cache head, and one of
+// `splits` stretches of `chunk` tokens.
+struct Place {
+  Drafts d;
+  uint32_t seq, head, block, split, splits, chunk, part;   // (part ~0: no work)
+};
+
+constexpr uint32_t kPlanned = 512;   // sequences, at most, of a call that is split
+constexpr uint32_t kPlanBytes = (kPlanned * 6 + 8 * 64 + 4) * 4;
+
+// How the call is cut, which each workgroup finds out by itself from the sequences' lengths
+// (the host does not know them): stretches of all sequences are no longer than one bound,
+// for which 64 values are tried, a lane each, and that is taken with which the workgroups,
+// in rounds of as many as run at once, end first; a workgroup's beginning and end take as
+// long as about 300 tokens. Work then varies by less than two between workgroups however
+// ragged the batch is: 24 sequences of 1 to 61 drafts and up to 8192 tokens (16 heads of 128,
+// four of the cache) take 64 us, with one stretch length from the host 117, 96 of them in bf16
+// 184 and 289; 32 equal ones of 1024 tokens, for which nothing is to be found, 38 and 35.
+// Workgroups of one stretch (its row blocks) follow each other, and each die, to which
+// every eighth goes, has an eighth of the list: its L2 has the stretch for all of them.
+template <int W, int ROWS>
+__device__ __forceinline__ Place plan(const TreeArgs& A, uint32_t* lds) {
+  Place p;
+  const uint32_t heads = A.cache.heads, die = blockIdx.x % 8, nth = blockIdx.x / 8, tid = threadIdx.x;
+  // A list of `total`: this workgroup's place in it, ~0 for none.
+  auto in_list = [&](uint32_t total) {
+    const uint32_t eighth = (total + 7) / 8, mine = die * eighth + nth;
+    return nth < eighth && mine < total ? mine : ~0u;
+  };
+  auto at = [&](uint32_t local, uint32_t blocks) {
+    p.block = local % blocks, p.head = local / blocks % heads, p.split = local / blocks / heads;
+    p.chunk = ((p.d.length + p.splits - 1) / p.splits + 63) & ~63u;
+  };
+  if (A.sequences > kPlanned) {   // nothing is split
+    p.part = in_list(A.sequences * heads * A.blocks);
+    if (p.part == ~0u) return p;
+    p.seq = p.part / A.blocks / heads, p.splits = 1;
+    p.d = drafts_of(A, p.seq);
+    at(p.part % (A.blocks * heads), A.blocks);
+    if (p.d.bad && A.status && tid == 0) atomicOr(A.status, p.d.bad);
+    if (p.d.bad == FR_HIP_BAD_OFFSET || p.block * ROWS >= p.d.n * A.per) p.part = ~0u;
+    return p;
+  }
+  if (A.sequences == 1) {         // as many stretches as there may be workgroups
+    p.seq = 0, p.d = drafts_of(A, 0);
+    if (p.d.bad && A.status && blockIdx.x == 0 && tid == 0) atomicOr(A.status, p.d.bad);
+    const uint32_t blocks = p.d.bad == FR_HIP_BAD_OFFSET ? 0 : (p.d.n * A.per + ROWS - 1) / ROWS, work = blocks * heads;
+    p.splits = 1;
+    if (work && 2 * work <= A.slots) {
+      const uint32_t n = min(A.slots / work, 256u), chunk = max((p.d.length / n + 64) & ~63u, 256u);
+      p.splits = max((p.d.length + chunk - 1) / chunk, 1u);
+    }
+    if (blockIdx.x == 0 && tid == 0 && A.slots) A.plan[0] = uint2v{0, p.splits};
+    p.part = in_list(work * p.splits);
+    if (p.part != ~0u) at(p.part, blocks);
+    return p;
+  }
+  uint32_t* const length = lds;                    // [sequences]
+  uint32_t* const blocks = length + kPlanned;      // row blocks (none: a sequence without work)
+  uint32_t* const first = blocks + kPlanned;       // its workgroups' place in the list
+  uint32_t* const stretches = first + kPlanned;
+  uint32_t* const start = stretches + kPlanned;    // its first row of q
+  uint32_t* const drafts = start + kPlanned;
+  uint32_t* const sums = drafts + kPlanned;        // [W][64]
+  uint32_t* const found = sums + 8 * 64;
+  const uint32_t lane = tid & 63, wave = tid >> 6;
+  if (wave == 0) {
+    uint32_t bad = 0, longest = 0;
+    int32_t before = 0;   // the largest offset so far
+    for (uint32_t s0 = 0; s0 < A.sequences; s0 += 64) {
+      const uint32_t s = min(s0 + lane, A.sequences - 1);
+      int32_t q0 = s * A.max_tokens, q1 = q0 + A.max_tokens;
+      if (A.offsets) q0 = A.offsets[s], q1 = A.offsets[s + 1];
+      int32_t most = max(q0, before);
+      if (__any(q1 < q0 || before > q0)) {   // (else they are in order)
+#pragma unroll
+        for (int o = 1; o < 64; o *= 2) {
+          const int32_t other = __shfl_up(most, o);
+          if (lane >= (uint32_t)o) most = max(most, other);
+        }
+      }
+      before = __shfl(most, 63);
+      uint32_t n = 0, len = (uint32_t)A.length[s];
+      if (most > q0 || fronk::bad_sequence(0, 1, q0, q1, A.tokens, A.max_tokens)) bad |= FR_HIP_BAD_OFFSET, len = 0;
+      else if (n = q1 - q0, (int32_t)len < (int32_t)n || len > A.max_context) bad |= FR_HIP_BAD_LENGTH, len = 0;
+      longest = max(longest, len);
+      if (s0 + lane < A.sequences) length[s] = len, blocks[s] = (n * A.per + ROWS - 1) / ROWS, start[s] = q0, drafts[s] = n;
+    }
+    if (blockIdx.x == 0 && A.status && bad) atomicOr(A.status, bad);
+#pragma unroll
+    for (int o = 1; o < 64; o *= 2) longest = max(longest, (uint32_t)__shfl_xor((int)longest, o));
+    if (lane == 0) found[0] = ~0u, found[1] = longest;
+  }
+  __syncthreads();
+  uint32_t chunk = ((max(found[1], 1u) + 63) & ~63u);
+  // Stretches of a sequence, of at most `chunk` tokens.
+  auto count = [&](uint32_t s, uint32_t chunk, uint32_t reciprocal) {
+    uint32_t q = __umulhi(length[s], reciprocal);   // tokens by chunk: this, one or two more
+    while (q * chunk < length[s]) ++q;
+    return q ? q : 1;
+  };
+  if (A.slots) {
+    // (2^(7/8) and so on; 64 of these: 2^7.9 stretches of the longest)
+    const uint32_t mine = max(((uint32_t)((float)chunk * __builtin_amdgcn_exp2f(lane * -.125f)) + 63) & ~63u, 256u);
+    const uint32_t reciprocal = 0xffffffffu / mine;
+    uint32_t total = 0;
+    for (uint32_t s = wave; s < A.sequences; s += W)
+      if (blocks[s]) total += blocks[s] * count(s, mine, reciprocal);
+    sums[wave * 64 + lane] = total;
+    __syncthreads();
+    total = 0;
+#pragma unroll
+    for (int w = 0; w < W; ++w) total += sums[w * 64 + lane];
+    total *= heads;
+    // (in 64 tokens; what has too many workgroups, or stretches beyond all use, comes last)
+    const uint32_t most = (1u << 26) - 1, rounds = (total + A.at_once - 1) / A.at_once;
+    uint32_t best = (total <= A.slots ? min(rounds * (mine / 64 + 5), most) : most) << 6 | lane;
+#pragma unroll
+    for (int o = 1; o < 64; o *= 2) best = min(best, (uint32_t)__shfl_xor((int)best, o));
+    chunk = __shfl((int)mine, (int)(best & 63));
+  }
+  if (wave == 0) {
+    const uint32_t reciprocal = 0xffffffffu / chunk;
+    uint32_t total = 0;
+    for (uint32_t s0 = 0; s0 < A.sequences; s0 += 64) {
+      const uint32_t s = s0 + lane;
+      const uint32_t n = s < A.sequences && blocks[s] ? count(s, chunk, reciprocal) : 0, work = n ? n * blocks[s] * heads : 0;
+      uint32_t sum = work;
+#pragma unroll
+      for (int o = 1; o < 64; o *= 2) {
+        const uint32_t other = __shfl_up((int)sum, o);
+        if (lane >= (uint32_t)o) sum += other;
+      }
+      if (s < A.sequences) {
+        first[s] = total + sum - work, stretches[s] = n;
+        if (blockIdx.x == 0 && A.slots) A.plan[s] = uint2v{total + sum - work, n};
+      }
+      total += __shfl((int)sum, 63);
+    }
+    const uint32_t mine = in_list(total);
+    if (mine != ~0u)
+      for (uint32_t s = lane; s < A.sequences; s += 64)
+        if (mine - first[s] < stretches[s] * blocks[s] * heads) found[0] = s;
+    found[2] = mine;
+  }
+  __syncthreads();
+  p.seq = same(found[0]), p.part = same(found[2]);
+  if (p.part == ~0u) return p;
+  p.d = Drafts{same(start[p.seq]), (uint32_t)same(drafts[p.seq]), (uint32_t)same(length[p.seq]), 0};
+  p.splits = same(stretches[p.seq]);
+  at(p.part - same(first[p.seq]), same(blocks[p.seq]));
+  __syncthreads();   // (LDS is written anew)
+  return p;
 }
 template <typename T> __device__ __forceinline__ T* draft_row(const TreeArgs& A, const Drafts& S, uint32_t head, uint32_t row) {
   return static_cast<T*>(A.o) + (int64_t)(S.q0 + row / A.per) * A.o_token + (int64_t)(head * A.per + row % A.per) * A.o_head;
@@ -123,22 +279,13 @@ __global__ __launch_bounds__((64 * kTreeWaves<T, D, RG>), (kTreeResident<T, D>))
   const uint32_t lane = threadIdx.x & 63, i = lane & 31, h = lane >> 5;
   const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), rg = wave % RG, kg = wave / RG;
   const Cache& C = A.cache;
-  // Workgroups go to the eight dies in turn. A stretch's row blocks follow each other on
-  // one die, whose L2 then has the stretch; stretches vary slowest, each turned one die on,
-  // so that neither contexts that end early nor sequences of few rows leave a die without work.
-  const uint32_t of_eight = blockIdx.x / (8 * A.blocks), rest = blockIdx.x % (8 * A.blocks);
-  const uint32_t block = rest / 8, unit = of_eight * 8 + rest % 8, items = A.sequences * C.heads;
-  if (unit >= items * A.splits) return;
-  const uint32_t split = unit / items, item = (unit % items + split) % items;
-  const uint32_t head = item % C.heads, seq = item / C.heads;
-  const Drafts P = drafts_of(A, seq);
-  if (P.bad) {
-    if (A.status && threadIdx.x == 0) atomicOr(A.status, P.bad);
-    if (P.bad == FR_HIP_BAD_OFFSET) return;
-  }
+  static_assert(kTreeLds<T, D, RG> >= kPlanBytes, "the plan is made in the tiles' place");
+  const Place place = plan<W, kRows>(A, reinterpret_cast<uint32_t*>(lds));
+  if (place.part == ~0u) return;
+  const Drafts P = place.d;
+  const uint32_t seq = place.seq, head = place.head, block = place.block;
   const uint32_t rows = P.n * A.per, row0 = block * kRows;
-  if (row0 >= rows) return;
-  const uint32_t begin = split * A.chunk, end = max(begin, min(P.length, begin + A.chunk));
+  const uint32_t begin = place.split * place.chunk, end = max(begin, min(P.length, begin + place.chunk));
   const uint32_t prefix = P.length - P.n;
   const uint32_t wave_row = row0 + rg * 32, row = wave_row + i;
   const int32_t* const table = A.table + (size_t)seq * A.table_stride;
@@ -312,6 +459,7 @@ __global__ __launch_bounds__((64 * kTreeWaves<T, D, RG>), (kTreeResident<T, D>))
       }
     }
     // Each step's operands are read while the one before it is worked on.
+    __builtin_amdgcn_s_setprio(1);   // (matrix work before other wavefronts': 4 % less at 64 rows)
     float16v st[ST];
     constexpr int kK = KS < 4 ? 1 : 2, kV = DT < 4 ? DT : 4;   // reads at once
     uint4v kc[2][kK];
@@ -377,6 +525,7 @@ __global__ __launch_bounds__((64 * kTreeWaves<T, D, RG>), (kTreeResident<T, D>))
         for (int r = 0; r < 16; ++r)
           if (!(seen_bits[t] >> (8 * h) & 1u << (16 * (r / 8) + r % 8))) st[t][r] = -INFINITY;
     }
+    __builtin_amdgcn_s_setprio(0);
     const float most = max_xor32(largest(st));
     if (__any(most * scale > top * scale + 8.f)) {   // (as in prompt_attend)
       const float now = fmaxf(top, most), to = now == -INFINITY ? 0.f : now * scale;
@@ -407,6 +556,7 @@ __global__ __launch_bounds__((64 * kTreeWaves<T, D, RG>), (kTreeResident<T, D>))
       }
     sum += (total[0] + total[1]) + (total[2] + total[3]);
     read_v(0);
+    __builtin_amdgcn_s_setprio(1);
 #pragma unroll
     for (int n = 0; n < 2 * ST * (DT / kV); ++n) {
       __builtin_amdgcn_sched_barrier(0);
@@ -420,6 +570,7 @@ __global__ __launch_bounds__((64 * kTreeWaves<T, D, RG>), (kTreeResident<T, D>))
         for (int p = PP - 1; p >= 0; --p) acc[d] = mma32(a, pf[s / 2][s % 2][p], acc[d]);
       }
     }
+    __builtin_amdgcn_s_setprio(0);
   };
 
   if (begin < end) {
@@ -437,7 +588,7 @@ __global__ __launch_bounds__((64 * kTreeWaves<T, D, RG>), (kTreeResident<T, D>))
 
   sum = add_xor32(sum);
   if (poisoned) sum = NAN;
-  const bool many = A.splits > 1;
+  const bool many = place.splits > 1;
   if constexpr (KG > 1) {
     // Join the key groups by halves, in LDS; from there all write the rows.
     if (h == 0) stat[wave][i][0] = sum == 0.f ? -INFINITY : shift, stat[wave][i][1] = sum;
@@ -457,7 +608,7 @@ __global__ __launch_bounds__((64 * kTreeWaves<T, D, RG>), (kTreeResident<T, D>))
     for (int d = 0; d < DT; ++d) acc[d] *= f;
     constexpr uint32_t kPitch = D + 4;
     float* const o = reinterpret_cast<float*>(lds);
-    auto place = [&](uint32_t group, int d, int q) __attribute__((always_inline)) {
+    auto lds_row = [&](uint32_t group, int d, int q) __attribute__((always_inline)) {
       return reinterpret_cast<float4v*>(o + (group * kRows + rg * 32 + i) * kPitch + d * 32 + q * 8 + 4 * h);
     };
 #pragma unroll
@@ -467,7 +618,7 @@ __global__ __launch_bounds__((64 * kTreeWaves<T, D, RG>), (kTreeResident<T, D>))
         for (int d = 0; d < DT; ++d)
 #pragma unroll
           for (int q = 0; q < 4; ++q)
-            *place(kg - half, d, q) = float4v{acc[d][q * 4], acc[d][q * 4 + 1], acc[d][q * 4 + 2], acc[d][q * 4 + 3]};
+            *lds_row(kg - half, d, q) = float4v{acc[d][q * 4], acc[d][q * 4 + 1], acc[d][q * 4 + 2], acc[d][q * 4 + 3]};
         if (!half && h == 0) stat[wave][i][0] = joined == 0.f ? -INFINITY : to, stat[wave][i][1] = joined;
       }
       __syncthreads();
@@ -477,14 +628,14 @@ __global__ __launch_bounds__((64 * kTreeWaves<T, D, RG>), (kTreeResident<T, D>))
         for (int d = 0; d < DT; ++d)
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
-            const float4v x = *place(kg, d, q);
+            const float4v x = *lds_row(kg, d, q);
 #pragma unroll
             for (int e = 0; e < 4; ++e) acc[d][q * 4 + e] += x[e];
           }
       }
       __syncthreads();
     }
-    const size_t part = (((size_t)(seq * A.blocks + block) * C.heads + head) * A.splits + split) * kRows;
+    const size_t part = (size_t)place.part * kRows;
     for (uint32_t e = threadIdx.x; e < kRows * (D / 4); e += 64 * W) {
       const uint32_t r = e / (D / 4), d = e % (D / 4) * 4;
       if (row0 + r >= rows) break;
@@ -501,7 +652,7 @@ __global__ __launch_bounds__((64 * kTreeWaves<T, D, RG>), (kTreeResident<T, D>))
   }
   if (row >= rows) return;
   if (many) {
-    const size_t to = (((size_t)(seq * A.blocks + block) * C.heads + head) * A.splits + split) * kRows + (row - row0);
+    const size_t to = (size_t)place.part * kRows + (row - row0);
     if (h == 0) A.part_ml[to * 2] = sum == 0.f ? -INFINITY : shift, A.part_ml[to * 2 + 1] = sum;
     if (begin == end) return;
 #pragma unroll
@@ -527,13 +678,17 @@ __global__ __launch_bounds__(256) void tree_merge(TreeArgs A, uint32_t block_row
   const uint32_t parts = block_rows / kAtOnce;
   const uint32_t item = blockIdx.x / parts, r = blockIdx.x % parts * kAtOnce + (MANY ? 0 : threadIdx.x / L);
   const uint32_t head = item % A.cache.heads, block = item / A.cache.heads % A.blocks, seq = item / A.cache.heads / A.blocks;
-  const Drafts W = drafts_of(A, seq);
-  const uint32_t row = block * block_rows + r;
-  if (W.bad == FR_HIP_BAD_OFFSET || row >= W.n * A.per) return;
+  const uint2v plan = A.plan[seq];
+  if (plan[1] < 2) return;   // (written as it is)
+  Drafts W = {(int32_t)(seq * A.max_tokens), A.max_tokens, 0, 0};
+  if (A.offsets) W.q0 = A.offsets[seq], W.n = A.offsets[seq + 1] - W.q0;
+  const uint32_t row = block * block_rows + r, rows = W.n * A.per;
+  if (row >= rows) return;
   float sum;
-  const size_t part = (size_t)item * A.splits * block_rows + r;
-  const float4v x = MANY ? join_many<D>(A.part_o, A.part_ml, part, A.splits, block_rows, &sum)
-                         : join_few<D>(A.part_o, A.part_ml, part, A.splits, block_rows, &sum);
+  const uint32_t blocks = (rows + block_rows - 1) / block_rows, apart = A.cache.heads * blocks * block_rows;
+  const size_t part = (size_t)(plan[0] + head * blocks + block) * block_rows + r;
+  const float4v x = MANY ? join_many<D>(A.part_o, A.part_ml, part, plan[1], apart, &sum)
+                         : join_few<D>(A.part_o, A.part_ml, part, plan[1], apart, &sum);
   if (!MANY || threadIdx.x < L) put4<T>(draft_row<T>(A, W, head, row) + threadIdx.x % L * 4, x, sum, A.wide);
 }
 
@@ -556,10 +711,11 @@ int check_tree(const fr_hip_kv_tree* r) {
   return FR_HIP_OK;
 }
 
-// How a call is cut: blocks of 32 `groups` rows of a sequence, stretches of the context.
+// How a call is cut: blocks of 32 `groups` rows of a sequence, and into how many
+// workgroups at most (plan).
 struct TreeCut {
-  uint32_t groups, blocks, splits, chunk;
-  uint64_t items;
+  uint32_t groups, blocks, at_once, slots;
+  uint64_t items, grid;
   size_t bytes;
 };
 TreeCut tree_cut(const fr_hip_kv_tree* r) {
@@ -570,39 +726,24 @@ TreeCut tree_cut(const fr_hip_kv_tree* r) {
   c.groups = rows <= 32 ? 1 : 2;
   c.blocks = (rows + 32 * c.groups - 1) / (32 * c.groups);
   c.items = (uint64_t)c.blocks * r->sequences * r->cache.heads;
-  // Stretches so that workgroups fill all units a whole number of times (two each at
-  // once, one at dim 256), beginning and ending each taking as long as about 300 tokens;
-  // none with less than 256.
-  const uint64_t slots = kUnits * (r->cache.dim == 256 ? 1 : 2), most = (r->max_context + 255) / 256;
-  uint64_t n = 1, best = UINT64_MAX;
-  for (uint64_t rounds = 1; c.items && rounds <= 4; ++rounds) {
-    uint64_t k = rounds * slots / c.items;
-    k = k < 1 ? 1 : k > 256 ? 256 : k;
-    if (k > most) k = most ? most : 1;
-    const uint64_t cost = (c.items * k + slots - 1) / slots * (r->max_context / k + 300);
-    if (cost < best) best = cost, n = k;
-  }
-  c.chunk = (uint32_t)((r->max_context + n * 64 - 1) / (n * 64)) * 64;
-  if (!c.chunk) c.chunk = 64;
-  c.splits = (r->max_context + c.chunk - 1) / c.chunk;
-  if (!c.splits) c.splits = 1;
-  c.bytes = c.splits > 1 ? (size_t)c.items * c.splits * 32 * c.groups * (r->cache.dim + 2) * sizeof(float) : 0;
+  // Two workgroups a unit at once, one at dim 256; up to three such rounds are split.
+  c.at_once = kUnits * (r->cache.dim == 256 ? 1 : 2);
+  const uint64_t rounds = (c.items + c.at_once - 1) / c.at_once;
+  c.slots = rounds > 3 || r->sequences > kPlanned || r->max_context <= 256 ? 0 : (uint32_t)rounds * c.at_once;
+  c.grid = ((c.items > c.slots ? c.items : c.slots) + 7) / 8 * 8;
+  c.bytes = c.slots ? (size_t)c.slots * 32 * c.groups * (r->cache.dim + 2) * sizeof(float) + r->sequences * sizeof(uint2v) : 0;
   return c;
 }
-// Grids of less than 2^32 threads, stretches rounded up to eight.
+// Grids of less than 2^32 threads.
 bool tree_fits(const TreeCut& c) {
-  return (c.items * c.splits + 7 * c.blocks) * 512 <= UINT32_MAX && (c.splits == 1 || c.items * 32 * c.groups * 256 <= UINT32_MAX);
-}
-
-uint32_t tree_grid(const TreeArgs& A, const TreeCut& c) {
-  return (A.sequences * A.cache.heads * c.splits + 7) / 8 * 8 * c.blocks;
+  return c.grid * 512 <= UINT32_MAX && c.items * 32 * c.groups * 256 <= (c.slots ? UINT32_MAX : UINT64_MAX);
 }
 
 template <typename T, int D, int RG>
 int launch_tree(const TreeArgs& A, const TreeCut& c, hipStream_t s) {
   static fronk::Devices done;
   if (allow_lds(kv_attend_tree<T, D, RG>, kTreeLds<T, D, RG>, &done)) return FR_HIP_IO;
-  hipLaunchKernelGGL((kv_attend_tree<T, D, RG>), dim3(tree_grid(A, c)), dim3(64 * kTreeWaves<T, D, RG>), (kTreeLds<T, D, RG>), s, A);
+  hipLaunchKernelGGL((kv_attend_tree<T, D, RG>), dim3((uint32_t)c.grid), dim3(64 * kTreeWaves<T, D, RG>), (kTreeLds<T, D, RG>), s, A);
   return FR_HIP_OK;
 }
 template <typename T, int D>
@@ -610,8 +751,9 @@ int launch_dim(const TreeArgs& A, const TreeCut& c, hipStream_t s) {
   const int rc = c.groups == 1 ? launch_tree<T, D, 1>(A, c, s) : launch_tree<T, D, 2>(A, c, s);
   if (rc) return rc;
   const uint32_t rows = 32 * c.groups;
-  if (c.splits > kFewSplits) hipLaunchKernelGGL((tree_merge<T, D, true>), dim3((uint32_t)(c.items * rows)), dim3(256), 0, s, A, rows);
-  else if (c.splits > 1) hipLaunchKernelGGL((tree_merge<T, D, false>), dim3((uint32_t)(c.items * rows / (1024 / D))), dim3(256), 0, s, A, rows);
+  // A workgroup a row where there are few (8000 of them take 29 us, those of 8 rows 9).
+  if (c.slots && c.items * rows <= 2048) hipLaunchKernelGGL((tree_merge<T, D, true>), dim3((uint32_t)(c.items * rows)), dim3(256), 0, s, A, rows);
+  else if (c.slots) hipLaunchKernelGGL((tree_merge<T, D, false>), dim3((uint32_t)(c.items * rows / (1024 / D))), dim3(256), 0, s, A, rows);
   FRONK_CK(hipGetLastError());
   return FR_HIP_OK;
 }
@@ -648,10 +790,12 @@ int fr_hip_kv_attend_tree(const fr_hip_kv_tree* r, void* workspace, size_t bytes
   A.q = r->q, A.o = r->o, A.tree = r->tree, A.offsets = r->offsets, A.table = r->table, A.length = r->length;
   A.status = r->status;
   A.part_o = static_cast<float*>(workspace);
-  A.part_ml = A.part_o + (c.splits > 1 ? (size_t)c.items * c.splits * 32 * c.groups * r->cache.dim : 0);
+  A.part_ml = A.part_o + (size_t)c.slots * 32 * c.groups * r->cache.dim;
+  A.plan = reinterpret_cast<uint2v*>(A.part_ml + (size_t)c.slots * 32 * c.groups * 2);
   A.q_token = r->q_token, A.q_head = r->q_head, A.o_token = r->o_token, A.o_head = r->o_head;
   A.sequences = r->sequences, A.tokens = r->tokens, A.max_tokens = r->max_tokens, A.per = r->heads / r->cache.heads;
-  A.max_context = r->max_context, A.table_stride = r->table_stride, A.splits = c.splits, A.chunk = c.chunk, A.blocks = c.blocks;
+  A.max_context = r->max_context, A.table_stride = r->table_stride, A.blocks = c.blocks;
+  A.slots = c.slots, A.at_once = c.at_once;
   A.page16 = r->cache.page / 16, A.reciprocal = 0xffffffffu / A.page16;
   A.scale = r->scale;
   A.wide = rows_wide(r->type, r->q, r->o, r->q_token, r->q_head, r->o_token, r->o_head);

@@ -189,6 +189,41 @@ def test_bad_lengths_pages_and_offsets():
         check(got, q, x, y, masks, lens, 0.125)
 
 
+@pytest.mark.parametrize("sequences,longest", [(2, 3000), (70, 1400), (70, 200), (200, 700), (520, 300)])
+def test_ragged_batches(sequences, longest):
+    """One long context among short ones, sequences without drafts, and an offset out of order behind
+    the first 64: rows of the others and behind the last stay as they are."""
+    r = random.Random(sequences)
+    lens = [r.choice((0, 1, 1, 2, 5, 9)) for _ in range(sequences)]
+    lens[1] = 17
+    lengths = [n + r.randint(0, 40) for n in lens]
+    lengths[1] = longest
+    cache, table, k, v = filled(31, lengths, 1, 16, 64)
+    masks, total = trees(32, lens), sum(lens)
+    q = torch.randn(total + 3, 3, 64, generator=gen(33)).to(BF16)
+    w = words(masks + [1, 1, 1]).cuda()
+    out, status = torch.full((total + 3, 3, 64), 9.0, dtype=BF16, device="cuda"), torch.zeros(1, dtype=torch.int32, device="cuda")
+    call = lambda offsets: dense.kv_attend_tree(cache, q.cuda(), w, table, ints(lengths), offsets=offsets, max_tokens=20, out=out, status=status)
+    want = call(starts(lens)).cpu()
+    assert status.item() == 0 and (want[total:] == 9).all()
+    check(want[:total], q[:total], k, v, masks, lens, 0.125)
+    if sequences > 66:
+        offsets = starts(lens)
+        offsets[66] -= 20   # ends before it, and all that begin below an earlier one
+        out.fill_(9.0)
+        got = call(offsets).cpu()
+        at = offsets.tolist()
+        bad = [max([0] + at[:s]) > at[s] or not 0 <= at[s + 1] - at[s] <= 20 for s in range(sequences)]
+        assert status.item() == dense.BAD_OFFSET and bad[65] and bad[66]
+        kept = torch.zeros(total + 3, dtype=torch.bool)
+        for s in range(sequences):
+            if not bad[s]:
+                kept[at[s]:at[s + 1]] = True
+        assert (got[~kept] == 9).all()
+        # (which may be cut at other places)
+        check(torch.where(kept[:, None, None], got, want)[:total], q[:total], k, v, masks, lens, 0.125, "kept")
+
+
 @pytest.mark.parametrize("dtype", [BF16, F32])
 @pytest.mark.parametrize("shift", [0, 1])
 def test_strides(dtype, shift):
