@@ -116,6 +116,16 @@ def test_cache_refusals(change, rc):
         assert lib.fr_hip_tree_workspace(C.addressof(r)) == 0
 
 
+def test_trees_of_too_many_blocks_are_refused():
+    """Places of 16 tokens and a head are numbered by 32 bits, the last number for none."""
+    no_engine()
+    lib = fa.lib()
+    for pages, heads, rc in ((1 << 24, 64, fa.UNSUPPORTED), ((1 << 24) - 1, 64, fa.STATE)):
+        r = tree_request(cache_request(pages=pages, heads=heads, page=64), heads=heads)
+        assert lib.fr_hip_kv_attend_tree(C.addressof(r), None, 0, None) == rc
+        assert lib.fr_hip_tree_workspace(C.addressof(r)) == 0
+
+
 @pytest.mark.parametrize("change,rc", [
     (dict(source=None), fa.INVALID), (dict(target=None), fa.INVALID), (dict(groups=1 << 31, moves=1), fa.INVALID),
     (dict(moves=65), fa.UNSUPPORTED), (dict(groups=1 << 23, moves=1), fa.UNSUPPORTED), (dict(moves=64), fa.STATE),
