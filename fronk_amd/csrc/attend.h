@@ -90,6 +90,9 @@ template <typename T> __device__ __forceinline__ void put4(T* p, float4v x, floa
   }
 }
 
+// A stretch's sums, for another kernel: not kept in this die's L2, which would have to be
+// written out when the kernel ends.
+__device__ __forceinline__ void part_store(float* to, float4v x) { __builtin_nontemporal_store(x, reinterpret_cast<float4v*>(to)); }
 // Four dims of a row from its stretches, joined in their order; `part` is the row's
 // place in the first, of `block_rows`. Few stretches: D / 4 lanes a row.
 template <int D>
@@ -111,12 +114,17 @@ __device__ __forceinline__ float4v join_few(const float* part_o, const float* pa
 // Up to 256 of them: a workgroup of 256 a row; the first D / 4 threads have the result.
 template <int D>
 __device__ __forceinline__ float4v join_many(const float* part_o, const float* part_ml, size_t part, uint32_t splits, uint32_t block_rows, float* sum) {
-  constexpr uint32_t L = D / 4, G = 256 / L;
+  constexpr uint32_t L = D / 4, G = 256 / L, kFirst = 16;
   __shared__ float weight[256], red[2][4];
   __shared__ float4v parts[G][L];
   const uint32_t s = threadIdx.x, c = s % L, g = s / L;
   const float m = s < splits ? part_ml[(part + (size_t)s * block_rows) * 2] : -INFINITY;
   const float l = s < splits ? part_ml[(part + (size_t)s * block_rows) * 2 + 1] : 0.f;
+  // The first values are under way while their weights are found.
+  float4v y[kFirst];
+#pragma unroll
+  for (uint32_t j = 0; j < kFirst; ++j)
+    y[j] = *reinterpret_cast<const float4v*>(part_o + (part + (size_t)min(g + j * G, splits - 1) * block_rows) * D + c * 4);
   float top = m;
   for (int o = 1; o < 64; o *= 2) top = fmaxf(top, __shfl_xor(top, o));
   if ((s & 63) == 0) red[0][s >> 6] = top;
@@ -131,12 +139,16 @@ __device__ __forceinline__ float4v join_many(const float* part_o, const float* p
   __syncthreads();
   *sum = (red[1][0] + red[1][1]) + (red[1][2] + red[1][3]);
   float4v x = {0, 0, 0, 0};
-#pragma unroll 8
-  for (uint32_t k = g; k < splits; k += G) {
+  auto add = [&](uint32_t k, float4v y) {
     const float f = weight[k];
-    const float4v y = *reinterpret_cast<const float4v*>(part_o + (part + (size_t)k * block_rows) * D + c * 4);
-    if (!(f < 0.f)) x += f * y;   // (else nothing is seen there, and y was not written)
-  }
+    if (!(f < 0.f)) x += f * y;   // (else nothing is seen there, or it is none, and y was not written)
+  };
+#pragma unroll
+  for (uint32_t j = 0; j < kFirst; ++j)
+    if (g + j * G < splits) add(g + j * G, y[j]);
+#pragma unroll 8
+  for (uint32_t k = g + kFirst * G; k < splits; k += G)
+    add(k, *reinterpret_cast<const float4v*>(part_o + (part + (size_t)k * block_rows) * D + c * 4));
   parts[g][c] = x;
   __syncthreads();
   for (uint32_t k = 1; k < G; ++k) x += parts[k][c];   // (by all, for the first group)

@@ -330,8 +330,8 @@ __global__ __launch_bounds__(64 * kWaves, (kResident<T, D>)) void prompt_attend(
     for (int d = 0; d < DT; ++d)
 #pragma unroll
       for (int g = 0; g < 4; ++g)
-        *reinterpret_cast<float4v*>(A.part_o + to * D + d * 32 + g * 8 + 4 * h) =
-            float4v{acc[d][g * 4], acc[d][g * 4 + 1], acc[d][g * 4 + 2], acc[d][g * 4 + 3]};
+        part_store(A.part_o + to * D + d * 32 + g * 8 + 4 * h,
+                   float4v{acc[d][g * 4], acc[d][g * 4 + 1], acc[d][g * 4 + 2], acc[d][g * 4 + 3]});
     return;
   }
   T* const p = output_row<T>(A, P, head, row) + 4 * h;

@@ -461,7 +461,8 @@ __global__ __launch_bounds__((64 * kTreeWaves<T, D, RG>), (kTreeResident<T, D>))
     // Each step's operands are read while the one before it is worked on.
     __builtin_amdgcn_s_setprio(1);   // (matrix work before other wavefronts': 4 % less at 64 rows)
     float16v st[ST];
-    constexpr int kK = KS < 4 ? 1 : 2, kV = DT < 4 ? DT : 4;   // reads at once
+    // Reads at once, as many as registers are left for.
+    constexpr int kK = KS == 4 ? 2 : 1, kV = D == 256 ? 2 : DT < 4 ? DT : 4;
     uint4v kc[2][kK];
     auto read_k = [&](int n) __attribute__((always_inline)) {
 #pragma unroll
@@ -475,6 +476,7 @@ __global__ __launch_bounds__((64 * kTreeWaves<T, D, RG>), (kTreeResident<T, D>))
     for (int n = 0; n < ST * KS / kK; ++n) {
       __builtin_amdgcn_sched_barrier(0);
       if (n + 1 < ST * KS / kK) read_k(n + 1);
+      __builtin_amdgcn_sched_barrier(0);
       const int t = n / (KS / kK);
       if (n % (KS / kK) == 0) st[t] = float16v{};
 #pragma unroll
@@ -561,6 +563,7 @@ __global__ __launch_bounds__((64 * kTreeWaves<T, D, RG>), (kTreeResident<T, D>))
     for (int n = 0; n < 2 * ST * (DT / kV); ++n) {
       __builtin_amdgcn_sched_barrier(0);
       if (n + 1 < 2 * ST * (DT / kV)) read_v(n + 1);
+      __builtin_amdgcn_sched_barrier(0);
       const int s = n / (DT / kV);
 #pragma unroll
       for (int k = 0; k < kV; ++k) {
@@ -643,7 +646,7 @@ __global__ __launch_bounds__((64 * kTreeWaves<T, D, RG>), (kTreeResident<T, D>))
       const float4v x = *reinterpret_cast<const float4v*>(o + r * kPitch + d);
       if (many) {
         if (d == 0) A.part_ml[(part + r) * 2] = stat[r / 32][r % 32][0], A.part_ml[(part + r) * 2 + 1] = total;
-        if (begin < end) *reinterpret_cast<float4v*>(A.part_o + (part + r) * D + d) = x;
+        if (begin < end) part_store(A.part_o + (part + r) * D + d, x);
       } else {
         put4<T>(draft_row<T>(A, P, head, row0 + r) + d, x, total, A.wide);
       }
@@ -659,8 +662,8 @@ __global__ __launch_bounds__((64 * kTreeWaves<T, D, RG>), (kTreeResident<T, D>))
     for (int d = 0; d < DT; ++d)
 #pragma unroll
       for (int g = 0; g < 4; ++g)
-        *reinterpret_cast<float4v*>(A.part_o + to * D + d * 32 + g * 8 + 4 * h) =
-            float4v{acc[d][g * 4], acc[d][g * 4 + 1], acc[d][g * 4 + 2], acc[d][g * 4 + 3]};
+        part_store(A.part_o + to * D + d * 32 + g * 8 + 4 * h,
+                   float4v{acc[d][g * 4], acc[d][g * 4 + 1], acc[d][g * 4 + 2], acc[d][g * 4 + 3]});
     return;
   }
   T* const p = draft_row<T>(A, P, head, row) + 4 * h;
