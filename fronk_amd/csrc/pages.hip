@@ -15,56 +15,63 @@ struct MoveArgs {
   uint32_t groups, moves;
 };
 
-// One workgroup: the K or the V of one head of one group, all of which it reads before
-// it writes any. A move's codes are D / 4 dwords of K, or D single bytes of V, 16
-// apart; N of these are a thread's, in registers.
-template <int D, int N>
+// One workgroup: the K or the V of one head of one group of up to M moves, all of which it
+// reads before it writes any. A move's codes are D / 4 dwords of K, or D single bytes of
+// V, 16 apart; a thread's are in registers, all loaded before the first is waited for.
+//
+// One path of 6 tokens takes 3.4 us (4.8 with its launch), three latencies: the slots, the codes and their exponents,
+// the writes. 128 groups of up to 24 tokens, 8 heads of 128: 11.2 us, bound by V's lines: a
+// token's 128 codes of a head lie in 2 KB, which are fetched and written back for them.
+constexpr size_t kNowhere = ~(size_t)0;
+template <typename T, int U, int APART, int M>
+__device__ __forceinline__ void move_codes(T* codes, const size_t* from, const size_t* to) {
+  constexpr uint32_t N = (M * U + 255) / 256;
+  T held[N];
+  size_t source[N], target[N];
+#pragma unroll
+  for (uint32_t n = 0; n < N; ++n) {
+    const uint32_t u = threadIdx.x + n * 256, move = min(u / U, M - 1u);
+    source[n] = from[move], target[n] = u < M * U ? to[move] : kNowhere;
+  }
+#pragma unroll
+  for (uint32_t n = 0; n < N; ++n)
+    if (target[n] != kNowhere) held[n] = codes[source[n] / sizeof(T) + (threadIdx.x + n * 256) % U * APART];
+  __builtin_amdgcn_s_waitcnt(0x0f70);   // vmcnt(0): all is read
+  __syncthreads();
+#pragma unroll
+  for (uint32_t n = 0; n < N; ++n)
+    if (target[n] != kNowhere) codes[target[n] / sizeof(T) + (threadIdx.x + n * 256) % U * APART] = held[n];
+}
+template <int D, int M>
 __global__ __launch_bounds__(256) void kv_move(MoveArgs A) {
-  __shared__ size_t from[kMoves], to[kMoves];   // of the codes
-  __shared__ size_t from_exp[kMoves], to_exp[kMoves];
-  __shared__ bool moved[kMoves];
+  __shared__ size_t from[M], to[M];   // of the codes
   const Cache& C = A.cache;
   const bool is_v = blockIdx.x & 1;
   const uint32_t head = blockIdx.x / 2 % C.heads, group = blockIdx.x / 2 / C.heads;
-  if (threadIdx.x < A.moves) {
-    const size_t at = (size_t)group * A.moves + threadIdx.x;
-    uint32_t p0 = 0, a0 = 0, p1 = 0, a1 = 0;
-    const int32_t source = A.source[at], target = A.target[at];
-    const int s = fronk::locate(source, C.page, C.pages, &p0, &a0), t = fronk::locate(target, C.page, C.pages, &p1, &a1);
-    if ((s == 2 || t == 2) && A.status) atomicOr(A.status, FR_HIP_BAD_SLOT);
-    const bool there = s == 1 && t == 1;
-    moved[threadIdx.x] = there;
-    const size_t e0 = there ? exp_at(C, p0, head, a0) : 0, e1 = there ? exp_at(C, p1, head, a1) : 0;
-    from_exp[threadIdx.x] = e0, to_exp[threadIdx.x] = e1;
-    from[threadIdx.x] = !there ? 0 : is_v ? v_at(C, p0, head, a0) : e0 * D;
-    to[threadIdx.x] = !there ? 0 : is_v ? v_at(C, p1, head, a1) : e1 * D;
-  }
-  __syncthreads();
   uint8_t* const exponents = is_v ? C.v_exp : C.k_exp;
-  uint32_t held[N], exponent = 0;
-  const bool one = threadIdx.x < A.moves && moved[threadIdx.x];
-  if (one) exponent = exponents[from_exp[threadIdx.x]];
-  const uint32_t units = A.moves * (is_v ? D : D / 4);
-#pragma unroll
-  for (int n = 0; n < N; ++n) {
-    const uint32_t u = threadIdx.x + n * 256;
-    if (u >= units) break;
-    // (what is not moved is read from the cache's first place)
-    held[n] = is_v ? C.v_codes[from[u / D] + u % D * 16] : *reinterpret_cast<const uint32_t*>(C.k_codes + from[u / (D / 4)] + u % (D / 4) * 4);
-  }
-  __builtin_amdgcn_s_waitcnt(0x0f70);   // vmcnt(0): all is read
-  __syncthreads();
-  if (one) exponents[to_exp[threadIdx.x]] = (uint8_t)exponent;
-#pragma unroll
-  for (int n = 0; n < N; ++n) {
-    const uint32_t u = threadIdx.x + n * 256;
-    if (u >= units) break;
-    if (is_v) {
-      if (moved[u / D]) C.v_codes[to[u / D] + u % D * 16] = (uint8_t)held[n];
-    } else if (moved[u / (D / 4)]) {
-      *reinterpret_cast<uint32_t*>(C.k_codes + to[u / (D / 4)] + u % (D / 4) * 4) = held[n];
+  size_t to_exp = 0;
+  uint32_t exponent = 0;
+  bool there = false;
+  if (threadIdx.x < M) {
+    uint32_t p0 = 0, a0 = 0, p1 = 0, a1 = 0;
+    if (threadIdx.x < A.moves) {
+      const size_t at = (size_t)group * A.moves + threadIdx.x;
+      const int32_t source = A.source[at], target = A.target[at];
+      const int s = fronk::locate(source, C.page, C.pages, &p0, &a0), t = fronk::locate(target, C.page, C.pages, &p1, &a1);
+      if ((s == 2 || t == 2) && A.status) atomicOr(A.status, FR_HIP_BAD_SLOT);
+      there = s == 1 && t == 1;
     }
+    const size_t from_exp = there ? exp_at(C, p0, head, a0) : 0;
+    to_exp = there ? exp_at(C, p1, head, a1) : 0;
+    from[threadIdx.x] = !there ? 0 : is_v ? v_at(C, p0, head, a0) : from_exp * D;
+    to[threadIdx.x] = !there ? kNowhere : is_v ? v_at(C, p1, head, a1) : to_exp * D;
+    exponent = exponents[from_exp];
   }
+  __syncthreads();
+  // (Its barrier is also the exponents': they are read by then and not yet written.)
+  if (is_v) move_codes<uint8_t, D, 16, M>(C.v_codes, from, to);
+  else move_codes<uint32_t, D / 4, 1, M>(reinterpret_cast<uint32_t*>(C.k_codes), from, to);
+  if (there) exponents[to_exp] = (uint8_t)exponent;
 }
 
 struct CopyArgs {
@@ -76,7 +83,9 @@ struct CopyArgs {
 constexpr uint32_t kVectors = 8;   // of 16 bytes, a thread
 
 // One workgroup: up to 32 KB of a page, which lies together in each of the cache's four
-// tensors, all loads before the first store.
+// tensors, all loads before the first store. 1024 pages of 64 tokens, two heads of 256 (135 MB
+// read and written): 21.3 us by itself, as part of it stays in the card's 256 MB cache, 30.8 in
+// a row with others, where a copy at its largest rate takes 26.
 __global__ __launch_bounds__(256) void kv_copy(CopyArgs A) {
   const Cache& C = A.cache;
   const uint32_t entry = blockIdx.x / A.parts, part = blockIdx.x % A.parts;
@@ -112,8 +121,11 @@ int check_moves(const fr_hip_kv_cache* c, uint64_t n, const int32_t* source, con
 
 template <int D>
 void launch_move(const MoveArgs& A, uint32_t grid, hipStream_t s) {
-  if (A.moves <= 8) hipLaunchKernelGGL((kv_move<D, D * 8 / 256>), dim3(grid), dim3(256), 0, s, A);
-  else hipLaunchKernelGGL((kv_move<D, D * 64 / 256>), dim3(grid), dim3(256), 0, s, A);
+  // (4 moves of one group take 3.0 us, of 128 groups 5.0, in the kernel for 64 4.0 and 11.1;
+  // 16 moves in that for 32 3.7 and 11.2, in that for 64 4.2 and 13.3)
+  if (A.moves <= 8) hipLaunchKernelGGL((kv_move<D, 8>), dim3(grid), dim3(256), 0, s, A);
+  else if (A.moves <= 32) hipLaunchKernelGGL((kv_move<D, 32>), dim3(grid), dim3(256), 0, s, A);
+  else hipLaunchKernelGGL((kv_move<D, kMoves>), dim3(grid), dim3(256), 0, s, A);
 }
 
 }  // namespace

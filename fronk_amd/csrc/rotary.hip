@@ -24,6 +24,11 @@ struct RotaryArgs {
 // size costs a cosine no more than fp32's rounding. Then one pass over the heads, V
 // elements (16 bytes) a step, or single ones where addresses or sizes are not of
 // whole 16 bytes. What is rotated is read and written by one lane: in place is safe.
+// Results are rounded once, from fp32.
+//
+// Bound by memory: 4096 tokens of 20 interleaved heads of 128 in fp16 (42 MB) take 9.9 us,
+// 4.2 TB/s; a copy of as much takes 9.8 at its largest rate. One token of 18 heads is one
+// workgroup for 3.8 us: position and frequency, the cosine, a head (5.3 with its launch).
 template <typename T, bool INTERLEAVED, int V>
 __global__ __launch_bounds__(256) void rotary(RotaryArgs A) {
   extern __shared__ __attribute__((aligned(16))) float2v turn[];   // [each][pairs]
@@ -131,7 +136,13 @@ extern "C" int fr_hip_rotate(const fr_hip_rotary* r, void* stream) {
   A.each = r->pairs < 256 ? 256 / r->pairs : 1;
   if (A.each > 16) A.each = 16;
   if (A.each > A.tokens && A.tokens) A.each = A.tokens;
-  A.at_once = A.all_heads;
+  // Few tokens: their heads over more workgroups, of 256 steps of 16 bytes or more each (16
+  // tokens of 136 heads of 64: 10 us in two workgroups, 2.9 in ten).
+  const uint32_t groups = (A.tokens + A.each - 1) / A.each, bytes = A.each * A.dim * (uint32_t)elem_size(r->type);
+  const uint32_t most = groups && kUnits > groups ? kUnits / groups : 1, least = (8192 + bytes - 1) / bytes;
+  A.at_once = (A.all_heads + most - 1) / most;
+  if (A.at_once < least) A.at_once = least;
+  if (A.at_once > A.all_heads) A.at_once = A.all_heads;
   const uint64_t grid = A.all_heads ? (uint64_t)((A.tokens + A.each - 1) / A.each) * ((A.all_heads + A.at_once - 1) / A.at_once) : 0;
   if (grid * 256 > UINT32_MAX) return FR_HIP_UNSUPPORTED;
   hipStream_t s;

@@ -201,18 +201,27 @@ template <typename T> __device__ __forceinline__ T* draft_row(const TreeArgs& A,
 }
 
 // One workgroup: one sequence, one cache head, 32 RG of its rows (query heads of that
-// cache head by drafts, draft-major) and one stretch of the context. Its four
-// wavefronts are RG groups of 32 rows by 4 / RG groups of keys; each takes every
-// (4 / RG)-th tile of KT keys. Products and fragments are those of prompt_attend
-// (attend.h), but that codes become operands as they are read from LDS: there they are
-// as the cache has them, S stages of 4 / RG tiles, loaded that far ahead, as a tile's
-// work (0.5 us) is less than a memory's latency. Codes times one are exact in bf16 and
-// fp16; a token's powers of two go to its scores and weights.
+// cache head by drafts, draft-major) and one stretch of the context. Its W wavefronts
+// are RG groups of 32 rows by KG groups of keys; each takes every KG-th tile of KT keys,
+// and the key groups are joined in LDS at the end. Products and fragments are those of
+// prompt_attend (attend.h), but that codes become operands as they are read from LDS:
+// there they are as the cache has them, which halves the bytes of its tiles and reads.
+// Codes times one are exact in bf16 and fp16; a token's powers of two go to its K
+// operand, or its scores (fp16, whose range they may leave), and to its weights.
+//
+// Bound by the vector work of making operands of the codes, masks, exponentials and
+// parts of P, next to as much time of the matrix cores; memory is read at a
+// quarter to a half of its rate. 24 sequences of up to 8192 tokens with 1 to 61 drafts (16 heads
+// of 128, four of the cache, fp16): 60 us and 9.6 for the join; 32 equal ones with 64 drafts in
+// bf16: 178 us, 770 TFLOP/s. One of 32768 tokens with 15 drafts (16 heads of 256, two of the
+// cache, bf16): 28.9 us, of which 8 pass until the first tile is there, 3 with each of four
+// tiles, 4 with the join in LDS and 2 with writing 17 MB of parts, and 5.9 for their join.
 //
 // K in LDS: [token][dim], chunk c of 16 codes at another place for each of eight
 // tokens, so that a read of one chunk of 32 of them goes to all banks; a lane's 16
 // codes are operands of two steps (Q is laid out alike). V: [block of 16 tokens][dim]
-// [16 tokens], a half's lanes hold weights of tokens 0-3 and 8-11, or 4-7 and 12-15.
+// [16 tokens]; rows of K's operand are tokens in an order that leaves a lane of half h with
+// the weights of tokens 16 s + 8 h .. 16 s + 8 h + 7, eight bytes of V.
 //
 // Q is an exact operand (fp32: three bf16 parts); P 2^e is in bf16 parts, of which there
 // are as many as keep it well below the output's own rounding but for bf16, where
@@ -236,7 +245,9 @@ template <> struct Row<float> {
 
 // Wavefronts, keys of a tile, stages, wavefronts a SIMD that the registers are for.
 // Where Q's three parts do not fit them beside the sums, Q is kept in LDS, and split
-// where it is used.
+// where it is used. Two stages: with three, one workgroup less fits a unit (32 sequences of
+// 8192 tokens, dim 128: 207 us with two, 264 with three); tiles of 32 keys instead of 64 there:
+// 217. Eight wavefronts at dim 256, as four of 512 registers each are slower (40 us for 37).
 template <typename T, int D> constexpr bool kTreeQInLds = D * sizeof(T) > 512;
 template <typename T, int D, int RG> constexpr int kTreeWaves = kTreeQInLds<T, D> ? 2 : D == 256 && RG > 1 ? 8 : 4;
 template <int D, int RG> constexpr int kTreeKeys = D == 256 || (D == 128 && RG == 1) ? 32 : 64;
@@ -725,7 +736,9 @@ TreeCut tree_cut(const fr_hip_kv_tree* r) {
   TreeCut c;
   const uint32_t drafts = r->max_tokens < r->tokens ? r->max_tokens : r->tokens;
   const uint32_t rows = drafts * (r->heads / r->cache.heads);
-  // 64 rows, or 32 where there are no more (128: the same to 20 % slower at 16 to 64 drafts).
+  // 64 rows, or 32 where there are no more: 16 sequences of 8192 tokens with 8 drafts of four
+  // heads take 39.8 us in groups of 32 and 42.2 of 64, with 16 drafts 48.1 and 46.4, 32 of them
+  // with 64 drafts 240 and 178 (128 rows: the same to 20 % slower at 16 to 64 drafts).
   c.groups = rows <= 32 ? 1 : 2;
   c.blocks = (rows + 32 * c.groups - 1) / (32 * c.groups);
   c.items = (uint64_t)c.blocks * r->sequences * r->cache.heads;
