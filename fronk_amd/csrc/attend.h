@@ -94,14 +94,15 @@ template <typename T> __device__ __forceinline__ void put4(T* p, float4v x, floa
 // written out when the kernel ends.
 __device__ __forceinline__ void part_store(float* to, float4v x) { __builtin_nontemporal_store(x, reinterpret_cast<float4v*>(to)); }
 // Four dims of a row from its stretches, joined in their order; `part` is the row's
-// place in the first, of `block_rows`. Few stretches: D / 4 lanes a row.
+// place in the first, of `block_rows`. Many rows: D / 4 lanes each.
 template <int D>
 __device__ __forceinline__ float4v join_few(const float* part_o, const float* part_ml, size_t part, uint32_t splits, uint32_t block_rows, float* sum) {
   const uint32_t d = threadIdx.x % (D / 4) * 4;
   float top = -INFINITY, total = 0;
+#pragma unroll 8
   for (uint32_t s = 0; s < splits; ++s) top = fmaxf(top, part_ml[(part + (size_t)s * block_rows) * 2]);
   float4v x = {0, 0, 0, 0};
-#pragma unroll 4
+#pragma unroll 8
   for (uint32_t s = 0; s < splits; ++s) {
     const size_t at = part + (size_t)s * block_rows;
     const float shift = part_ml[at * 2], l = part_ml[at * 2 + 1], w = __builtin_amdgcn_exp2f(shift - top);
@@ -111,7 +112,7 @@ __device__ __forceinline__ float4v join_few(const float* part_o, const float* pa
   *sum = total;
   return x;
 }
-// Up to 256 of them: a workgroup of 256 a row; the first D / 4 threads have the result.
+// Up to 256 stretches of few rows: a workgroup of 256 a row; the first D / 4 threads have the result.
 template <int D>
 __device__ __forceinline__ float4v join_many(const float* part_o, const float* part_ml, size_t part, uint32_t splits, uint32_t block_rows, float* sum) {
   constexpr uint32_t L = D / 4, G = 256 / L, kFirst = 16;
@@ -154,6 +155,9 @@ __device__ __forceinline__ float4v join_many(const float* part_o, const float* p
   for (uint32_t k = 1; k < G; ++k) x += parts[k][c];   // (by all, for the first group)
   return x;
 }
-constexpr uint32_t kFewSplits = 4;
+// Rows below which each has a workgroup (join_many). Whole calls, us, by a workgroup each and by
+// D / 4 lanes each: 1024 rows of 64 stretches 37 and 72, 2048 45 and 59, 4096 63 and 63, 8192
+// rows of eight 103 and 87.
+constexpr uint64_t kJoinRows = 4096;
 
 }  // namespace

@@ -429,7 +429,7 @@ int launch_prompt(const PromptArgs& A, const PromptCut& c, hipStream_t s) {
   static fronk::Devices done;
   if (allow_lds(prompt_attend<T, D, WIDE>, kLds, &done)) return FR_HIP_IO;
   hipLaunchKernelGGL((prompt_attend<T, D, WIDE>), dim3((uint32_t)(c.items * c.splits)), dim3(64 * kWaves), kLds, s, A);
-  if (c.splits > kFewSplits)
+  if (c.splits > 1 && c.items * R < kJoinRows)
     hipLaunchKernelGGL((prompt_merge<T, D, WIDE, true>), dim3((uint32_t)(c.items * R)), dim3(256), 0, s, A);
   else if (c.splits > 1)
     hipLaunchKernelGGL((prompt_merge<T, D, WIDE, false>), dim3((uint32_t)(c.items * R / (1024 / D))), dim3(256), 0, s, A);

@@ -767,8 +767,7 @@ int launch_dim(const TreeArgs& A, const TreeCut& c, hipStream_t s) {
   const int rc = c.groups == 1 ? launch_tree<T, D, 1>(A, c, s) : launch_tree<T, D, 2>(A, c, s);
   if (rc) return rc;
   const uint32_t rows = 32 * c.groups;
-  // A workgroup a row where there are few (8000 of them take 29 us, those of 8 rows 9).
-  if (c.slots && c.items * rows <= 2048) hipLaunchKernelGGL((tree_merge<T, D, true>), dim3((uint32_t)(c.items * rows)), dim3(256), 0, s, A, rows);
+  if (c.slots && c.items * rows < kJoinRows) hipLaunchKernelGGL((tree_merge<T, D, true>), dim3((uint32_t)(c.items * rows)), dim3(256), 0, s, A, rows);
   else if (c.slots) hipLaunchKernelGGL((tree_merge<T, D, false>), dim3((uint32_t)(c.items * rows / (1024 / D))), dim3(256), 0, s, A, rows);
   FRONK_CK(hipGetLastError());
   return FR_HIP_OK;

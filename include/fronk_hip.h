@@ -458,7 +458,9 @@ int fr_hip_prompt_attend(const fr_hip_prompt *req, void *workspace, size_t bytes
  * outside the cache counts as not seen. o shares no memory with an input.
  * What is held of drafts that no draft sees may be anything. A draft held with infinity or
  * NaN makes the drafts that see it NaN, and no others. bf16 outputs: weights are rounded to
- * bf16, their sums are not. */
+ * bf16, their sums are not (fp16: to 2^-16, fp32: to 2^-23). How a context is cut, and so
+ * the order of sums, follows the lengths of all sequences of the call. Caches of 2^32 - 1
+ * or more blocks of 16 tokens and a head are not supported. */
 typedef struct {
     fr_hip_kv_cache cache;
     unsigned sequences, tokens, max_tokens, heads, max_context, type, table_stride;
