@@ -19,9 +19,10 @@ struct MoveArgs {
 // reads before it writes any. A move's codes are D / 4 dwords of K, or D single bytes of
 // V, 16 apart; a thread's are in registers, all loaded before the first is waited for.
 //
-// One path of 6 tokens takes 3.4 us (4.8 with its launch), three latencies: the slots, the codes and their exponents,
-// the writes. 128 groups of up to 24 tokens, 8 heads of 128: 11.2 us, bound by V's lines: a
-// token's 128 codes of a head lie in 2 KB, which are fetched and written back for them.
+// One path of 6 tokens takes 3.4 us (4.8 with its launch), three latencies: the slots, the
+// codes and their exponents, the writes. 128 groups of up to 24 tokens, 8 heads of 128: 11.2
+// us, bound by V's lines: a token's 128 codes of a head lie in 2 KB, which are fetched
+// and written back for them.
 constexpr size_t kNowhere = ~(size_t)0;
 template <typename T, int U, int APART, int M>
 __device__ __forceinline__ void move_codes(T* codes, const size_t* from, const size_t* to) {

@@ -64,8 +64,9 @@ template <typename T> __device__ __forceinline__ T* output_row(const PromptArgs&
 // 256 over two key heads, bf16, take 159 us or 860 TFLOP/s of what is seen, 7 prompts of
 // up to 1531 tokens (20 heads of 128, fp16) 36 us. 128 rows share what a tile of keys takes
 // to load. The running maximum is let stay while no weight would pass 2^8, which saves
-// rescaling the sums at nearly every tile. Steps of both products are interleaved with the LDS reads of the one after next
-// (schedule), and matrix work goes before other wavefronts' vector work.
+// rescaling the sums at nearly every tile. Steps of both products are interleaved with the
+// LDS reads of the one after next (schedule), and matrix work goes before other
+// wavefronts' vector work.
 // Keys of a tile, and workgroups a compute unit that the registers are for.
 template <typename T, int D> constexpr int kKeys = sizeof(T) == 4 || D > 64 ? 32 : 64;
 template <typename T, int D> constexpr int kResident = D * sizeof(T) > 512 ? 1 : sizeof(T) == 2 && D == 128 ? 3 : 2;
