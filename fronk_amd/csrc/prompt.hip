@@ -395,10 +395,11 @@ PromptCut prompt_cut(const fr_hip_prompt* r) {
   const uint32_t context = r->max_context < r->k_tokens ? r->max_context : r->k_tokens;
   c.blocks = (uint32_t)(((uint64_t)tokens * (r->heads / r->kv_heads) + R - 1) / R);
   c.items = (uint64_t)c.blocks * r->sequences * r->kv_heads;
-  // Two workgroups for each of 256 compute units, none with less than 256 keys (512 tokens
-  // over 8192 keys, 32 heads of 128 over four: 77 us and 12 for the join of four stretches,
-  // 175 in one).
-  const uint64_t want = c.items ? 2 * kUnits / c.items : 1, most = (context + 255) / 256;
+  // Two workgroups for each of 256 compute units, at dim 256 one, which is what runs at once;
+  // none with less than 256 keys. 512 tokens over 8192 keys, 32 heads of 128 over four: 86 us
+  // with the join of four stretches, 177 in one, 106 in two, 90 in six; 128 tokens of 16 heads of
+  // 256 over two: 44 with one workgroup a unit, 57 with two, 53 with a half.
+  const uint64_t want = c.items ? (r->dim == 256 ? 1 : 2) * kUnits / c.items : 1, most = (context + 255) / 256;
   uint64_t n = want < most ? want : most;
   n = n < 1 ? 1 : n > 64 ? 64 : n;
   c.chunk = (uint32_t)((context + n * 64 - 1) / (n * 64)) * 64;
