@@ -97,18 +97,30 @@ __device__ __forceinline__ void part_store(float* to, float4v x) { __builtin_non
 // place in the first, of `block_rows`. Many rows: D / 4 lanes each.
 template <int D>
 __device__ __forceinline__ float4v join_few(const float* part_o, const float* part_ml, size_t part, uint32_t splits, uint32_t block_rows, float* sum) {
+  constexpr uint32_t kFirst = 4;
   const uint32_t d = threadIdx.x % (D / 4) * 4;
+  auto value = [&](uint32_t s) { return *reinterpret_cast<const float4v*>(part_o + (part + (size_t)s * block_rows) * D + d); };
+  auto of = [&](uint32_t s) { return *reinterpret_cast<const float2v*>(part_ml + (part + (size_t)s * block_rows) * 2); };
+  // The first ones are under way at once.
+  float4v y[kFirst];
+  float2v ml[kFirst];
+#pragma unroll
+  for (uint32_t s = 0; s < kFirst; ++s) y[s] = value(min(s, splits - 1)), ml[s] = of(min(s, splits - 1));
   float top = -INFINITY, total = 0;
+#pragma unroll
+  for (uint32_t s = 0; s < kFirst; ++s) top = fmaxf(top, ml[s][0]);
 #pragma unroll 8
-  for (uint32_t s = 0; s < splits; ++s) top = fmaxf(top, part_ml[(part + (size_t)s * block_rows) * 2]);
+  for (uint32_t s = kFirst; s < splits; ++s) top = fmaxf(top, of(s)[0]);
   float4v x = {0, 0, 0, 0};
+  auto add = [&](float2v ml, float4v y) {
+    const float w = __builtin_amdgcn_exp2f(ml[0] - top);
+    if (ml[0] != -INFINITY) total += w * ml[1], x += w * y;   // (else nothing is seen there, and y was not written)
+  };
+#pragma unroll
+  for (uint32_t s = 0; s < kFirst; ++s)
+    if (s < splits) add(ml[s], y[s]);
 #pragma unroll 8
-  for (uint32_t s = 0; s < splits; ++s) {
-    const size_t at = part + (size_t)s * block_rows;
-    const float shift = part_ml[at * 2], l = part_ml[at * 2 + 1], w = __builtin_amdgcn_exp2f(shift - top);
-    const float4v y = *reinterpret_cast<const float4v*>(part_o + at * D + d);
-    if (shift != -INFINITY) total += w * l, x += w * y;   // (else nothing is seen there, and y was not written)
-  }
+  for (uint32_t s = kFirst; s < splits; ++s) add(of(s), value(s));
   *sum = total;
   return x;
 }

@@ -693,9 +693,9 @@ __global__ __launch_bounds__(256) void tree_merge(TreeArgs A, uint32_t block_row
   const uint32_t item = blockIdx.x / parts, r = blockIdx.x % parts * kAtOnce + (MANY ? 0 : threadIdx.x / L);
   const uint32_t head = item % A.cache.heads, block = item / A.cache.heads % A.blocks, seq = item / A.cache.heads / A.blocks;
   const uint2v plan = A.plan[seq];
-  if (plan[1] < 2) return;   // (written as it is)
   Drafts W = {(int32_t)(seq * A.max_tokens), A.max_tokens, 0, 0};
   if (A.offsets) W.q0 = A.offsets[seq], W.n = A.offsets[seq + 1] - W.q0;
+  if (plan[1] < 2) return;   // (written as it is)
   const uint32_t row = block * block_rows + r, rows = W.n * A.per;
   if (row >= rows) return;
   float sum;
