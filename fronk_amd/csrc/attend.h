@@ -168,8 +168,8 @@ __device__ __forceinline__ float4v join_many(const float* part_o, const float* p
   return x;
 }
 // Rows below which each has a workgroup (join_many). Whole calls, us, by a workgroup each and by
-// D / 4 lanes each: 1024 rows of 64 stretches 37 and 72, 2048 45 and 59, 4096 63 and 63, 8192
-// rows of eight 103 and 87.
-constexpr uint64_t kJoinRows = 4096;
+// D / 4 lanes each: 512 rows of 64 stretches 26 and 36, 1024 of them 37 and 44, 2048 of 32
+// 46 and 46, 4096 of 16 64 and 58, 8192 of eight 106 and 87.
+constexpr uint64_t kJoinRows = 2048;
 
 }  // namespace

@@ -58,7 +58,7 @@ constexpr uint32_t kPlanBytes = (kPlanned * 6 + 8 * 64 + 4) * 4;
 // in rounds of as many as run at once, end first; a workgroup's beginning and end take as
 // long as about 300 tokens. Work then varies by less than two between workgroups however
 // ragged the batch is: 24 sequences of 1 to 61 drafts and up to 8192 tokens (16 heads of 128,
-// four of the cache) take 64 us, with one stretch length from the host 117, 96 of them in bf16
+// four of the cache) take 63 us, with one stretch length from the host 117, 96 of them in bf16
 // 184 and 289; 32 equal ones of 1024 tokens, for which nothing is to be found, 38 and 35.
 // Workgroups of one stretch (its row blocks) follow each other, and each die, to which
 // every eighth goes, has an eighth of the list: its L2 has the stretch for all of them.
@@ -212,7 +212,7 @@ template <typename T> __device__ __forceinline__ T* draft_row(const TreeArgs& A,
 // Bound by the vector work of making operands of the codes, masks, exponentials and
 // parts of P, next to as much time of the matrix cores; memory is read at a
 // quarter to a half of its rate. 24 sequences of up to 8192 tokens with 1 to 61 drafts (16 heads
-// of 128, four of the cache, fp16): 60 us and 9.6 for the join; 32 equal ones with 64 drafts in
+// of 128, four of the cache, fp16): 60 us and 6.1 for the join; 32 equal ones with 64 drafts in
 // bf16: 178 us, 770 TFLOP/s. One of 32768 tokens with 15 drafts (16 heads of 256, two of the
 // cache, bf16): 28.9 us, of which 8 pass until the first tile is there, 3 with each of four
 // tiles, 4 with the join in LDS and 2 with writing 17 MB of parts, and 5.9 for their join.
