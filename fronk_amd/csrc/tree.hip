@@ -56,13 +56,14 @@ constexpr uint32_t kPlanBytes = (kPlanned * 6 + 8 * 64 + 4) * 4;
 // (the host does not know them): stretches of all sequences are no longer than one bound,
 // for which 64 values are tried, a lane each, and that is taken with which the workgroups,
 // in rounds of as many as run at once, end first; a workgroup's beginning and end take as
-// long as about 300 tokens. Work then varies by less than two between workgroups however
+// long as about 300 tokens, and more where two share a unit (one stream of 32768 tokens and 16
+// drafts, dim 128: 21.6 us in 256 workgroups, 25.2 in 512; of 131072 42.4 and 40.1). Work then varies by less than two between workgroups however
 // ragged the batch is: 24 sequences of 1 to 61 drafts and up to 8192 tokens (16 heads of 128,
 // four of the cache) take 63 us, with one stretch length from the host 117, 96 of them in bf16
 // 184 and 289; 32 equal ones of 1024 tokens, for which nothing is to be found, 38 and 35.
 // Workgroups of one stretch (its row blocks) follow each other, and each die, to which
 // every eighth goes, has an eighth of the list: its L2 has the stretch for all of them.
-template <int W, int ROWS>
+template <int W, int ROWS, int D>
 __device__ __forceinline__ Place plan(const TreeArgs& A, uint32_t* lds) {
   Place p;
   const uint32_t heads = A.cache.heads, die = blockIdx.x % 8, nth = blockIdx.x / 8, tid = threadIdx.x;
@@ -75,6 +76,13 @@ __device__ __forceinline__ Place plan(const TreeArgs& A, uint32_t* lds) {
     p.block = local % blocks, p.head = local / blocks % heads, p.split = local / blocks / heads;
     p.chunk = ((p.d.length + p.splits - 1) / p.splits + 63) & ~63u;
   };
+  // What `total` workgroups of `chunk` tokens take, in 64 tokens of one that has a unit to
+  // itself. Two on a unit take 1.5 times as long, and begin and end for longer.
+  auto cost = [&](uint32_t total, uint32_t chunk) {
+    const uint32_t rounds = (total + A.at_once - 1) / A.at_once, c = chunk / 64;
+    if (D == 256) return rounds * (c + 5);
+    return 2 * total <= A.at_once ? c + 5 : rounds * (c + c / 2 + 5) + (D == 64 ? 2 : 5);
+  };
   if (A.sequences > kPlanned) {   // nothing is split
     p.part = in_list(A.sequences * heads * A.blocks);
     if (p.part == ~0u) return p;
@@ -85,14 +93,22 @@ __device__ __forceinline__ Place plan(const TreeArgs& A, uint32_t* lds) {
     if (p.d.bad == FR_HIP_BAD_OFFSET || p.block * ROWS >= p.d.n * A.per) p.part = ~0u;
     return p;
   }
-  if (A.sequences == 1) {         // as many stretches as there may be workgroups
+  if (A.sequences == 1) {         // as many stretches as there may be workgroups, or as units
     p.seq = 0, p.d = drafts_of(A, 0);
     if (p.d.bad && A.status && blockIdx.x == 0 && tid == 0) atomicOr(A.status, p.d.bad);
     const uint32_t blocks = p.d.bad == FR_HIP_BAD_OFFSET ? 0 : (p.d.n * A.per + ROWS - 1) / ROWS, work = blocks * heads;
     p.splits = 1;
     if (work && 2 * work <= A.slots) {
-      const uint32_t n = min(A.slots / work, 256u), chunk = max((p.d.length / n + 64) & ~63u, 256u);
-      p.splits = max((p.d.length + chunk - 1) / chunk, 1u);
+      auto stretches = [&](uint32_t n, uint32_t* chunk) {
+        *chunk = max((p.d.length / n + 64) & ~63u, 256u);
+        return max((p.d.length + *chunk - 1) / *chunk, 1u);
+      };
+      uint32_t chunk, other;
+      p.splits = stretches(min(A.slots / work, 256u), &chunk);
+      if (D < 256 && 2 * work <= A.at_once) {
+        const uint32_t fewer = stretches(min(A.at_once / 2 / work, 256u), &other);
+        if (cost(work * fewer, other) <= cost(work * p.splits, chunk)) p.splits = fewer;
+      }
     }
     if (blockIdx.x == 0 && tid == 0 && A.slots) A.plan[0] = uint2v{0, p.splits};
     p.part = in_list(work * p.splits);
@@ -157,8 +173,8 @@ __device__ __forceinline__ Place plan(const TreeArgs& A, uint32_t* lds) {
     for (int w = 0; w < W; ++w) total += sums[w * 64 + lane];
     total *= heads;
     // (in 64 tokens; what has too many workgroups, or stretches beyond all use, comes last)
-    const uint32_t most = (1u << 26) - 1, rounds = (total + A.at_once - 1) / A.at_once;
-    uint32_t best = (total <= A.slots ? min(rounds * (mine / 64 + 5), most) : most) << 6 | lane;
+    const uint32_t most = (1u << 26) - 1;
+    uint32_t best = (total <= A.slots ? min(cost(total, mine), most) : most) << 6 | lane;
 #pragma unroll
     for (int o = 1; o < 64; o *= 2) best = min(best, (uint32_t)__shfl_xor((int)best, o));
     chunk = __shfl((int)mine, (int)(best & 63));
@@ -291,7 +307,7 @@ __global__ __launch_bounds__((64 * kTreeWaves<T, D, RG>), (kTreeResident<T, D>))
   const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), rg = wave % RG, kg = wave / RG;
   const Cache& C = A.cache;
   static_assert(kTreeLds<T, D, RG> >= kPlanBytes, "the plan is made in the tiles' place");
-  const Place place = plan<W, kRows>(A, reinterpret_cast<uint32_t*>(lds));
+  const Place place = plan<W, kRows, D>(A, reinterpret_cast<uint32_t*>(lds));
   if (place.part == ~0u) return;
   const Drafts P = place.d;
   const uint32_t seq = place.seq, head = place.head, block = place.block;
