@@ -26,8 +26,8 @@ struct RotaryArgs {
 // whole 16 bytes. What is rotated is read and written by one lane: in place is safe.
 // Results are rounded once, from fp32.
 //
-// Bound by memory: 4096 tokens of 20 interleaved heads of 128 in fp16 (42 MB) take 9.9 us,
-// 4.2 TB/s; a copy of as much takes 9.8 at its largest rate. One token of 18 heads is one
+// Bound by memory: 4096 tokens of 24 interleaved heads of 128 in fp16 (50 MB) take 9.9 us,
+// 5.1 TB/s, as a large copy does. One token of 18 heads is one
 // workgroup for 3.8 us: position and frequency, the cosine, a head (5.3 with its launch).
 template <typename T, bool INTERLEAVED, int V>
 __global__ __launch_bounds__(256) void rotary(RotaryArgs A) {
