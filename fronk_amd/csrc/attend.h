@@ -64,12 +64,12 @@ template <int N> __device__ __forceinline__ void loads_done() {
   asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
 }
 
-// N operands of READS reads each, one matrix instruction each: kAhead ahead.
-template <int N, int READS, int kAhead> __device__ __forceinline__ void schedule() {
+// N operands of READS reads each, for EACH matrix instructions: kAhead ahead.
+template <int N, int READS, int kAhead, int EACH = 1> __device__ __forceinline__ void schedule() {
   __builtin_amdgcn_sched_group_barrier(0x100, kAhead * READS, 0);
 #pragma unroll
   for (int n = 0; n < N; ++n) {
-    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+    __builtin_amdgcn_sched_group_barrier(0x008, EACH, 0);
     if (n + kAhead < N) __builtin_amdgcn_sched_group_barrier(0x100, READS, 0);
   }
   __builtin_amdgcn_sched_barrier(0);

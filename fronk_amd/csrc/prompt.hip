@@ -54,39 +54,51 @@ template <typename T> __device__ __forceinline__ T* output_row(const PromptArgs&
 // second's operand where it stands: register r of a lane in half h is key
 // 8 (r / 4) + 4 h + r % 4 of 32, and V^T's operand is read in that order.
 //
-// 16-bit types: v_mfma_f32_32x32x16, eight values a lane; fp32: v_mfma_f32_32x32x2,
-// exact products. P is rounded to the values' type (the sum is not): half a step
-// of it at each weight, as independent errors no more than what the output's own
-// rounding makes.
+// 16-bit types: v_mfma_f32_32x32x16, eight values a lane, with P in two parts (Weights);
+// fp32: v_mfma_f32_32x32x2, exact products.
 //
 // Bound by the matrix cores and by the vector work beside them (per 32 x 32 scores a
-// maximum, 16 exponentials a lane, their sum and P's rounding): 4096 tokens of 16 heads of
-// 256 over two key heads, bf16, take 159 us or 860 TFLOP/s of what is seen, 7 prompts of
-// up to 1531 tokens (20 heads of 128, fp16) 36 us. 128 rows share what a tile of keys takes
-// to load. The running maximum is let stay while no weight would pass 2^8, which saves
-// rescaling the sums at nearly every tile. Steps of both products are interleaved with the
+// maximum, 16 exponentials a lane, their sum and P's parts): 4096 tokens of 16 heads of
+// 256 over two key heads, bf16, take 213 us or 640 TFLOP/s of what is seen (960 of what is
+// multiplied), eight prompts of 1 to 1531 tokens (20 heads of 128 over four) 112 us in fp16
+// and 105 in bf16; in fp32 2048 tokens of 16 heads 141 us at dim 64, 264 at 128 (four key
+// heads), 550 at 256 (two). 128 rows share what a tile of keys takes to load. The running
+// maximum is let stay while no weight would pass 2^8, which saves rescaling the sums at nearly every tile. Steps of both products are interleaved with the
 // LDS reads of the one after next (schedule), and matrix work goes before other
 // wavefronts' vector work.
 // Keys of a tile, and workgroups a compute unit that the registers are for.
 template <typename T, int D> constexpr int kKeys = sizeof(T) == 4 || D > 64 ? 32 : 64;
 template <typename T, int D> constexpr int kResident = D * sizeof(T) > 512 ? 1 : sizeof(T) == 2 && D == 128 ? 3 : 2;
 
-// Weights' range. A half has no bits for what is far below a row's largest weight, though
+// How weights are held. Parts: with P rounded to 16 bits once, outputs are off by about as
+// much again as their own rounding makes, and by far more where values nearly cancel. A
+// second part leaves 2^-16 of a weight in bf16, 2^-22 in fp16, and outputs off by their
+// rounding alone: against 64 bits (relative, 512 tokens over 8192 keys of 128) 0.00165 in
+// bf16 for 0.00223 with one part, 0.00021 in fp16 for 0.00028. It is half as many products
+// again: those 512 tokens take 116 us for 87, 4096 of 16 heads of 256 213 for 165.
+//
+// Range: a half has no bits for what is far below a row's largest weight, though
 // thousands of such keys may be all that a row gets (the largest one's value being zero). So
 // in fp16 a row's largest weight of each tile is kept within 1 and 2^15, and set to 2^kBias
 // when it leaves that: what weights are taken from goes down again where a tile's scores
 // are all lower. A weight is then off by 2^-25 of its tile's largest beside its
 // rounding. Down by 2^60 at most from the row's largest, which leaves the sums in fp32
 // (2^75 of a weight, 2^16 of a value and 2^31 keys are 2^122); keys yet lower add nothing
-// that a half holds. It takes 1 to 2 % of a call (4096 tokens of 16 heads of 256 over two:
-// 177 us for 174, seven prompts of 766 tokens, 20 heads of 128: 37.6 for 37.1).
+// that a half holds. It takes 1 to 2 % of a call.
 template <typename T> struct Weights {
+  static constexpr int kParts = 2;
   static constexpr bool kDown = false;
   static constexpr float kBias = 0.f;
 };
 template <> struct Weights<_Float16> {
+  static constexpr int kParts = 2;
   static constexpr bool kDown = true;
   static constexpr float kBias = 7.f;
+};
+template <> struct Weights<float> {
+  static constexpr int kParts = 1;
+  static constexpr bool kDown = false;
+  static constexpr float kBias = 0.f;
 };
 
 // WIDE: rows begin at multiples of 16 bytes.
@@ -266,7 +278,7 @@ __global__ __launch_bounds__(64 * kWaves, (kResident<T, D>)) void prompt_attend(
     }
     __builtin_amdgcn_s_setprio(0);
     __builtin_amdgcn_sched_barrier(0);
-    frag pf[ST][PS];
+    frag pf[ST][PS][W::kParts];
     float total[4] = {};
 #pragma unroll
     for (int t = 0; t < ST; ++t)
@@ -274,7 +286,12 @@ __global__ __launch_bounds__(64 * kWaves, (kResident<T, D>)) void prompt_attend(
       for (int r = 0; r < 16; ++r) {
         const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(st[t][r], scale, -shift));
         total[r % 4] += p;
-        pf[t][r / kEach][r % kEach] = (T)p;
+        float rest = p;
+#pragma unroll
+        for (int n = 0; n < W::kParts; ++n) {
+          const T part = (T)rest;
+          pf[t][r / kEach][n][r % kEach] = part, rest -= (float)part;
+        }
       }
     sum += (total[0] + total[1]) + (total[2] + total[3]);
     __builtin_amdgcn_s_setprio(1);
@@ -297,9 +314,10 @@ __global__ __launch_bounds__(64 * kWaves, (kResident<T, D>)) void prompt_attend(
             for (int e = 0; e < 4; ++e)
               a[e] = *reinterpret_cast<const float*>(tile + v_at[e] + (t * 32 + s * 8) * kRow + d * 128);
           }
-          acc[d] = mma32(a, pf[t][s], acc[d]);
+#pragma unroll
+          for (int n = W::kParts - 1; n >= 0; --n) acc[d] = mma32(a, pf[t][s][n], acc[d]);
         }
-    schedule<ST * PS * DT, sizeof(T) == 2 ? 2 : 4, 3>();
+    schedule<ST * PS * DT, sizeof(T) == 2 ? 2 : 4, 3, W::kParts>();
   };
 
   // A value that is not finite times a weight of zero is NaN, also in rows that do

@@ -431,9 +431,8 @@ int fr_hip_rotate(const fr_hip_rotary *req, void *stream);
  * or 256. o shares no memory with an input.
  * A value (v) that is not finite makes its dim not finite (NaN or infinity) in the queries that
  * see it, and in no others; a key that is not finite may make all of theirs NaN.
- * Weights are rounded to `type`, their sums are not; in fp16 a weight is off by no more than
- * 2^-25 of the largest of the 32 or 64 keys around it beside that, however far it is below the row's
- * largest. */
+ * Weights are held to 2^-16 of them in bf16, to 2^-22 in fp16 (and there 2^-25 of the largest
+ * of the 32 or 64 keys around, however far they are below the row's largest), their sums in fp32. */
 typedef struct {
     unsigned sequences, tokens, k_tokens, max_tokens, max_context;
     unsigned heads, kv_heads, dim, type;

@@ -1,5 +1,6 @@
 """Weights of prompt attention: those far below a row's largest, which in fp16 would
-leave the range of a half, one after the other in every order."""
+leave the range of a half, one after the other in every order, and the bits that
+weights keep beside the outputs' own rounding."""
 import math
 
 import pytest
@@ -24,11 +25,12 @@ def lines(scores, heads, dim, rows, dtype):
     return q.to(dtype), k.to(dtype)
 
 
-def check(q, k, v, weights, scale=1.0, tile=0.0, **kw):
+def check(q, k, v, weights, scale=1.0, tile=0.0, aligned=True):
     """Outputs against 64 bits: their own rounding (fp16: at least half of 2^-24), `weights`
     of each weight, fp32's share as attend_tolerance has it, and of the largest value `tile`
     and, for each key, the 2^-126 below which an exponential in 32 bits is zero."""
-    got = dense.prompt_attend(q.cuda(), k.cuda(), v.cuda(), scale=scale, **kw)
+    at = torch.zeros(q.numel() + 8, dtype=q.dtype, device="cuda")[8 if aligned else 1:][:q.numel()].view(q.shape)
+    got = dense.prompt_attend(at.copy_(q), k.cuda(), v.cuda(), scale=scale)
     tile += k.shape[0] * 2.0 ** -126
     o, size, terms = prompt(q, k, v, [q.shape[0]], [k.shape[0]], scale)
     delta = U * ((q.shape[2] + 2) * terms + k.shape[0]) + 2.0 ** -22
@@ -117,8 +119,18 @@ def test_rows_that_see_nothing_of_a_tile(dtype, aligned):
     v = torch.rand(n, 1, 64, generator=gen(33))
     v[0] = 0.0
     v = v.to(dtype)
-    if not aligned:
-        flat = torch.zeros(q.numel() + 1, dtype=dtype)
-        flat[1:] = q.flatten()
-        q = flat[1:].view(q.shape)
-    check(q, k, v, WEIGHT[dtype], tile=ORDER[dtype])
+    check(q, k, v, WEIGHT[dtype], tile=ORDER[dtype], aligned=aligned)
+
+
+# In two parts a weight is off by the square of a rounding: 2^-16 in bf16; in fp16 the second part
+# leaves at most 2^-25 as above.
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("heads,kv_heads,dim,n,m", [(4, 2, 64, 130, 130), (4, 1, 128, 70, 500), (2, 1, 256, 200, 200), (2, 2, 128, 4, 3000)])
+def test_weights_keep_their_bits(heads, kv_heads, dim, n, m, dtype):
+    r = gen(34)
+    q, k, v = (torch.randn(t, h, dim, generator=r).to(dtype) for t, h in ((n, heads), (m, kv_heads), (m, kv_heads)))
+    check(q, k, v, HALF[dtype] ** 2, scale=dim ** -0.5, tile=ORDER[dtype])
+    # Signs that nearly cancel: outputs are small beside their values.
+    v = (v.abs() + 4).to(dtype)
+    v[1::2] *= -1
+    check(q, k, v, HALF[dtype] ** 2, scale=dim ** -0.5, tile=ORDER[dtype])
