@@ -63,9 +63,9 @@ template <typename T> __device__ __forceinline__ T* output_row(const PromptArgs&
 // multiplied), eight prompts of 1 to 1531 tokens (20 heads of 128 over four) 112 us in fp16
 // and 105 in bf16; in fp32 2048 tokens of 16 heads 141 us at dim 64, 264 at 128 (four key
 // heads), 550 at 256 (two). 128 rows share what a tile of keys takes to load. The running
-// maximum is let stay while no weight would pass 2^8, which saves rescaling the sums at nearly every tile. Steps of both products are interleaved with the
-// LDS reads of the one after next (schedule), and matrix work goes before other
-// wavefronts' vector work.
+// maximum is let stay while no weight would pass 2^8, which saves rescaling the sums at
+// nearly every tile. Steps of both products are interleaved with the LDS reads of the one
+// after next (schedule), and matrix work goes before other wavefronts' vector work.
 // Keys of a tile, and workgroups a compute unit that the registers are for.
 template <typename T, int D> constexpr int kKeys = sizeof(T) == 4 || D > 64 ? 32 : 64;
 template <typename T, int D> constexpr int kResident = D * sizeof(T) > 512 ? 1 : sizeof(T) == 2 && D == 128 ? 3 : 2;
