@@ -229,7 +229,7 @@ template <typename T> __device__ __forceinline__ T* draft_row(const TreeArgs& A,
 // parts of P, next to as much time of the matrix cores; memory is read at a
 // quarter to a half of its rate. 24 sequences of up to 8192 tokens with 1 to 61 drafts (16 heads
 // of 128, four of the cache, fp16): 60 us and 6.1 for the join; 32 equal ones with 64 drafts in
-// bf16: 178 us, 770 TFLOP/s. One of 32768 tokens with 15 drafts (16 heads of 256, two of the
+// bf16: 240 us. One of 32768 tokens with 15 drafts (16 heads of 256, two of the
 // cache, bf16): 28.9 us, of which 8 pass until the first tile is there, 3 with each of four
 // tiles, 4 with the join in LDS and 2 with writing 17 MB of parts, and 5.9 for their join.
 //
@@ -240,13 +240,15 @@ template <typename T> __device__ __forceinline__ T* draft_row(const TreeArgs& A,
 // the weights of tokens 16 s + 8 h .. 16 s + 8 h + 7, eight bytes of V.
 //
 // Q is an exact operand (fp32: three bf16 parts); P 2^e is in bf16 parts, of which there
-// are as many as keep it well below the output's own rounding but for bf16, where
-// half a step of independent weights is no more than that.
+// are as many as keep it well below the output's own rounding: two for 16-bit types,
+// as in kv_attend, three for fp32. (In bf16 one made outputs off by 2^-8 of the weighted
+// values' size; the ragged batch above took 53.6 us so and takes 62, one stream of 32768
+// tokens and 15 drafts 34.9 and 39.6.)
 template <typename T> struct Row;
 template <> struct Row<__bf16> {   // (kFold: K's powers of two go into its operand)
   static constexpr bool kFold = true;
   typedef bf16x8 frag;
-  static constexpr int kQ = 1, kP = 1;
+  static constexpr int kQ = 1, kP = 2;
 };
 template <> struct Row<_Float16> {
   static constexpr bool kFold = false;

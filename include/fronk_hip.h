@@ -458,8 +458,8 @@ int fr_hip_prompt_attend(const fr_hip_prompt *req, void *workspace, size_t bytes
  * fr_hip_kv_attend: softmax(scale q k) v per query head, pages by table, a page
  * outside the cache counts as not seen. o shares no memory with an input.
  * What is held of drafts that no draft sees may be anything. A draft held with infinity or
- * NaN makes the drafts that see it NaN, and no others. bf16 outputs: weights are rounded to
- * bf16, their sums are not (fp16: to 2^-16, fp32: to 2^-23). How a context is cut, and so
+ * NaN makes the drafts that see it NaN, and no others. Weights are held to 2^-16 of them
+ * (fp32: to 2^-23), their sums in fp32. How a context is cut, and so
  * the order of sums, follows the lengths of all sequences of the call. Caches of 2^32 - 1
  * or more blocks of 16 tokens and a head are not supported. */
 typedef struct {
