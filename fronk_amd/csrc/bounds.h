@@ -47,4 +47,18 @@ FRONK_BOTH uint32_t bad_sequence(int32_t slot, uint32_t slots, int32_t first, in
   return bad;
 }
 
+// A bound on the tokens of a stretch: `part` of the longest sequence's (a multiple of 64), 256 or
+// more. A part of 1 is all of it, which leaves every sequence whole: not by way of a float, which from
+// 2^30 on may be less.
+FRONK_BOTH uint32_t stretch_bound(uint32_t longest, float part) {
+  const uint32_t n = part < 1.f ? ((uint32_t)((float)longest * part) + 63) & ~63u : longest;
+  return n > 256 ? n : 256;
+}
+// Stretches of at most `bound` tokens, at least one; reciprocal: 2^32 - 1 by it, rounded down.
+FRONK_BOTH uint32_t stretches(uint32_t length, uint32_t bound, uint32_t reciprocal) {
+  uint32_t n = (uint32_t)(((uint64_t)length * reciprocal) >> 32);   // this, one or two more
+  while (n * bound < length) ++n;
+  return n ? n : 1;
+}
+
 }  // namespace fronk

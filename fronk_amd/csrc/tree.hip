@@ -153,15 +153,10 @@ __device__ __forceinline__ Place plan(const TreeArgs& A, uint32_t* lds) {
   }
   __syncthreads();
   uint32_t chunk = ((max(found[1], 1u) + 63) & ~63u);
-  // Stretches of a sequence, of at most `chunk` tokens.
-  auto count = [&](uint32_t s, uint32_t chunk, uint32_t reciprocal) {
-    uint32_t q = __umulhi(length[s], reciprocal);   // tokens by chunk: this, one or two more
-    while (q * chunk < length[s]) ++q;
-    return q ? q : 1;
-  };
+  auto count = [&](uint32_t s, uint32_t chunk, uint32_t reciprocal) { return fronk::stretches(length[s], chunk, reciprocal); };
   if (A.slots) {
     // (2^(7/8) and so on; 64 of these: 2^7.9 stretches of the longest)
-    const uint32_t mine = max(((uint32_t)((float)chunk * __builtin_amdgcn_exp2f(lane * -.125f)) + 63) & ~63u, 256u);
+    const uint32_t mine = fronk::stretch_bound(chunk, lane ? __builtin_amdgcn_exp2f(lane * -.125f) : 1.f);
     const uint32_t reciprocal = 0xffffffffu / mine;
     uint32_t total = 0;
     for (uint32_t s = wave; s < A.sequences; s += W)
