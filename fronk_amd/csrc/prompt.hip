@@ -28,16 +28,25 @@ struct Prompt {
   bool bad;
 };
 __device__ __forceinline__ Prompt prompt_of(const PromptArgs& A, uint32_t seq) {
-  int32_t q0 = seq * A.max_tokens, q1 = q0 + A.max_tokens, k0 = seq * A.max_context, k1 = k0 + A.max_context, before = 0;
+  int32_t q0 = seq * A.max_tokens, q1 = q0 + A.max_tokens, k0 = seq * A.max_context, k1 = k0 + A.max_context;
+  // Whether an offset before a sequence's is above it.
+  auto falls = [&](const int32_t* offsets, int32_t own) {
+    int32_t most = 0;
+    for (uint32_t s = threadIdx.x; s < seq; s += blockDim.x) most = max(most, offsets[s]);
+    return most > own;
+  };
+  bool bad = false;
   if (A.offsets) {
     q0 = same(A.offsets[seq]), q1 = same(A.offsets[seq + 1]);
-    for (uint32_t s = threadIdx.x; s < seq; s += blockDim.x) before = max(before, A.offsets[s]);
+    bad = falls(A.offsets, q0);
     if (!A.k_offsets) k0 = q0, k1 = q1;
   }
-  if (A.k_offsets) k0 = same(A.k_offsets[seq]), k1 = same(A.k_offsets[seq + 1]);
-  const uint32_t bad = fronk::bad_sequence(0, 1, q0, q1, A.tokens, A.max_tokens) |
-                       fronk::bad_sequence(0, 1, k0, k1, A.k_tokens, A.max_context);
-  return Prompt{q0, k0, (uint32_t)(q1 - q0), (uint32_t)(k1 - k0), __syncthreads_or(before > q0 || bad) != 0};
+  if (A.k_offsets) {
+    k0 = same(A.k_offsets[seq]), k1 = same(A.k_offsets[seq + 1]);
+    bad |= falls(A.k_offsets, k0);
+  }
+  bad |= (fronk::bad_sequence(0, 1, q0, q1, A.tokens, A.max_tokens) | fronk::bad_sequence(0, 1, k0, k1, A.k_tokens, A.max_context)) != 0;
+  return Prompt{q0, k0, (uint32_t)(q1 - q0), (uint32_t)(k1 - k0), __syncthreads_or(bad) != 0};
 }
 template <typename T> __device__ __forceinline__ T* output_row(const PromptArgs& A, const Prompt& P, uint32_t head, uint32_t row) {
   return static_cast<T*>(A.o) + (int64_t)(P.q0 + row / A.per) * A.o_token + (int64_t)(head * A.per + row % A.per) * A.o_head;

@@ -424,9 +424,9 @@ int fr_hip_rotate(const fr_hip_rotary *req, void *stream);
  * k_offsets[i] .. k_offsets[i+1]-1, at most max_context; its queries are the last of its
  * keys: query t of n, of m keys, sees keys 0 .. m - n + t. One that sees nothing has
  * zeros. offsets NULL: max_tokens queries each; k_offsets NULL: the keys are the queries'
- * own (without offsets, max_context of them each). Offsets do not go down: a sequence that
- * begins below an offset before it is bad, as is one that ends below its start, is too long or
- * out of range, and a bad one's outputs are left as they were. max_tokens and max_context
+ * own (without offsets, max_context of them each). Neither offsets nor k_offsets go down: a
+ * sequence whose queries or keys begin below an offset before theirs is bad, as is one that ends below
+ * its start, is too long or out of range, and a bad one's outputs are left as they were. max_tokens and max_context
  * bound the launch. kv_heads divides heads, at most 64 query heads for each; dim 64, 128
  * or 256. o shares no memory with an input.
  * A value (v) that is not finite makes its dim not finite (NaN or infinity) in the queries that
