@@ -91,9 +91,9 @@ __global__ __launch_bounds__(256) void kv_copy(CopyArgs A) {
   const Cache& C = A.cache;
   const uint32_t entry = blockIdx.x / A.parts, part = blockIdx.x % A.parts;
   const int32_t source = A.source[entry], target = A.target[entry];
-  if (source == -1 || target == -1) return;
-  if (!fronk::page_there(source, C.pages) || !fronk::page_there(target, C.pages)) {
-    if (A.status && threadIdx.x == 0) atomicOr(A.status, FR_HIP_BAD_PAGE);
+  const bool from = fronk::page_there(source, C.pages), to = fronk::page_there(target, C.pages);
+  if (!from || !to) {   // (-1: skipped)
+    if (((!from && source != -1) || (!to && target != -1)) && A.status && threadIdx.x == 0) atomicOr(A.status, FR_HIP_BAD_PAGE);
     return;
   }
   const uint32_t exps = C.heads * C.page / 16, codes = exps * C.dim;   // of 16 bytes

@@ -255,12 +255,12 @@ def kv_attend_tree(cache, q, tree, table, lengths, *, offsets=None, max_tokens=N
 def kv_move(cache, source, target, *, status=None):
     """Writes what is held at slots source to slots target, bit for bit. Both int32
     [groups, moves] or [moves], up to 64 moves; a group's are all read before any is
-    written, so that accepted drafts can be moved together. -1 in either: skipped.
-    Targets are distinct, and no group's target is another group's source."""
+    written, so that accepted drafts can be moved together. -1 in either: skipped (what is
+    out of range beside it is still bad). Targets are distinct, and no group's target is another group's source."""
     _attention.kv_move(cache, source, target, status)
 
 
 def kv_copy(cache, source, target, *, status=None):
-    """Copies pages source to pages target (int32 [count]); -1 in either: skipped.
+    """Copies pages source to pages target (int32 [count]); -1 in either: skipped, as above.
     Targets are distinct, and none is the source of another."""
     _attention.kv_copy(cache, source, target, status)

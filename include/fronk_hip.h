@@ -478,8 +478,8 @@ int fr_hip_kv_attend_tree(const fr_hip_kv_tree *req, void *workspace, size_t byt
 
 /* What slot source[g * moves + i] holds is written to slot target[g * moves + i], bit
  * for bit, each group's as if all of it were read before any is written (accepted drafts
- * moved together). -1 in either: that one is skipped. Targets are distinct, and no
- * group's target is another's source. moves up to 64. */
+ * moved together). -1 in either: that one is skipped; what is out of range is bad also
+ * beside it. Targets are distinct, and no group's target is another's source. moves up to 64. */
 typedef struct {
     fr_hip_kv_cache cache;
     unsigned groups, moves;
@@ -487,7 +487,7 @@ typedef struct {
     uint32_t *status;
 } fr_hip_kv_moves;
 int fr_hip_kv_move(const fr_hip_kv_moves *req, void *stream);
-/* Pages source[i] copied to pages target[i]; -1 in either: skipped. Targets are
+/* Pages source[i] copied to pages target[i]; -1 in either: skipped, as above. Targets are
  * distinct, and none is the source of another. */
 typedef struct {
     fr_hip_kv_cache cache;
