@@ -15,6 +15,7 @@
 #include <string>
 
 #include "fronk_hip.h"
+#include "overlap.h"
 
 namespace {
 
@@ -78,12 +79,19 @@ at::Tensor make(const at::Tensor* out, at::IntArrayRef shape, const at::Tensor& 
   if (at::has_internal_overlap(*out) == at::MemOverlap::Yes) refuse("out has places of its own for all elements");
   return *out;
 }
+// A tensor's places: within its storage where another one has the same (which may be of no
+// memory yet), by address otherwise.
+fronk::Strided strided(const at::Tensor& t, bool within) {
+  const int64_t size = (int64_t)t.element_size();
+  const uintptr_t at = within ? (uintptr_t)(t.storage_offset() * size) : (uintptr_t)t.data_ptr();
+  return {at, size, t.dim(), t.sizes().data(), t.strides().data()};
+}
 // An output whose places are also read, by other workgroups than write them.
 void apart(const at::Tensor* out, const at::Tensor& in, const char* name) {
   if (!out || !out->numel() || !in.numel()) return;
-  const auto both = at::get_overlap_status(*out, in);
-  if (both == at::MemOverlapStatus::Full || both == at::MemOverlapStatus::Partial || out->data_ptr() == in.data_ptr())
-    refuse(std::string("out shares memory with ") + name);
+  const bool one = out->is_alias_of(in);
+  if (!one && (!out->data_ptr() || !in.data_ptr())) return;
+  if (fronk::share(strided(*out, one), strided(in, one))) refuse(std::string("out shares memory with ") + name);
 }
 
 // The engine is one GPU's: on another one's tensors it would work out of order with
