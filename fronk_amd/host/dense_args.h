@@ -5,7 +5,6 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <ATen/ATen.h>
-#include <ATen/MemoryOverlap.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/core/GradMode.h>
 
@@ -73,18 +72,18 @@ unsigned u32(int64_t n, const char* name) {
   return (unsigned)n;
 }
 
-at::Tensor make(const at::Tensor* out, at::IntArrayRef shape, const at::Tensor& as, const char* what) {
-  if (!out) return at::empty(shape, as.options());
-  if (out->sizes() != shape || out->scalar_type() != as.scalar_type() || out->device() != as.device()) refuse(what);
-  if (at::has_internal_overlap(*out) == at::MemOverlap::Yes) refuse("out has places of its own for all elements");
-  return *out;
-}
 // A tensor's places: within its storage where another one has the same (which may be of no
 // memory yet), by address otherwise.
 fronk::Strided strided(const at::Tensor& t, bool within) {
   const int64_t size = (int64_t)t.element_size();
   const uintptr_t at = within ? (uintptr_t)(t.storage_offset() * size) : (uintptr_t)t.data_ptr();
   return {at, size, t.dim(), t.sizes().data(), t.strides().data()};
+}
+at::Tensor make(const at::Tensor* out, at::IntArrayRef shape, const at::Tensor& as, const char* what) {
+  if (!out) return at::empty(shape, as.options());
+  if (out->sizes() != shape || out->scalar_type() != as.scalar_type() || out->device() != as.device()) refuse(what);
+  if (out->numel() && fronk::shares(strided(*out, true))) refuse("out has places of its own for all elements");
+  return *out;
 }
 // An output whose places are also read, by other workgroups than write them.
 void apart(const at::Tensor* out, const at::Tensor& in, const char* name) {

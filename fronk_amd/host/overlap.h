@@ -1,5 +1,5 @@
-// overlap.h - whether two strided arrays share memory, exactly, in plain C++ so that it is
-// tested on the host.
+// overlap.h - whether two strided arrays, or two elements of one, share memory, exactly, in
+// plain C++ so that it is tested on the host.
 //
 // An array's bytes are its address, plus multiples of its strides, plus 0 .. size - 1 of an
 // element. Two share one where their addresses' difference d and some multiples t, within
@@ -53,17 +53,17 @@ inline int64_t runs(const Strided& a, int sign, Axes* out) {
   return run;
 }
 
-// Whether some multiples of axes i and on bring d to within low .. high. `left` steps are taken at most;
-// without an answer by then it is yes.
-inline bool reaches(const Axes& a, int i, int64_t d, int64_t low, int64_t high, int64_t* left) {
-  if (i == a.n) return d >= low && d <= high;
+// Whether some multiples of axes i and on bring d to within low .. high; not all 0, unless `moved`. `left`
+// steps are taken at most; without an answer by then it is yes.
+inline bool reaches(const Axes& a, int i, int64_t d, int64_t low, int64_t high, bool moved, int64_t* left) {
+  if (i == a.n) return moved && d >= low && d <= high;
   int64_t least = 0, most = 0;   // what the axes behind this one can add
   for (int k = i + 1; k < a.n; ++k) least += a.axis[k].stride * a.axis[k].low, most += a.axis[k].stride * a.axis[k].high;
   auto floor_div = [](int64_t x, int64_t y) { return x / y - (x % y < 0); };
   const int64_t s = a.axis[i].stride;
   const int64_t first = std::max(a.axis[i].low, -floor_div(d + most - low, s)), last = std::min(a.axis[i].high, floor_div(high - least - d, s));
   for (int64_t t = first; t <= last; ++t)
-    if (--*left < 0 || reaches(a, i + 1, d + s * t, low, high, left)) return true;
+    if (--*left < 0 || reaches(a, i + 1, d + s * t, low, high, moved || t, left)) return true;
   return false;
 }
 
@@ -81,7 +81,20 @@ inline bool share(const Strided& a, const Strided& b) {
   }
   axes.n = n;
   int64_t left = 1 << 20;
-  return reaches(axes, 0, (int64_t)(b.at - a.at), 1 - run_b, run_a - 1, &left);
+  return reaches(axes, 0, (int64_t)(b.at - a.at), 1 - run_b, run_a - 1, true, &left);
+}
+
+// Whether two of an array's elements share memory.
+inline bool shares(const Strided& a) {
+  if (a.axes > kAxes) return true;
+  for (int64_t i = 0; i < a.axes; ++i)
+    if (a.sizes[i] > 1 && !a.strides[i]) return true;
+  Axes axes;
+  const int64_t run = runs(a, 1, &axes);
+  std::sort(axes.axis, axes.axis + axes.n, [](const Axis& x, const Axis& y) { return x.stride > y.stride; });
+  for (int i = 0; i < axes.n; ++i) axes.axis[i].low = -axes.axis[i].high;
+  int64_t left = 1 << 20;
+  return reaches(axes, 0, 0, 1 - run, run - 1, false, &left);
 }
 
 }  // namespace fronk

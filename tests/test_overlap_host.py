@@ -17,6 +17,7 @@ typedef const int64_t* L;
 extern "C" int share(int64_t at, int64_t e, int64_t n, L sizes, L strides, int64_t at2, int64_t e2, int64_t n2, L sizes2, L strides2) {
   return fronk::share({(uintptr_t)at, e, n, sizes, strides}, {(uintptr_t)at2, e2, n2, sizes2, strides2});
 }
+extern "C" int shares(int64_t at, int64_t e, int64_t n, L sizes, L strides) { return fronk::shares({(uintptr_t)at, e, n, sizes, strides}); }
 '''
 
 
@@ -41,6 +42,10 @@ def share(shim, a, b):
     return bool(shim.share(*args))
 
 
+def shares(shim, at, element, sizes, strides):
+    return bool(shim.shares(C.c_int64(at), C.c_int64(element), C.c_int64(len(sizes)), longs(sizes), longs(strides)))
+
+
 def places(at, element, sizes, strides):
     out = [at]
     for n, s in zip(sizes, strides):
@@ -60,6 +65,24 @@ def test_against_all_addresses(shim):
         seen[want] += 1
         assert share(shim, *arrays) == share(shim, *arrays[::-1]) == want, arrays
     assert min(seen) > 1000
+
+
+def test_elements_of_one_array(shim):
+    r, seen = random.Random(2), [0, 0]
+    for _ in range(6000):
+        n = r.randint(0, 4)
+        strides = [r.choice([0, 1, 2, 3, 4, 5, 6, 8, 10, 12, 15, 20, 24, 40, 60, 120]) for _ in range(n)]
+        a = (r.randint(0, 9), r.choice([1, 2, 4, 8]), [r.randint(1, 5) for _ in range(n)], strides)
+        count = a[1]
+        for x in a[2]:
+            count *= x
+        want = len(places(*a)) < count
+        seen[want] += 1
+        assert shares(shim, *a) == want, a
+    assert min(seen) > 1000
+    rows = lambda each, step: (1 << 40, 2, [100000, 20, 128], [each, step, 1])
+    assert not shares(shim, *rows(24 * 128, 128)) and not shares(shim, *rows(128, 100000 * 128))
+    assert shares(shim, *rows(19 * 128, 128)) and shares(shim, *rows(24 * 128, 127)) and shares(shim, *rows(128, 128))
 
 
 def test_rows_of_one_projection(shim):
@@ -123,3 +146,23 @@ with mode:
 
 def test_views_of_a_projections_rows(folder):   # noqa: F811
     run(folder, OUTPUTS.replace("{body}", ""))
+
+
+def test_outputs_whose_elements_share_memory(folder):   # noqa: F811
+    run(folder, """
+mode = FakeTensorMode()
+with mode:
+    b = torch.empty(4096, dtype=torch.bfloat16, device="cuda:0")
+    x = lambda: torch.empty(9, 2, 64, dtype=torch.bfloat16, device="cuda:0")
+    for strides in ((64, 64, 1), (127, 64, 1), (128, 63, 1), (0, 64, 1), (64, 128, 1)):
+        try:
+            _attention.prompt_attend(x(), x(), x(), None, None, None, None, None, b.as_strided((9, 2, 64), strides), None)
+        except ValueError as e:
+            assert "places of its own" in str(e), str(e)
+        else:
+            raise AssertionError(strides)
+    assert calls.value == 0
+    for strides in ((128, 64, 1), (64, 640, 1), (192, 64, 1), (129, 65, 1)):
+        _attention.prompt_attend(x(), x(), x(), None, None, None, None, None, b.as_strided((9, 2, 64), strides), None)
+    assert calls.value == 4
+""")
