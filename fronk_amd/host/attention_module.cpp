@@ -102,6 +102,8 @@ PyObject* prompt_attend(PyObject*, Args a, Py_ssize_t n) {
     const at::Tensor o = make(out, q.sizes(), q, "out is like q");
     row(q, "q"), row(k, "k"), row(v, "v"), row(o, "out");
     apart(out, q, "q"), apart(out, k, "k"), apart(out, v, "v");
+    if (offsets) apart(out, *offsets, "offsets");
+    if (k_offsets) apart(out, *k_offsets, "k_offsets");
     r.tokens = u32(tokens, "tokens"), r.k_tokens = u32(k_tokens, "k_tokens");
     r.heads = u32(q.size(1), "heads"), r.kv_heads = u32(k.size(1), "kv_heads"), r.dim = u32(dim, "dim");
     r.scale = (float)(a[7] == Py_None ? 1.0 / sqrt((double)dim) : number(a[7]));
@@ -148,7 +150,8 @@ PyObject* kv_attend_tree(PyObject*, Args a, Py_ssize_t n) {
     r.length = ints<const int32_t*>(&lengths, sequences, q, "lengths");
     r.status = ints<uint32_t*>(status, 1, q, "status");
     row(q, "q"), row(o, "out");
-    apart(out, q, "q");
+    apart(out, q, "q"), apart(out, tree, "tree"), apart(out, table, "table"), apart(out, lengths, "lengths");
+    if (offsets) apart(out, *offsets, "offsets");
     for (int i = 0; i < 4; ++i) apart(out, THPVariable_Unpack(PyTuple_GET_ITEM(a[0], i)), "the cache");
     if (!sequences || !tokens) return THPVariable_Wrap(o);
     r.sequences = u32(sequences, "sequences"), r.tokens = u32(tokens, "tokens"), r.max_tokens = u32(longest, "max_tokens");

@@ -166,3 +166,56 @@ with mode:
         _attention.prompt_attend(x(), x(), x(), None, None, None, None, None, b.as_strided((9, 2, 64), strides), None)
     assert calls.value == 4
 """)
+
+
+WHOLE = """
+mode = FakeTensorMode()
+
+
+def each(name, make, call, names):
+    # All inputs apart from out, then each in turn in its first bytes, and in its last.
+    with mode:
+        for victim in [None] + names:
+            for end in (False, True):
+                args = make()
+                size = 4 * 9 * 2 * 64
+                if victim is not None:
+                    t = args[victim]
+                    flat = torch.empty(2 * size + t.numel() * t.element_size(), dtype=torch.uint8, device="cuda:0")
+                    at = 0 if end else size - t.element_size()
+                    args[victim] = flat[at:at + t.numel() * t.element_size()].view(t.dtype).view(t.shape)
+                    first = (t.numel() - 1) * t.element_size() // 8 * 8 if end else 0
+                    out = flat[first:first + size].view(torch.float32).view(9, 2, 64)
+                else:
+                    out = torch.empty(9, 2, 64, device="cuda:0")
+                n = calls.value
+                try:
+                    call(args, out)
+                except ValueError as e:
+                    assert victim is not None and "out shares memory" in str(e), (name, victim, end, str(e))
+                else:
+                    assert victim is None and calls.value == n + 1, (name, victim, end)
+
+
+def t(*shape, dtype=torch.float32):
+    return torch.empty(*shape, dtype=dtype, device="cuda:0")
+
+
+i32, i64, u8 = torch.int32, torch.int64, torch.uint8
+{cases}
+"""
+
+
+def test_outputs_over_what_is_looked_up(folder):   # noqa: F811
+    """Offsets, tables, words and lengths count as inputs as q does: other workgroups, and the join of a context's
+    stretches, read them when some outputs are written."""
+    run(folder, WHOLE.replace("{cases}", """
+each("prompt", lambda: dict(q=t(9, 2, 64), k=t(12, 1, 64), v=t(12, 1, 64), offsets=t(3, dtype=i32), k_offsets=t(3, dtype=i32)),
+     lambda a, out: _attention.prompt_attend(a["q"], a["k"], a["v"], a["offsets"], a["k_offsets"], 9, 12, None, out, None),
+     ["q", "k", "v", "offsets", "k_offsets"])
+each("tree", lambda: dict(q=t(9, 2, 64), tree=t(9, dtype=i64), table=t(2, 3, dtype=i32), lengths=t(2, dtype=i32), offsets=t(3, dtype=i32),
+                          k=t(2, 1, 16, 64, dtype=u8), v=t(2, 1, 1, 64, 16, dtype=u8), ke=t(2, 1, 16, dtype=u8), ve=t(2, 1, 16, dtype=u8)),
+     lambda a, out: _attention.kv_attend_tree((a["k"], a["v"], a["ke"], a["ve"]), a["q"], a["tree"], a["table"], a["lengths"], a["offsets"],
+                                              None, None, None, out, None),
+     ["q", "tree", "table", "lengths", "offsets", "k", "v", "ke", "ve"])
+"""))
