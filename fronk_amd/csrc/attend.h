@@ -167,9 +167,9 @@ __device__ __forceinline__ float4v join_many(const float* part_o, const float* p
   for (uint32_t k = 1; k < G; ++k) x += parts[k][c];   // (by all, for the first group)
   return x;
 }
-// Rows below which each has a workgroup (join_many). Whole calls, us, by a workgroup each and by
-// D / 4 lanes each: 512 rows of 64 stretches 26 and 36, 1024 of them 37 and 44, 2048 of 32
-// 46 and 46, 4096 of 16 64 and 58, 8192 of eight 106 and 87.
+// Rows below which each has a workgroup (join_many). Whole calls of trees (bf16, dim 128), us, by a
+// workgroup each and by D / 4 lanes each: 512 rows of 64 stretches 36 and 42, 1024 of 32 48 and
+// 53, 2048 of 16 49 and 48, 4096 of eight 54 and 47, 8192 of four 99 and 79.
 constexpr uint64_t kJoinRows = 2048;
 
 }  // namespace

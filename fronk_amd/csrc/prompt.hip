@@ -67,14 +67,18 @@ template <typename T> __device__ __forceinline__ T* output_row(const PromptArgs&
 // fp32: v_mfma_f32_32x32x2, exact products.
 //
 // Bound by the matrix cores and by the vector work beside them (per 32 x 32 scores a
-// maximum, 16 exponentials a lane, their sum and P's parts): 4096 tokens of 16 heads of
-// 256 over two key heads, bf16, take 213 us or 640 TFLOP/s of what is seen (960 of what is
-// multiplied), eight prompts of 1 to 1531 tokens (20 heads of 128 over four) 112 us in fp16
-// and 105 in bf16; in fp32 2048 tokens of 16 heads 141 us at dim 64, 264 at 128 (four key
-// heads), 550 at 256 (two). 128 rows share what a tile of keys takes to load. The running
-// maximum is let stay while no weight would pass 2^8, which saves rescaling the sums at
-// nearly every tile. Steps of both products are interleaved with the LDS reads of the one
-// after next (schedule), and matrix work goes before other wavefronts' vector work.
+// maximum, 16 exponentials a lane, their sum and P's parts), which overlap in part: 4096
+// tokens of 16 heads of 256 over two key heads, bf16, take 211 to 245 us from run to run, at
+// 213 640 TFLOP/s of what is seen and 960 of what is multiplied, and have the matrix cores
+// busy for 60 % of the cycles and the vector units for 35; at dim 128 it is 43 to 53 % and 52
+// to 56. Eight prompts of 1 to 1531 tokens (20 heads of 128 over four) 112 us in fp16 and 105 in
+// bf16; in fp32 2048 tokens of 16 heads 141 us at dim 64, 264 at 128 (four key heads), 550 at
+// 256 (two). 128 rows share what a tile of keys takes to load. The running maximum is let
+// stay while no weight would pass 2^8, which saves rescaling the sums at nearly every tile.
+// Steps of both products are interleaved with the LDS reads of the one after next
+// (schedule), and matrix work goes before other wavefronts' vector work. One to three
+// registers of the 16-bit forms at dims 128 and 256 are in scratch.
+//
 // Keys of a tile, and workgroups a compute unit that the registers are for.
 template <typename T, int D> constexpr int kKeys = sizeof(T) == 4 || D > 64 ? 32 : 64;
 template <typename T, int D> constexpr int kResident = D * sizeof(T) > 512 ? 1 : sizeof(T) == 2 && D == 128 ? 3 : 2;
@@ -449,10 +453,10 @@ PromptCut prompt_cut(const fr_hip_prompt* r) {
   const uint32_t context = r->max_context < r->k_tokens ? r->max_context : r->k_tokens;
   c.blocks = (uint32_t)(((uint64_t)tokens * (r->heads / r->kv_heads) + R - 1) / R);
   c.items = (uint64_t)c.blocks * r->sequences * r->kv_heads;
-  // Two workgroups for each of 256 compute units, at dim 256 one, which is what runs at once;
-  // none with less than 256 keys. 512 tokens over 8192 keys, 32 heads of 128 over four: 86 us
-  // with the join of four stretches, 177 in one, 106 in two, 90 in six; 128 tokens of 16 heads of
-  // 256 over two: 44 with one workgroup a unit, 57 with two, 53 with a half.
+  // Two workgroups for each of 256 compute units, at dim 256 one (two fit a unit there too, but their
+  // parts are twice the size); none with less than 256 keys. 512 tokens over 8192 keys, 32 heads of 128
+  // over four, bf16: 118 us with the join of four stretches, 227 in one, 140 in two, 119 in six; 128
+  // tokens over them of 16 heads of 256 over two: 50 with one workgroup a unit, 62 with two, 60 with a half.
   const uint64_t want = c.items ? (r->dim == 256 ? 1 : 2) * kUnits / c.items : 1, most = (context + 255) / 256;
   uint64_t n = want < most ? want : most;
   n = n < 1 ? 1 : n > 64 ? 64 : n;

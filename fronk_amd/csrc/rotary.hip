@@ -20,15 +20,16 @@ struct RotaryArgs {
 
 // One workgroup: `each` tokens and `at_once` of their heads (q's, then k's). First the
 // tokens' cosines and sines, once for all heads: the angle in turns is formed in 64
-// bits and brought to half a turn to either side of zero, so that a position of any
-// size costs a cosine no more than fp32's rounding. Then one pass over the heads, V
-// elements (16 bytes) a step, or single ones where addresses or sizes are not of
-// whole 16 bytes. What is rotated is read and written by one lane: in place is safe.
+// bits and brought to half a turn to either side of zero, which costs a cosine no more
+// than fp32's rounding for angles up to 2^27 radians (2^-51 of them beyond). Then one pass
+// over the heads, V elements (16 bytes) a step, or single ones where addresses or sizes
+// are not of whole 16 bytes. What is rotated is read and written by one lane: in place is safe.
 // Results are rounded once, from fp32.
 //
 // Bound by memory: 4096 tokens of 24 interleaved heads of 128 in fp16 (50 MB) take 9.9 us,
-// 5.1 TB/s, as a large copy does. One token of 18 heads is one
-// workgroup for 3.8 us: position and frequency, the cosine, a head (5.3 with its launch).
+// 5.1 TB/s, as a large copy does, in fp32 17.2; 4096 of 24 heads of 126 in single elements
+// 53 (two divisions a step). One token of 18 heads of 256 takes two workgroups 3.9 us: position and
+// frequency, the cosine, a head (5.5 with its launch).
 template <typename T, bool INTERLEAVED, int V>
 __global__ __launch_bounds__(256) void rotary(RotaryArgs A) {
   extern __shared__ __attribute__((aligned(16))) float2v turn[];   // [each][pairs]

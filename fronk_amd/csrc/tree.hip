@@ -57,10 +57,11 @@ constexpr uint32_t kPlanBytes = (kPlanned * 6 + 8 * 64 + 4) * 4;
 // for which 64 values are tried, a lane each, and that is taken with which the workgroups,
 // in rounds of as many as run at once, end first; a workgroup's beginning and end take as
 // long as about 300 tokens, and more where two share a unit (one stream of 32768 tokens and 16
-// drafts, dim 128: 21.6 us in 256 workgroups, 25.2 in 512; of 131072 42.4 and 40.1). Work then varies by less than two between workgroups however
-// ragged the batch is: 24 sequences of 1 to 61 drafts and up to 8192 tokens (16 heads of 128,
-// four of the cache) take 63 us, with one stretch length from the host 117, 96 of them in bf16
-// 184 and 289; 32 equal ones of 1024 tokens, for which nothing is to be found, 38 and 35.
+// drafts, bf16, dim 128: 26.1 us in 256 workgroups, 27.7 in 512; of 131072 53.6 and 51.6). Work
+// then varies by less than two between workgroups however ragged the batch is: 24 sequences
+// of 1 to 61 drafts and up to 8192 tokens (16 heads of 128, four of the cache, fp16) take 63
+// us, with one stretch length from the host 117. For 32 equal ones, for which nothing is to be
+// found, it is 3 us more. 96 of 1 to 61 drafts in bf16 take 216 us.
 // Workgroups of one stretch (its row blocks) follow each other, and each die, to which
 // every eighth goes, has an eighth of the list: its L2 has the stretch for all of them.
 template <int W, int ROWS, int D>
@@ -221,12 +222,15 @@ template <typename T> __device__ __forceinline__ T* draft_row(const TreeArgs& A,
 // operand, or its scores (fp16, whose range they may leave), and to its weights.
 //
 // Bound by the vector work of making operands of the codes, masks, exponentials and
-// parts of P, next to as much time of the matrix cores; memory is read at a
-// quarter to a half of its rate. 24 sequences of up to 8192 tokens with 1 to 61 drafts (16 heads
-// of 128, four of the cache, fp16): 60 us and 6.1 for the join; 32 equal ones with 64 drafts in
-// bf16: 240 us. One of 32768 tokens with 15 drafts (16 heads of 256, two of the
-// cache, bf16): 28.9 us, of which 8 pass until the first tile is there, 3 with each of four
-// tiles, 4 with the join in LDS and 2 with writing 17 MB of parts, and 5.9 for their join.
+// parts of P, by waits between it and the matrix work, and for few tiles by beginning and
+// end; memory is read at a quarter to a half of its rate. 24 sequences of up to 8192 tokens
+// with 1 to 61 drafts (16 heads of 128, four of the cache): in fp16 60 us and 6.0 for the join,
+// the vector units busy for 44 % of the cycles and the matrix cores for 26; in bf16 60 and 6.0,
+// in fp32 81 and 6.5. 32 equal ones with 64 drafts in bf16: 240 us. One of 32768 tokens with 15 drafts
+// (16 heads of 256, two of the cache, bf16): 33.4 us and 5.7 (32 % and 19), of which 8 pass until the
+// first tile is there, 4 with each of four tiles, 4 with the join in LDS and 2 with writing 17
+// MB of parts; in fp32 86 and 5.7, as two of a unit's four SIMDs have work. One to eight registers of
+// the 16-bit forms at dim 256, and three of fp32's at dim 128 and 64 rows, are in scratch.
 //
 // K in LDS: [token][dim], chunk c of 16 codes at another place for each of eight
 // tokens, so that a read of one chunk of 32 of them goes to all banks; a lane's 16
@@ -259,8 +263,9 @@ template <> struct Row<float> {
 // Wavefronts, keys of a tile, stages, wavefronts a SIMD that the registers are for.
 // Where Q's three parts do not fit them beside the sums, Q is kept in LDS, and split
 // where it is used. Two stages: with three, one workgroup less fits a unit (32 sequences of
-// 8192 tokens, dim 128: 207 us with two, 264 with three); tiles of 32 keys instead of 64 there:
-// 217. Eight wavefronts at dim 256, as four of 512 registers each are slower (40 us for 37).
+// 8192 tokens and 64 drafts, bf16, dim 128: 240 us with two, 298 with three); tiles of 32 keys
+// instead of 64 there: 255. Eight wavefronts at dim 256, as four of 512 registers each are
+// slower (one stream of 32768 tokens 43 us for 39.5).
 template <typename T, int D> constexpr bool kTreeQInLds = D * sizeof(T) > 512;
 template <typename T, int D, int RG> constexpr int kTreeWaves = kTreeQInLds<T, D> ? 2 : D == 256 && RG > 1 ? 8 : 4;
 template <int D, int RG> constexpr int kTreeKeys = D == 256 || (D == 128 && RG == 1) ? 32 : 64;
@@ -483,7 +488,7 @@ __global__ __launch_bounds__((64 * kTreeWaves<T, D, RG>), (kTreeResident<T, D>))
       }
     }
     // Each step's operands are read while the one before it is worked on.
-    __builtin_amdgcn_s_setprio(1);   // (matrix work before other wavefronts': 4 % less at 64 rows)
+    __builtin_amdgcn_s_setprio(1);   // (matrix work before other wavefronts': 7 % less at 64 rows)
     float16v st[ST];
     // Reads at once, as many as registers are left for.
     constexpr int kK = KS == 4 ? 2 : 1, kV = D == 256 ? 2 : DT < 4 ? DT : 4;
@@ -750,14 +755,15 @@ TreeCut tree_cut(const fr_hip_kv_tree* r) {
   const uint32_t drafts = r->max_tokens < r->tokens ? r->max_tokens : r->tokens;
   const uint32_t rows = drafts * (r->heads / r->cache.heads);
   // 64 rows, or 32 where there are no more: 16 sequences of 8192 tokens with 8 drafts of four
-  // heads take 39.8 us in groups of 32 and 42.2 of 64, with 16 drafts 48.1 and 46.4, 32 of them
-  // with 64 drafts 240 and 178 (128 rows: the same to 20 % slower at 16 to 64 drafts).
+  // heads (bf16, dim 128) take 40.2 us in groups of 32 and 40.8 of 64, with 16 drafts 52.0 and 49.8, 32
+  // of them with 64 drafts 286 and 238 (128 rows: the same to 20 % slower at 16 to 64 drafts).
   c.groups = rows <= 32 ? 1 : 2;
   c.blocks = (rows + 32 * c.groups - 1) / (32 * c.groups);
   c.items = (uint64_t)c.blocks * r->sequences * r->cache.heads;
-  // Two workgroups a unit at once, one at dim 256 (16 drafts over 131072 tokens, 16 heads: two
-  // key heads of 256 60 us with one a unit and 77 with two, four of 128 42 and 40); up to
-  // three such rounds are split.
+  // Two workgroups a unit at once, one at dim 256 (16 drafts over 131072 tokens, 16 heads, bf16: two
+  // key heads of 256 84 us with one a unit and 104 with two, four of 128 50 and 47); up to
+  // three such rounds are split, and no call of more sequences than are planned: beyond, each of
+  // a sequence's blocks is one workgroup's, however long it is.
   c.at_once = kUnits * (r->cache.dim == 256 ? 1 : 2);
   const uint64_t rounds = (c.items + c.at_once - 1) / c.at_once;
   c.slots = rounds > 3 || r->sequences > kPlanned || r->max_context <= 256 ? 0 : (uint32_t)rounds * c.at_once;

@@ -18,8 +18,9 @@ under torch.no_grad() (or inference_mode), one with a forward-mode tangent alway
 A refused call raises ValueError before anything is enqueued. What only the
 device can see (offsets, slots, pages, lengths) is bounds-checked there: a bad
 entry reads nothing, leaves what it would write as it was (zeros in kv_read's,
-kv_attend's and, for lengths, kv_attend_tree's outputs) and sets its bit (BAD_*) in `status`, an int32 tensor of one
-element that the caller clears. Call once before capturing a graph.
+kv_attend's and, for lengths, kv_attend_tree's outputs) and sets its bit (BAD_*) in
+`status`, an int32 tensor of one element that the caller clears. Call once before
+capturing a graph.
 """
 import ctypes as C
 import importlib
@@ -196,7 +197,9 @@ def rotary_frequencies(dim, base=10000.0, *, factor=1.0, context=None, slow=1.0,
     long as the model's own. Without `context` (that length) all frequencies are
     divided by it. With it they are by the turns that they make in it (the published
     method YaRN): up to `slow` of them divided, from `fast` on kept, and in between
-    a ramp from the one to the other; magnitude is then 1 + ln(factor) / 10, else 1."""
+    a ramp over the turns; magnitude is then 1 + ln(factor) / 10, else 1. A model whose
+    configuration means a ramp over i, between rounded borders, has other frequencies
+    there: pass its own to rotary."""
     if dim <= 0 or dim % 2:
         raise ValueError("dim is positive and even")
     if not factor >= 1 or not fast > slow:

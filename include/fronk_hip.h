@@ -399,7 +399,7 @@ size_t fr_hip_kv_workspace(const fr_hip_kv_query *req);   /* as fr_hip_delta_wor
 int fr_hip_kv_attend(const fr_hip_kv_query *req, void *workspace, size_t bytes, void *stream);
 
 /* Rotary positions of q and k. With pair i's angle a = position * frequencies[i]
- * (radians, formed in 64 bits) and m = magnitude, its two values become
+ * (radians, formed in 64 bits: a cosine keeps fp32's accuracy to angles of 2^27) and m = magnitude, its two values become
  *     m (x cos a - y sin a),  m (x sin a + y cos a) ;
  * pair i is values i and i + pairs of a head, or 2i and 2i + 1 with
  * FR_HIP_ROTARY_INTERLEAVED. Values from 2 * pairs on stay as they are. q_out
@@ -432,7 +432,9 @@ int fr_hip_rotate(const fr_hip_rotary *req, void *stream);
  * A value (v) that is not finite makes its dim not finite (NaN or infinity) in the queries that
  * see it, and in no others; a key that is not finite may make all of theirs NaN.
  * Weights are held to 2^-16 of them in bf16, to 2^-22 in fp16 (and there 2^-25 of the largest
- * of the 32 or 64 keys around, however far they are below the row's largest), their sums in fp32. */
+ * of the 32 or 64 keys around, however far they are below the row's largest), their sums in fp32,
+ * where a row's largest weight may be 2^8 and the division comes last: in bf16 and fp32, outputs may
+ * be infinite or NaN where 2^8 |v| keys, or |q| |k| dim, passes 3.4e38. */
 typedef struct {
     unsigned sequences, tokens, k_tokens, max_tokens, max_context;
     unsigned heads, kv_heads, dim, type;
@@ -459,7 +461,8 @@ int fr_hip_prompt_attend(const fr_hip_prompt *req, void *workspace, size_t bytes
  * outside the cache counts as not seen. o shares no memory with an input.
  * What is held of drafts that no draft sees may be anything. A draft held with infinity or
  * NaN makes the drafts that see it NaN, and no others. Weights are held to 2^-16 of them
- * (fp32: to 2^-23), their sums in fp32. How a context is cut, and so
+ * (fp32: to 2^-23), their sums in fp32 (outputs may be infinite or NaN where 2^8 |v| length[i], or
+ * |q| |k| dim, passes 3.4e38). How a context is cut, and so
  * the order of sums, follows the lengths of all sequences of the call. Caches of 2^32 - 1
  * or more blocks of 16 tokens and a head are not supported. */
 typedef struct {
